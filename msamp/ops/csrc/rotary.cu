@@ -1,0 +1,161 @@
+// Rotary positions: each pair (x1, x2) of the first `part` elements of a head is turned by the angle position * freq[pair],
+//   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin     (the gradient: by the negative angle),
+// pairs (i, i + part / 2) of a head, or (2 i, 2 i + 1) when interleaved; the other elements are copied.
+//
+// The angle is taken in 64 bits, in turns, and reduced to (-1/2, 1/2] before it is rounded to 32 bits: at position 10^6 a 32-bit
+// angle is off by 0.06.  Sine and cosine belong to a token, not to a head, so a CTA computes those of its tokens once
+// (in shared memory) and takes all heads of both tensors through them.  Bound by memory: one read and one write of every head.
+#include "common.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxPart = 1024;
+
+struct RotTensor {
+  const void* x;
+  void* y;
+  int64_t x_sb, x_ss, x_sh, y_sb, y_ss, y_sh;    // element strides: batch, sequence, head; the elements of a head are adjacent
+  int heads;
+};
+struct RotParams {
+  RotTensor t[2];
+  const double* freqs;       // [part / 2], radians per position
+  const void* positions;     // int32 or int64, or null: the index in the sequence
+  int64_t p_sb, p_ss;
+  int pos64, batch, seq, dim, part, per_cta, inplace;
+  float sign;
+};
+
+template <typename T, bool INTER>
+__device__ __forceinline__ void turn_vectors(const T* x, T* y, const float2* cs, int slot, int half) {
+  constexpr int V = 16 / sizeof(T);
+  if (INTER) {
+    Bytes16 a = *reinterpret_cast<const Bytes16*>(x + slot * V), o;
+    const T* e = reinterpret_cast<const T*>(&a);
+    T* oe = reinterpret_cast<T*>(&o);
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 w = cs[(slot * V + j) / 2];
+      const float x1 = to_f32<T>(e[j]), x2 = to_f32<T>(e[j + 1]);
+      oe[j] = from_f32<T>(x1 * w.x - x2 * w.y);
+      oe[j + 1] = from_f32<T>(x2 * w.x + x1 * w.y);
+    }
+    *reinterpret_cast<Bytes16*>(y + slot * V) = o;
+  } else {
+    Bytes16 a = *reinterpret_cast<const Bytes16*>(x + slot * V), b = *reinterpret_cast<const Bytes16*>(x + half + slot * V), p, q;
+    const T *ea = reinterpret_cast<const T*>(&a), *eb = reinterpret_cast<const T*>(&b);
+    T *ep = reinterpret_cast<T*>(&p), *eq = reinterpret_cast<T*>(&q);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 w = cs[slot * V + j];
+      const float x1 = to_f32<T>(ea[j]), x2 = to_f32<T>(eb[j]);
+      ep[j] = from_f32<T>(x1 * w.x - x2 * w.y);
+      eq[j] = from_f32<T>(x2 * w.x + x1 * w.y);
+    }
+    *reinterpret_cast<Bytes16*>(y + slot * V) = p;
+    *reinterpret_cast<Bytes16*>(y + half + slot * V) = q;
+  }
+}
+
+template <typename T, bool INTER, bool VEC>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotParams p) {
+  extern __shared__ float2 s_cs[];    // [per_cta][half] cosine, signed sine
+  constexpr int V = VEC ? 16 / sizeof(T) : 1;
+  const int half = p.part / 2;
+  const int64_t tokens = (int64_t)p.batch * p.seq, t0 = (int64_t)blockIdx.x * p.per_cta;
+  const int n_tok = (int)min((int64_t)p.per_cta, tokens - t0);
+  for (int i = threadIdx.x; i < n_tok * half; i += kThreads) {
+    const int j = i / half;
+    const int64_t b = (t0 + j) / p.seq, s = (t0 + j) - b * p.seq;
+    double pos = (double)s;
+    if (p.positions) {
+      const int64_t at = b * p.p_sb + s * p.p_ss;
+      pos = p.pos64 ? (double)reinterpret_cast<const int64_t*>(p.positions)[at] : (double)reinterpret_cast<const int*>(p.positions)[at];
+    }
+    double turns = pos * p.freqs[i - j * half] * 0.15915494309189533577;    // 1 / (2 pi)
+    turns -= rint(turns);
+    float sn, cs;
+    sincospif((float)(2.0 * turns), &sn, &cs);
+    s_cs[i] = make_float2(cs, sn * p.sign);
+  }
+  __syncthreads();
+  // slots of a head: vectors (or elements) of its pairs, then of what is only copied
+  const int turn = VEC && INTER ? p.part / V : half / V;
+  const int slots = turn + (p.inplace ? 0 : (p.dim - p.part) / V);
+  const int per_tok = (p.t[0].heads + p.t[1].heads) * slots;
+  for (int i = threadIdx.x; i < n_tok * per_tok; i += kThreads) {
+    const int j = i / per_tok, r = i - j * per_tok;
+    int h = r / slots;
+    const int slot = r - h * slots;
+    const int64_t b = (t0 + j) / p.seq, s = (t0 + j) - b * p.seq;
+    const bool second = h >= p.t[0].heads;
+    const RotTensor& t = p.t[second];
+    if (second) h -= p.t[0].heads;
+    const T* x = reinterpret_cast<const T*>(t.x) + b * t.x_sb + s * t.x_ss + h * t.x_sh;
+    T* y = reinterpret_cast<T*>(t.y) + b * t.y_sb + s * t.y_ss + h * t.y_sh;
+    const float2* cs = s_cs + j * half;
+    if (slot >= turn) {
+      const int at = p.part + (slot - turn) * V;
+      if (VEC) *reinterpret_cast<Bytes16*>(y + at) = *reinterpret_cast<const Bytes16*>(x + at);
+      else     y[at] = x[at];
+    } else if (VEC) {
+      turn_vectors<T, INTER>(x, y, cs, slot, half);
+    } else {
+      const int i1 = INTER ? 2 * slot : slot, i2 = INTER ? i1 + 1 : slot + half;
+      const float x1 = to_f32<T>(x[i1]), x2 = to_f32<T>(x[i2]);
+      const float2 w = cs[slot];
+      y[i1] = from_f32<T>(x1 * w.x - x2 * w.y);
+      y[i2] = from_f32<T>(x2 * w.x + x1 * w.y);
+    }
+  }
+}
+
+}    // namespace
+
+// x0 [batch, seq, heads0, dim] -> y0 and x1 [batch, seq, heads1, dim] -> y1 (heads1 may be 0).  strides: (batch, seq, head) element strides
+// of x0, y0, x1, y1.  y may be x itself with the same strides; otherwise the two must not overlap.  p_sb, p_ss: strides of the positions.
+MSAMP_API int msamp_rotary(const void* x0, void* y0, const void* x1, void* y1, const int64_t* strides, const double* freqs, const void* positions,
+                           int pos64, int64_t p_sb, int64_t p_ss, int batch, int seq, int heads0, int heads1, int dim, int part, int interleaved,
+                           int inverse, int dtype, void* stream_) {
+  MSAMP_REQUIRE(batch >= 0 && seq >= 0 && heads0 >= 0 && heads1 >= 0, "rotary: negative size");
+  MSAMP_REQUIRE(part >= 2 && part % 2 == 0 && part <= dim && part <= kMaxPart, "rotary: part %d of a head of %d (even, at most %d)", part, dim, kMaxPart);
+  MSAMP_REQUIRE(freqs, "rotary: no frequencies");
+  if (batch == 0 || seq == 0 || heads0 + heads1 == 0) return MSAMP_OK;
+  RotParams p = {};
+  const bool in0 = heads0 == 0 || x0 == y0, in1 = heads1 == 0 || x1 == y1;
+  p.inplace = in0 && in1;
+  const void *px[2] = {x0, x1};
+  void* py[2] = {y0, y1};
+  const int heads[2] = {heads0, heads1};
+  int64_t each = 0;    // every stride and address, OR-ed: vectors need all of them to be multiples of 16 bytes
+  const int size = dtype == DT_F32 ? 4 : 2;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* s = strides + 6 * i;
+    if (heads[i] > 0) {
+      MSAMP_REQUIRE(px[i] && py[i], "rotary: null pointer");
+      if (px[i] == py[i]) MSAMP_REQUIRE(s[0] == s[3] && s[1] == s[4] && s[2] == s[5], "rotary: in place with other strides");
+      for (int k = 0; k < 6; ++k) each |= s[k] * size;
+      each |= (int64_t)(uintptr_t)px[i] | (int64_t)(uintptr_t)py[i];
+    }
+    p.t[i] = RotTensor{px[i], py[i], s[0], s[1], s[2], s[3], s[4], s[5], heads[i]};
+  }
+  p.freqs = freqs; p.positions = positions; p.pos64 = pos64; p.p_sb = p_sb; p.p_ss = p_ss;
+  p.batch = batch; p.seq = seq; p.dim = dim; p.part = part; p.sign = inverse ? -1.0f : 1.0f;
+  const int half = part / 2;
+  p.per_cta = half >= kThreads ? 1 : kThreads / half;
+  if (p.per_cta > 4) p.per_cta = 4;
+  const int64_t tokens = (int64_t)batch * seq, grid = (tokens + p.per_cta - 1) / p.per_cta;
+  MSAMP_REQUIRE(grid <= 0x7fffffff, "rotary: too many tokens");
+  const int v = 16 / size;
+  const bool vec = each % 16 == 0 && dim % v == 0 && (interleaved ? part % v == 0 : half % v == 0);
+  const int smem = p.per_cta * half * (int)sizeof(float2);
+  cudaStream_t stream = (cudaStream_t)stream_;
+  MSAMP_DISPATCH_HP(dtype, T, {
+    if (vec && interleaved)  rotary_kernel<T, true, true><<<(unsigned)grid, kThreads, smem, stream>>>(p);
+    else if (vec)            rotary_kernel<T, false, true><<<(unsigned)grid, kThreads, smem, stream>>>(p);
+    else if (interleaved)    rotary_kernel<T, true, false><<<(unsigned)grid, kThreads, smem, stream>>>(p);
+    else                     rotary_kernel<T, false, false><<<(unsigned)grid, kThreads, smem, stream>>>(p);
+  });
+  return msamp_check_launch("msamp_rotary");
+}

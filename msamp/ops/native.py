@@ -1,4 +1,5 @@
 """ctypes loader for the sm_100a kernel library."""
+import contextlib
 import ctypes
 import os
 import threading
@@ -39,6 +40,7 @@ _ARGTYPES = {
     'msamp_attention_tc_fwd': [_P] * 6 + [_I] * 4 + [_F, _I, _P],
     'msamp_attention_bwd': [_P] * 11 + [_I] * 4 + [_F, _I, _P],
     'msamp_attention_tc_bwd': [_P] * 11 + [_I] * 4 + [_F, _I, _P],
+    'msamp_rotary': [_P] * 7 + [_I, _L, _L] + [_I] * 9 + [_P],
 }
 
 
@@ -111,6 +113,16 @@ def raw_stream():
     if _raw_stream is not None and _raw_device is not None:
         return _raw_stream(_raw_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(t):
+    """Context in which the device of ``t`` is the current one (its current stream is then the one that ``raw_stream`` names)."""
+    if _raw_device is not None and t.device.index == _raw_device():
+        return _here
+    return torch.cuda.device(t.device)
 
 
 def addr(t):

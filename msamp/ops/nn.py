@@ -11,6 +11,7 @@ import torch
 import torch.nn.functional as F
 
 from msamp.ops import native
+from msamp.ops.rotary import rotary, rotary_frequencies, rotary_raw    # noqa: F401
 
 _i64x24 = ctypes.c_int64 * 24
 

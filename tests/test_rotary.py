@@ -1,0 +1,218 @@
+"""Rotary positions against the rotation in 64 bits: layouts, parts of a head, far positions, strided views, gradients, refusals.
+
+Tolerance of a value y1 = x1 cos - x2 sin: the angle in half turns is rounded to 32 bits (at most 2^-24 half turns, pi 2^-24 rad) and sine and
+cosine are good to an ulp (2^-23 of at most 1); two products and a sum round to 2^-24 each.  Together less than 2^-20 (|x1| + |x2|), and half a
+step of the output type relative to the value.
+"""
+import math
+
+import pytest
+import torch
+
+from msamp.ops import native
+from msamp.ops import nn as K
+
+CPU_GPU = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+
+
+def _exact(x, freqs, positions, interleaved, inverse=False):
+    """The rotation as a complex product in 64 bits, and |x1| + |x2| beside it."""
+    x, f = x.detach().double().cpu(), freqs.cpu()
+    r, s = f.numel(), x.shape[1]
+    pos = torch.arange(s) if positions is None else positions.cpu()
+    angle = (pos.double()[..., None] * f).expand(x.shape[0], s, r)[:, :, None] * (-1.0 if inverse else 1.0)
+    u = torch.polar(torch.ones_like(angle), angle)
+    y, size = x.clone(), torch.zeros_like(x)
+    one, two = (slice(0, 2 * r, 2), slice(1, 2 * r, 2)) if interleaved else (slice(0, r), slice(r, 2 * r))
+    w = torch.complex(x[..., one].contiguous(), x[..., two].contiguous()) * u
+    y[..., one], y[..., two] = w.real, w.imag
+    size[..., one] = size[..., two] = x[..., one].abs() + x[..., two].abs()
+    return y, size
+
+
+def _check(got, x, freqs, positions, interleaved, inverse=False):
+    want, size = _exact(x, freqs, positions, interleaved, inverse)
+    step = torch.finfo(got.dtype).eps / 2
+    tiny = torch.finfo(got.dtype).smallest_normal * step    # below the smallest normal number steps stop shrinking
+    err = (got.detach().double().cpu() - want).abs()
+    assert (err <= want.abs() * step + size * 2.0**-20 + tiny).all(), (err - want.abs() * step).max().item()
+    part = 2 * freqs.numel()
+    assert torch.equal(got[..., part:], x.detach()[..., part:])
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('dim, part', [(64, 64), (64, 16), (128, 128), (96, 96), (80, 20), (32, 2), (256, 256), (7, 6), (640, 640)])
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16, torch.bfloat16])
+def test_values_and_gradients(device, interleaved, dim, part, dtype):
+    torch.manual_seed(dim + part)
+    freqs = K.rotary_frequencies(part, device=device)
+    for batch, seq, heads, kv in ((2, 5, 4, 2), (1, 1, 3, 1), (3, 37, 2, 2)):
+        q = torch.randn(batch, seq, heads, dim, device=device).to(dtype).requires_grad_(True)
+        k = torch.randn(batch, seq, kv, dim, device=device).to(dtype).requires_grad_(True)
+        yq, yk = K.rotary(q, k, freqs, interleaved=interleaved)
+        assert yq.is_contiguous() and yk.is_contiguous() and yq.dtype == dtype
+        _check(yq, q, freqs, None, interleaved)
+        _check(yk, k, freqs, None, interleaved)
+        gq, gk = torch.randn_like(yq), torch.randn_like(yk)
+        dq, dk = torch.autograd.grad((yq, yk), (q, k), (gq, gk))
+        _check(dq, gq, freqs, None, interleaved, inverse=True)
+        _check(dk, gk, freqs, None, interleaved, inverse=True)
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('kind', [torch.int32, torch.int64])
+@pytest.mark.parametrize('shared', [False, True])
+def test_positions_far_and_negative(device, kind, shared):
+    torch.manual_seed(1)
+    freqs = K.rotary_frequencies(64, base=500000.0, device=device)
+    pos = torch.randint(-5, 10_000_000, (9, ) if shared else (2, 9), device=device, dtype=kind)
+    q = torch.randn(2, 9, 3, 64, device=device)
+    _check(K.rotary(q, None, freqs, positions=pos), q, freqs, pos, False)
+    # a column of a wider table of positions
+    wide = torch.randint(0, 1 << 20, (2, 9, 2), device=device, dtype=kind)[..., 1]
+    _check(K.rotary(q, None, freqs, positions=wide, interleaved=True), q, freqs, wide, True)
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_views_of_a_packed_projection(device, dtype):
+    """Strided heads, a start off the 16-byte grid, an expanded batch, other orders, an unused output."""
+    torch.manual_seed(2)
+    freqs = K.rotary_frequencies(32, device=device)
+    packed = torch.randn(2, 6, 8, 64, device=device).to(dtype)
+    q, k = packed[:, :, :4], packed[:, :, 4:6]
+    yq, yk = K.rotary(q, k, freqs)
+    _check(yq, q, freqs, None, False)
+    _check(yk, k, freqs, None, False)
+    off = torch.randn(2 * 6 * 4 * 64 + 3, device=device).to(dtype)[3:].view(2, 6, 4, 64)
+    _check(K.rotary(off, None, freqs), off, freqs, None, False)
+    wide = packed[:1].expand(3, 6, 8, 64)
+    _check(K.rotary(wide, None, freqs), wide, freqs, None, False)
+    heads_first = torch.randn(2, 4, 6, 64, device=device).to(dtype).transpose(1, 2)
+    _check(K.rotary(heads_first, k, freqs)[0], heads_first, freqs, None, False)
+    last_outer = torch.randn(2, 6, 64, 4, device=device).to(dtype).transpose(2, 3)
+    _check(K.rotary(last_outer, None, freqs), last_outer, freqs, None, False)
+    leaf_q, leaf_k = q.detach().clone().requires_grad_(True), k.detach().clone().requires_grad_(True)
+    yq, yk = K.rotary(leaf_q, leaf_k, freqs)
+    yk.sum().backward()    # an expanded gradient of one output
+    assert leaf_q.grad is None
+    _check(leaf_k.grad, torch.ones_like(leaf_k), freqs, None, False, inverse=True)
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('interleaved', [False, True])
+def test_in_place(device, interleaved):
+    torch.manual_seed(3)
+    freqs = K.rotary_frequencies(48, device=device)
+    for offset in (0, 1):
+        packed = torch.randn(2 * 5 * 6 * 64 + offset, device=device).bfloat16()[offset:].view(2, 5, 6, 64)
+        before = packed.clone()
+        K.rotary_raw([packed[:, :, :4]], [packed[:, :, :4]], freqs, None, interleaved, False)
+        _check(packed[:, :, :4], before[:, :, :4], freqs, None, interleaved)
+        assert torch.equal(packed[:, :, 4:], before[:, :, 4:])
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+def test_empty(device):
+    freqs = K.rotary_frequencies(8, device=device)
+    for shape in ((0, 3, 2, 8), (2, 0, 2, 8)):
+        q = torch.empty(shape, device=device, requires_grad=True)
+        y = K.rotary(q, None, freqs)
+        assert y.shape == shape
+        y.sum().backward()
+        assert q.grad.shape == shape
+
+
+def test_not_finite_values_stay_in_their_pair():
+    freqs = K.rotary_frequencies(8)
+    q = torch.randn(1, 2, 1, 8)
+    q[0, 1, 0, 2] = float('inf')
+    y = K.rotary(q, None, freqs)
+    assert torch.isfinite(y).view(-1).tolist() == [i not in (10, 14) for i in range(16)]
+
+
+def test_frequencies():
+    f = K.rotary_frequencies(8)
+    assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-15)
+    assert torch.equal(K.rotary_frequencies(8, scaling='linear', factor=4.0), f / 4.0)
+    g = K.rotary_frequencies(8, scaling='base', factor=4.0)
+    assert g[0] == 1.0 and math.isclose(g[-1].item(), f[-1].item() / 4.0, rel_tol=1e-12)
+    h = K.rotary_frequencies(64, scaling='parts', factor=8.0, trained=2048, fast=32.0, slow=1.0)
+    plain = K.rotary_frequencies(64)
+    turns = plain * 2048 / (2 * math.pi)
+    assert torch.equal(h[turns >= 32], plain[turns >= 32]) and torch.allclose(h[turns <= 1], plain[turns <= 1] / 8, rtol=1e-15)
+    between = (turns > 1) & (turns < 32)
+    assert between.any() and (h[between] < plain[between]).all() and (h[between] > plain[between] / 8).all()
+
+
+@pytest.mark.parametrize('kw', [dict(dim=0), dict(dim=7), dict(dim=8, base=0.0), dict(dim=8, factor=-1.0), dict(dim=8, scaling='yes'),
+                                dict(dim=2, scaling='base'), dict(dim=8, scaling='parts'), dict(dim=8, scaling='parts', trained=64, fast=1.0, slow=2.0)])
+def test_frequencies_refused(kw):
+    with pytest.raises(ValueError):
+        K.rotary_frequencies(**kw)
+
+
+def test_refusals():
+    f, q, k = K.rotary_frequencies(8), torch.randn(2, 3, 4, 8), torch.randn(2, 3, 1, 8)
+    with pytest.raises(ValueError):
+        K.rotary(q[0], None, f)
+    with pytest.raises(ValueError):
+        K.rotary(q, k[:, :2], f)
+    with pytest.raises(ValueError):
+        K.rotary(q, k[..., :6], K.rotary_frequencies(6))
+    with pytest.raises(ValueError):
+        K.rotary(q, k.bfloat16(), f)
+    with pytest.raises(ValueError):
+        K.rotary(q, None, K.rotary_frequencies(10))
+    with pytest.raises(ValueError):
+        K.rotary(q, None, f.float())
+    with pytest.raises(ValueError):
+        K.rotary(q, None, f, positions=torch.arange(4))
+    with pytest.raises(TypeError):
+        K.rotary(q, None, f, positions=torch.arange(3.0))
+    with pytest.raises(TypeError):
+        K.rotary(q.double(), None, f)
+    with pytest.raises(ValueError):
+        K.rotary(q, None, f.to('meta'))
+
+
+@pytest.mark.skipif(not native.available(), reason='kernel library not built')
+def test_entry_point_refuses():
+    """No launch: every call is refused by its arguments."""
+    import ctypes
+    lib, at = native.lib(), 1 << 20
+    st = (ctypes.c_int64 * 12)(*([24, 8, 8] * 4))
+    other = (ctypes.c_int64 * 12)(*([24, 8, 8] + [48, 8, 8] + [24, 8, 8] * 2))
+
+    def call(x=at, y=at, strides=st, freqs=at, batch=1, part=8, dim=8):
+        return lib.msamp_rotary(x, y, None, None, strides, freqs, None, 0, 0, 0, batch, 3, 1, 0, dim, part, 0, 0, 0, None)
+
+    for kw in (dict(x=None), dict(y=None), dict(freqs=None), dict(batch=-1), dict(part=7), dict(part=10), dict(part=0), dict(strides=other),
+               dict(part=2048, dim=2048)):
+        assert call(**kw) == 1, kw
+    assert call(batch=0) == 0
+
+
+@pytest.mark.gpu
+def test_captured_and_on_a_side_stream():
+    torch.manual_seed(4)
+    freqs = K.rotary_frequencies(64, device='cuda')
+    q = torch.randn(2, 33, 4, 64, device='cuda').bfloat16()
+    pos = torch.arange(33, device='cuda')
+    K.rotary(q, None, freqs, positions=pos)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = K.rotary(q, None, freqs, positions=pos)
+    pos += 1000
+    q.normal_()
+    g.replay()
+    _check(y, q, freqs, pos, False)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        z = K.rotary(q, None, freqs, positions=pos)
+    s.synchronize()
+    assert torch.equal(y, z)
+    assert native.device_status() == 0
