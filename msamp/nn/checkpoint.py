@@ -1,0 +1,62 @@
+"""Activation recomputation from an input that is kept in 8 bits."""
+import torch
+
+from msamp.ops import cast as _c
+
+
+def _outputs(out):
+    return (out, ) if isinstance(out, torch.Tensor) else tuple(out)
+
+
+class _CheckpointFp8Fn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, anchor, function, preserve_rng_state, args, x):
+        ctx.function, ctx.args = function, args
+        ctx.dtype, ctx.needs_x = x.dtype, x.requires_grad
+        ctx.device = x.device
+        ctx.autocast = (torch.is_autocast_enabled(x.device.type), torch.get_autocast_dtype(x.device.type), torch.is_autocast_cache_enabled())
+        ctx.rng = None
+        if preserve_rng_state:
+            ctx.rng = (torch.get_rng_state(), torch.cuda.get_rng_state(x.device) if x.is_cuda else None)
+        with torch.no_grad():
+            out = function(x, *args)
+        ctx.single = isinstance(out, torch.Tensor)
+        ctx.save_for_backward(*_c.cast_blocks_to_fp8(x))
+        return out if ctx.single else tuple(out)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        codes, exponents = ctx.saved_tensors
+        x = _c.cast_blocks_from_fp8(codes, exponents, ctx.dtype).requires_grad_(ctx.needs_x)
+        cuda = [ctx.device] if ctx.rng is not None and ctx.rng[1] is not None else []
+        enabled, dtype, cache = ctx.autocast
+        with torch.random.fork_rng(devices=cuda, enabled=ctx.rng is not None):
+            if ctx.rng is not None:
+                torch.set_rng_state(ctx.rng[0])
+                if cuda:
+                    torch.cuda.set_rng_state(ctx.rng[1], ctx.device)
+            with torch.enable_grad(), torch.autocast(ctx.device.type, enabled=enabled, dtype=dtype, cache_enabled=cache):
+                out = _outputs(ctx.function(x, *ctx.args))
+        pairs = [(o, g) for o, g in zip(out, grads) if g is not None and o.requires_grad]
+        if pairs:
+            torch.autograd.backward([o for o, _ in pairs], [g for _, g in pairs])
+        return None, None, None, None, x.grad
+
+
+def checkpoint_fp8(function, x, *args, preserve_rng_state=True):
+    """``function(x, *args)`` whose activations are not kept: the backward pass runs it again, from an ``x`` kept in 8 bits.
+
+    ``x`` (fp32, fp16 or bf16) is stored as e4m3 with a power-of-two scale per 32 elements (1.03 bytes each,
+    :func:`msamp.ops.cast.cast_blocks_to_fp8`), so the outputs are those of ``function(x)`` and the gradients those at the stored
+    value, which is within 2^-4 of every element (of the small ones of a block: within 2^-17 of its largest).  Scaling metas of FP8 layers record the amaxes of the second run.  ``function``
+    returns a tensor or a tuple of tensors; ``args`` are handed on as they are and get no gradients.  Parameters receive theirs in
+    ``.grad``: use ``backward()``, not ``torch.autograd.grad``.  The random state of the first run is used again unless
+    ``preserve_rng_state`` is false.
+    """
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f'checkpoint_fp8: unsupported dtype {x.dtype}')
+    if not torch.is_grad_enabled():
+        return function(x, *args)
+    # the anchor makes the outputs part of the graph where only parameters need gradients
+    anchor = torch.empty(0, requires_grad=True)
+    return _CheckpointFp8Fn.apply(anchor, function, preserve_rng_state, args, x)

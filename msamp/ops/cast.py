@@ -276,3 +276,83 @@ def roll_windows(amaxs, scales, qtype, margin=0, bad_out=None):
     amaxs[:, 0] = 0
     if bad_out is not None:
         bad_out.copy_(bad.to(torch.int32))
+
+
+# ---------------------------------------------------------------------------------------- e4m3 with an exponent per 32 elements
+BLOCK = 32
+
+
+def _block_shift(amax):
+    """k of a block from its largest finite magnitude: the largest with ``amax * 2**k <= 448``, at most 127; 0 for 0."""
+    m, e = torch.frexp(amax)    # amax = m * 2**e, 0.5 <= m < 1, and 448 = 0.875 * 2**9
+    k = torch.where(m <= 0.875, 9 - e, 8 - e).clamp(max=127)
+    return torch.where(amax == 0, torch.zeros_like(k), k)
+
+
+def _check_blocks(codes, exponents):
+    if codes.dtype != torch.uint8 or exponents.dtype != torch.uint8 or exponents.device != codes.device:
+        raise TypeError(f'blocks: codes and exponents are uint8 tensors on one device (got {codes.dtype}, {exponents.dtype})')
+    if exponents.numel() != (codes.numel() + BLOCK - 1) // BLOCK:
+        raise ValueError(f'blocks: {codes.numel()} codes need {(codes.numel() + BLOCK - 1) // BLOCK} exponents (got {exponents.numel()})')
+
+
+def _blocks_cast(x, want_gelu):
+    """``(codes, exponents, gelu(x) or None)`` of a contiguous CUDA tensor in one pass."""
+    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    exponents = torch.empty((x.numel() + BLOCK - 1) // BLOCK, dtype=torch.uint8, device=x.device)
+    y = torch.empty_like(x) if want_gelu else None
+    with native.on_device(x):
+        native.check(
+            native.lib().msamp_blocks_cast(
+                x.data_ptr(), native.addr(y), codes.data_ptr(), exponents.data_ptr(), x.numel(), native.dt(x.dtype), native.raw_stream()
+            ), 'cast_blocks_to_fp8'
+        )
+    return codes, exponents, y
+
+
+def cast_blocks_to_fp8(x):
+    """Quantise ``x`` (fp32/fp16/bf16) to e4m3 with a power-of-two scale for every 32 consecutive elements (in row-major order).
+
+    Returns ``(codes, exponents)``: uint8 codes in the shape of ``x`` and one byte ``127 - k`` per block, where ``k <= 127`` is the largest
+    shift that keeps the block's finite values times ``2**k`` within 448.  Nothing finite saturates; NaN and infinities become the NaN
+    code and do not affect the rest of their block.  1.03 bytes per element, each value within 2^-4 of itself (below 2^-13 of the
+    largest of its block: within 2^-17 of that).
+    """
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f'cast_blocks_to_fp8: unsupported dtype {x.dtype}')
+    if x.is_cuda:
+        return _blocks_cast(x.contiguous(), False)[:2]
+    n = x.numel()
+    rows = torch.nn.functional.pad(x.detach().float().reshape(-1), (0, -n % BLOCK)).view(-1, BLOCK)
+    finite = torch.isfinite(rows)
+    if n == 0:
+        return torch.empty(x.shape, dtype=torch.uint8), torch.empty(0, dtype=torch.uint8)
+    k = _block_shift(torch.where(finite, rows.abs(), 0.0).amax(1, keepdim=True))
+    # in 64 bits: 2**k and the product are exact for subnormal numbers too
+    scaled = torch.where(finite, torch.ldexp(rows.double(), k), float('nan')).float()
+    codes = scaled.to(torch.float8_e4m3fn).view(torch.uint8).view(-1)[:n].view(x.shape)
+    return codes.contiguous(), (127 - k).to(torch.uint8).view(-1)
+
+
+def cast_blocks_from_fp8(codes, exponents, out_dtype):
+    """The values of :func:`cast_blocks_to_fp8` in ``out_dtype``, no larger than its largest finite number."""
+    if out_dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f'cast_blocks_from_fp8: unsupported dtype {out_dtype}')
+    _check_blocks(codes, exponents)
+    codes, exponents = codes.contiguous(), exponents.contiguous()
+    n = codes.numel()
+    if codes.is_cuda:
+        out = torch.empty(codes.shape, dtype=out_dtype, device=codes.device)
+        with native.on_device(codes):
+            native.check(
+                native.lib().msamp_blocks_uncast(
+                    codes.data_ptr(), exponents.data_ptr(), None, out.data_ptr(), n, native.dt(out_dtype), native.raw_stream()
+                ), 'cast_blocks_from_fp8'
+            )
+        return out
+    if n == 0:
+        return torch.empty(codes.shape, dtype=out_dtype)
+    v = torch.nn.functional.pad(codes.view(-1), (0, -n % BLOCK)).view(torch.float8_e4m3fn).double().view(-1, BLOCK)
+    v = torch.ldexp(v, exponents.view(-1, 1).int() - 127).view(-1)[:n].view(codes.shape)
+    top = torch.finfo(out_dtype).max
+    return torch.where(torch.isnan(v), v, v.clamp(-top, top)).to(out_dtype)

@@ -1,0 +1,192 @@
+// Activations kept in 8 bits: e4m3 codes with one power-of-two exponent for every 32 consecutive elements.
+//
+// A block of 32 elements x with a = max |x| over its finite elements has the shift k = floor(log2(448 / a)), at most 127 (0 when a is 0),
+// so that every |x 2^k| is at most 448 and no finite value saturates; code = e4m3(x 2^k), nearest even; NaN and +-inf become the NaN
+// code and leave the rest of their block alone.  The exponent byte is 127 - k, i.e. the fp32 exponent field of 2^-k, and a code stands
+// for code * 2^-k.  k is read off the bits of a (448 = 1.75 * 2^8), and the products with 2^k are exact, so the rounding to e4m3 is the
+// only one: at most 2^-4 of a value that is above 2^-13 of its block's largest, and 2^-17 of the largest below that.
+//
+//   blocks_cast_kernel         x -> codes and exponents; with GELU also y = gelu(x) from the same read of x
+//   blocks_uncast_kernel       codes and exponents -> values; with GELU dx = dy * gelu'(value), the values never written
+//
+// The products with 2^k keep subnormal numbers (mul.rn.f32 written out: the library is compiled with flush-to-zero arithmetic).
+#include "common.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 32;
+
+__device__ __forceinline__ float mul_keep(float a, float b) {
+  float d;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// k of a block from the bits of its largest finite |x|
+__device__ __forceinline__ int block_shift(uint32_t amax) {
+  if (amax == 0) return 0;
+  const int e = (int)(amax >> 23) - 127;
+  return min(127, 8 - e - ((amax & 0x7fffffu) > 0x600000u ? 1 : 0));
+}
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+__device__ __forceinline__ float inf_to_nan(float v) {
+  return (__float_as_uint(v) & 0x7fffffffu) == 0x7f800000u ? __uint_as_float(0x7fffffffu) : v;
+}
+// 2^-k from the exponent byte; byte 0 is the subnormal 2^-127
+__device__ __forceinline__ float block_unit(uint32_t byte) { return __uint_as_float(byte ? byte << 23 : 0x00400000u); }
+
+template <typename T>
+__device__ __forceinline__ float largest();
+template <>
+__device__ __forceinline__ float largest<float>() { return 3.4028234663852886e38f; }
+template <>
+__device__ __forceinline__ float largest<__half>() { return 65504.0f; }
+template <>
+__device__ __forceinline__ float largest<__nv_bfloat16>() { return 3.3895313892515355e38f; }
+// rounding to a code can carry the largest numbers of T past its range; NaN passes
+template <typename T>
+__device__ __forceinline__ float in_range(float v) {
+  const float m = largest<T>();
+  return v > m ? m : (v < -m ? -m : v);
+}
+
+// 32 elements of any alignment, one per lane
+template <typename T, bool GELU>
+__device__ __forceinline__ void cast_block_by_lane(const T* x, T* y, uint8_t* codes, uint8_t* exps, int64_t n, int64_t blk) {
+  const int lane = threadIdx.x & 31;
+  const int64_t i = blk * kBlock + lane;
+  const float v = i < n ? to_f32<T>(x[i]) : 0.0f;
+  const int k = block_shift(__reduce_max_sync(0xffffffffu, finite_bits(v)));
+  if (i < n) {
+    codes[i] = f32_to_fp8<FMT_E4M3>(mul_keep(inf_to_nan(v), __uint_as_float((uint32_t)(k + 127) << 23)));
+    if (GELU) y[i] = from_f32<T>(gelu_f(v));
+  }
+  if (lane == 0) exps[blk] = (uint8_t)(127 - k);
+}
+
+// VEC: every pointer aligned for whole vectors of 16 bytes of T; V elements a thread, L = 32 / V lanes a block.
+template <typename T, bool GELU, bool VEC>
+__global__ void __launch_bounds__(kThreads) blocks_cast_kernel(const T* __restrict__ x, T* __restrict__ y, uint8_t* __restrict__ codes,
+                                                               uint8_t* __restrict__ exps, int64_t n) {
+  const int64_t tid = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t threads = (int64_t)gridDim.x * kThreads;
+  const int64_t full = VEC ? n / kBlock : 0;    // blocks taken by vectors
+  if (VEC) {
+    constexpr int V = 16 / sizeof(T), L = kBlock / V;
+    const int64_t nv = full * L;
+    const int64_t top = (nv + 31) / 32 * 32;    // whole warps go round, for the shuffles
+    for (int64_t i = tid; i < top; i += threads) {
+      Bytes16 raw = {};
+      if (i < nv) raw = reinterpret_cast<const Bytes16*>(x)[i];
+      const T* e = reinterpret_cast<const T*>(&raw);
+      float v[V];
+      uint32_t a = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[j] = to_f32<T>(e[j]);
+        a = max(a, finite_bits(v[j]));
+      }
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+      if (i >= nv) continue;
+      const int k = block_shift(a);
+      const float s = __uint_as_float((uint32_t)(k + 127) << 23);
+      uint32_t c[V / 4];
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        const uint32_t lo = f32x2_to_fp8x2<FMT_E4M3>(mul_keep(inf_to_nan(v[j]), s), mul_keep(inf_to_nan(v[j + 1]), s));
+        const uint32_t hi = f32x2_to_fp8x2<FMT_E4M3>(mul_keep(inf_to_nan(v[j + 2]), s), mul_keep(inf_to_nan(v[j + 3]), s));
+        c[j / 4] = lo | hi << 16;
+      }
+      if (V == 8) reinterpret_cast<uint2*>(codes)[i] = make_uint2(c[0], c[V / 4 - 1]);
+      else        reinterpret_cast<uint32_t*>(codes)[i] = c[0];
+      if (i % L == 0) exps[i / L] = (uint8_t)(127 - k);
+      if (GELU) {
+        Bytes16 out;
+        T* oe = reinterpret_cast<T*>(&out);
+#pragma unroll
+        for (int j = 0; j < V; ++j) oe[j] = from_f32<T>(gelu_f(v[j]));
+        reinterpret_cast<Bytes16*>(y)[i] = out;
+      }
+    }
+  }
+  const int64_t blocks = (n + kBlock - 1) / kBlock;
+  for (int64_t b = full + tid / 32; b < blocks; b += threads / 32) cast_block_by_lane<T, GELU>(x, y, codes, exps, n, b);
+}
+
+template <typename T, bool GELU>
+__device__ __forceinline__ T uncast_one(float v, T dy) {
+  if (GELU) return from_f32<T>(to_f32<T>(dy) * gelu_grad_f(v));
+  return from_f32<T>(in_range<T>(v));
+}
+
+template <typename T, bool GELU, bool VEC>
+__global__ void __launch_bounds__(kThreads) blocks_uncast_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
+                                                                 const T* __restrict__ dy, T* __restrict__ out, int64_t n) {
+  const int64_t tid = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t threads = (int64_t)gridDim.x * kThreads;
+  constexpr int V = 16 / sizeof(T), L = kBlock / V;
+  const int64_t nv = VEC ? n / V : 0;
+  if (VEC) {
+    for (int64_t i = tid; i < nv; i += threads) {
+      uint32_t c[2];
+      if (V == 8) {
+        const uint2 r = reinterpret_cast<const uint2*>(codes)[i];
+        c[0] = r.x;
+        c[1] = r.y;
+      } else {
+        c[0] = reinterpret_cast<const uint32_t*>(codes)[i];
+      }
+      Bytes16 g = {}, o;
+      if (GELU) g = reinterpret_cast<const Bytes16*>(dy)[i];
+      const float u = block_unit(exps[i / L]);
+      const T* ge = reinterpret_cast<const T*>(&g);
+      T* oe = reinterpret_cast<T*>(&o);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        oe[j] = uncast_one<T, GELU>(mul_keep(fp8_to_f32<FMT_E4M3>((uint8_t)(c[j / 4] >> (8 * (j & 3)))), u), ge[j]);
+      reinterpret_cast<Bytes16*>(out)[i] = o;
+    }
+  }
+  for (int64_t i = nv * V + tid; i < n; i += threads)
+    out[i] = uncast_one<T, GELU>(mul_keep(fp8_to_f32<FMT_E4M3>(codes[i]), block_unit(exps[i / kBlock])), GELU ? dy[i] : T());
+}
+
+}    // namespace
+
+// x -> codes [n], exps [ceil(n / 32)] and, where y is given, y = gelu(x) (tanh form) in the type of x.
+MSAMP_API int msamp_blocks_cast(const void* x, void* y, void* codes, void* exps, int64_t n, int dtype, void* stream_) {
+  if (n <= 0) return MSAMP_OK;
+  MSAMP_REQUIRE(x && codes && exps, "blocks_cast: null pointer");
+  cudaStream_t stream = (cudaStream_t)stream_;
+  const bool vec = aligned16(x) && aligned16(codes) && (!y || aligned16(y));
+  MSAMP_DISPATCH_HP(dtype, T, {
+    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 15) / 16 : n, kThreads, 8);
+    if (vec && y)  blocks_cast_kernel<T, true, true><<<grid, kThreads, 0, stream>>>((const T*)x, (T*)y, (uint8_t*)codes, (uint8_t*)exps, n);
+    else if (vec)  blocks_cast_kernel<T, false, true><<<grid, kThreads, 0, stream>>>((const T*)x, nullptr, (uint8_t*)codes, (uint8_t*)exps, n);
+    else if (y)    blocks_cast_kernel<T, true, false><<<grid, kThreads, 0, stream>>>((const T*)x, (T*)y, (uint8_t*)codes, (uint8_t*)exps, n);
+    else           blocks_cast_kernel<T, false, false><<<grid, kThreads, 0, stream>>>((const T*)x, nullptr, (uint8_t*)codes, (uint8_t*)exps, n);
+  });
+  return msamp_check_launch("msamp_blocks_cast");
+}
+
+// codes, exps -> out = values, or out = dy * gelu'(values) where dy is given; dtype is that of dy and out.
+MSAMP_API int msamp_blocks_uncast(const void* codes, const void* exps, const void* dy, void* out, int64_t n, int dtype, void* stream_) {
+  if (n <= 0) return MSAMP_OK;
+  MSAMP_REQUIRE(codes && exps && out, "blocks_uncast: null pointer");
+  cudaStream_t stream = (cudaStream_t)stream_;
+  const bool vec = aligned16(codes) && aligned16(out) && (!dy || aligned16(dy));
+  MSAMP_DISPATCH_HP(dtype, T, {
+    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 15) / 16 : n, kThreads, 8);
+    const uint8_t *c = (const uint8_t*)codes, *e = (const uint8_t*)exps;
+    if (vec && dy) blocks_uncast_kernel<T, true, true><<<grid, kThreads, 0, stream>>>(c, e, (const T*)dy, (T*)out, n);
+    else if (vec)  blocks_uncast_kernel<T, false, true><<<grid, kThreads, 0, stream>>>(c, e, nullptr, (T*)out, n);
+    else if (dy)   blocks_uncast_kernel<T, true, false><<<grid, kThreads, 0, stream>>>(c, e, (const T*)dy, (T*)out, n);
+    else           blocks_uncast_kernel<T, false, false><<<grid, kThreads, 0, stream>>>(c, e, nullptr, (T*)out, n);
+  });
+  return msamp_check_launch("msamp_blocks_uncast");
+}

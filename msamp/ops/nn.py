@@ -10,7 +10,7 @@ import os
 import torch
 import torch.nn.functional as F
 
-from msamp.ops import native
+from msamp.ops import cast as _c, native
 from msamp.ops.rotary import rotary, rotary_frequencies, rotary_raw    # noqa: F401
 
 _i64x24 = ctypes.c_int64 * 24
@@ -93,7 +93,6 @@ def layer_norm_fwd_raw(x2, weight, bias, eps, want_y=True, y8_scale=None, amax_i
         )
         return y, y8, mean, rstd
     from msamp.common.dtype import Dtypes
-    from msamp.ops import cast as _c
     xf = x2.float()
     mean = xf.mean(1)
     var = xf.var(1, unbiased=False)
@@ -131,7 +130,6 @@ def layer_norm_bwd_raw(dy2, x2, weight, mean, rstd, has_bias, dres=None, amax_ou
             ), 'layernorm_bwd'
         )
         return dx, dgamma, dbeta
-    from msamp.ops import cast as _c
     xh = (x2.float() - mean[:, None]) * rstd[:, None]
     d = dy2.float()
     gd = d * weight.float()
@@ -183,8 +181,54 @@ class _GeluFn(torch.autograd.Function):
         return dx
 
 
-def gelu(x):
-    """GeLU, tanh form."""
+class _GeluKeepFn(torch.autograd.Function):
+    """GeLU whose input is kept as e4m3 blocks: written by the forward kernel next to the output, read by the backward kernel."""
+    @staticmethod
+    def forward(ctx, x):
+        if x.is_cuda:
+            codes, exponents, y = _c._blocks_cast(x.contiguous(), True)
+        else:
+            codes, exponents = _c.cast_blocks_to_fp8(x)
+            y = F.gelu(x.float(), approximate='tanh').to(x.dtype)
+        ctx.save_for_backward(codes, exponents)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        return gelu_bwd_blocks(*ctx.saved_tensors, dy)
+
+
+def gelu_bwd_blocks(codes, exponents, dy):
+    """``dy * gelu'(x)`` for the ``x`` that the e4m3 blocks stand for (see ``cast.cast_blocks_to_fp8``), in the type of ``dy``."""
+    _c._check_blocks(codes, exponents)
+    if codes.shape != dy.shape or codes.device != dy.device:
+        raise ValueError(f'gelu: codes {tuple(codes.shape)} and gradient {tuple(dy.shape)} differ')
+    if dy.is_cuda:
+        dy, codes, exponents = dy.contiguous(), codes.contiguous(), exponents.contiguous()
+        dx = torch.empty_like(dy)
+        with native.on_device(dy):
+            native.check(
+                native.lib().msamp_blocks_uncast(
+                    codes.data_ptr(), exponents.data_ptr(), dy.data_ptr(), dx.data_ptr(), dy.numel(), native.dt(dy.dtype), native.raw_stream()
+                ), 'gelu_bwd_blocks'
+            )
+        return dx
+    with torch.enable_grad():
+        x = _c.cast_blocks_from_fp8(codes, exponents, torch.float32).requires_grad_(True)
+        grad, = torch.autograd.grad(F.gelu(x, approximate='tanh'), x, dy.float())
+    return grad.to(dy.dtype)
+
+
+def gelu(x, keep_fp8=False):
+    """GeLU, tanh form.
+
+    ``keep_fp8`` keeps the input of the backward pass as e4m3 with a power-of-two scale per 32 elements (1.03 bytes each, see
+    ``cast.cast_blocks_to_fp8``) instead of ``x`` itself: the output is the same, the gradient is the slope at the kept value.
+    """
+    if keep_fp8:
+        if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise TypeError(f'gelu: unsupported dtype {x.dtype}')
+        return _GeluKeepFn.apply(x)
     if _use_native(x):
         return _GeluFn.apply(x)
     return F.gelu(x.float(), approximate='tanh').to(x.dtype)

@@ -1,0 +1,248 @@
+"""Activations in 8 bits: the codes against their definition, the GeLU that reads them, recomputation from them.
+
+The codes are exact (equal bytes); the GeLU gradient is half a step of its type from the slope at the kept value, up to the error of the
+exponential and the division in 32 bits (a few ulp of numbers that are at most 1, times |dy| (1 + |v|): 2^-18 covers them).
+"""
+import math
+
+import pytest
+import torch
+
+import msamp
+from msamp.nn import checkpoint_fp8
+from msamp.ops import cast, native
+from msamp.ops import nn as K
+
+CPU_GPU = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def _values(n, dtype, seed):
+    """Magnitudes over the whole range of the type, zeros, whole blocks of zeros, powers of two and numbers just beside 1.75 * 2^k."""
+    gen = torch.Generator().manual_seed(seed)
+    info = torch.finfo(dtype)
+    lo, hi = math.log2(info.smallest_normal) - 3, math.log2(info.max)
+    x = torch.randn(n, generator=gen, dtype=torch.float64)
+    block = torch.arange(n) // 32
+    x = x * torch.exp2(lo + (hi - lo - 3) * torch.rand(int(n // 32) + 1, generator=gen, dtype=torch.float64))[block]
+    x[block % 7 == 3] = 0.0
+    x[torch.rand(n, generator=gen) < 0.05] = 0.0
+    edge = block % 5 == 2
+    x[edge] = (1.75 * torch.exp2(torch.randint(-6, 6, (n, ), generator=gen).double()) * (1 + info.eps * torch.randint(-1, 2, (n, ), generator=gen)))[edge]
+    return x.clamp(-info.max, info.max).to(dtype)
+
+
+def _definition(x):
+    """(codes' values, k) by the definition, in 64 bits."""
+    flat = x.detach().double().cpu().reshape(-1)
+    n = flat.numel()
+    rows = torch.cat([flat, flat.new_zeros(-n % 32)]).view(-1, 32)
+    finite = torch.isfinite(rows)
+    top = torch.where(finite, rows.abs(), 0.0).amax(1)
+    k = torch.zeros_like(top)
+    for j in range(-127, 128):    # the largest shift that keeps the block within 448
+        k = torch.where((top > 0) & (top * 2.0**j <= 448.0), torch.full_like(top, j), k)
+    y = torch.where(finite, rows * torch.exp2(k)[:, None], float('nan'))
+    step = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0**-6))) - 3)    # e4m3: 3 bits of fraction, no finer than 2^-9
+    return (torch.round(y / step) * step).view(-1)[:n], k
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n', [1, 31, 32, 33, 100, 1024, 4097, 40000])
+def test_codes(device, dtype, n):
+    x = _values(n, dtype, n).to(device)
+    codes, exps = cast.cast_blocks_to_fp8(x)
+    want, k = _definition(x)
+    assert codes.shape == x.shape and codes.dtype == torch.uint8 and exps.numel() == (n + 31) // 32
+    assert torch.equal(127 - exps.cpu().double(), k)
+    assert torch.equal(codes.cpu().view(torch.float8_e4m3fn).double(), want)
+    back = cast.cast_blocks_from_fp8(codes, exps, dtype)
+    top = torch.finfo(dtype).max
+    exact = (want * torch.exp2(-k).repeat_interleave(32)[:n]).clamp(-top, top)
+    assert torch.equal(back.cpu(), exact.to(dtype)) and torch.isfinite(back).all()
+    for out in TYPES:
+        other = cast.cast_blocks_from_fp8(codes, exps, out).cpu()
+        lim = torch.finfo(out).max
+        assert torch.equal(other, exact_to(want, k, n, lim).to(out))
+
+
+def exact_to(want, k, n, lim):
+    return (want * torch.exp2(-k).repeat_interleave(32)[:n]).clamp(-lim, lim)
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('dtype', TYPES)
+def test_distance(device, dtype):
+    """The largest of a block is over 224 in steps of its unit 2^-k.  e4m3 rounds numbers from 2^-6 on by at most 2^-4 of themselves, so
+    values above 2^-6 / 224 < 2^-13 of the largest; below, by half of 2^-9, which is under 2^-10 / 224 < 2^-17 of the largest."""
+    x = torch.randn(64, 256, generator=torch.Generator().manual_seed(0)).mul_(0.02)
+    x = (x * torch.exp2(-20 * torch.rand(64, 256, generator=torch.Generator().manual_seed(1)))).to(dtype).to(device)
+    v = cast.cast_blocks_from_fp8(*cast.cast_blocks_to_fp8(x), torch.float32).double()
+    top = x.double().abs().view(-1, 32).amax(1).repeat_interleave(32).view_as(x)
+    err = (v - x.double()).abs()
+    small = x.double().abs() < top * 2.0**-13
+    assert small.any() and (err[~small] <= x.double().abs()[~small] * 2.0**-4).all() and (err[small] <= top[small] * 2.0**-17).all()
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('offset', [0, 1])
+def test_not_finite(device, dtype, offset):
+    x = _values(200 + offset, dtype, 5)[offset:]
+    plain = cast.cast_blocks_to_fp8(x.to(device))
+    bad = x.clone()
+    bad[3], bad[40], bad[41], bad[199] = float('inf'), float('nan'), -float('inf'), float('inf')
+    at = torch.zeros(200, dtype=torch.bool)
+    at[[3, 40, 41, 199]] = True
+    codes, exps = cast.cast_blocks_to_fp8(bad.to(device))
+    want, k = _definition(bad)
+    assert torch.equal(127 - exps.cpu().double(), k)
+    back = cast.cast_blocks_from_fp8(codes, exps, dtype).cpu()
+    assert torch.equal(torch.isnan(back), at) and torch.isfinite(back[~at]).all()
+    assert torch.equal(codes.cpu().view(torch.float8_e4m3fn).double()[~at], want[~at])
+    untouched = torch.arange(200) // 32
+    keep = (untouched != 0) & (untouched != 1) & (untouched != 6)
+    assert torch.equal(codes.cpu()[keep], plain[0].cpu()[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_gpu_equals_cpu_for_views(dtype):
+    base = _values(3 * 70 * 50 + 1, dtype, 9)
+    for view in (lambda t: t[1:], lambda t: t[:-1].view(3, 70, 50).transpose(0, 2), lambda t: t[:-1].view(3, 70, 50)[:, ::2]):
+        a, b = cast.cast_blocks_to_fp8(view(base)), cast.cast_blocks_to_fp8(view(base.cuda()))
+        assert torch.equal(a[0], b[0].cpu()) and torch.equal(a[1], b[1].cpu())
+        for out in TYPES:
+            assert torch.equal(cast.cast_blocks_from_fp8(*a, out), cast.cast_blocks_from_fp8(*b, out).cpu())
+    odd = torch.empty(base.numel() + 1, dtype=torch.uint8, device='cuda')[1:]    # codes off the 16-byte grid
+    c, e = cast.cast_blocks_to_fp8(base.cuda())
+    odd.copy_(c)
+    assert torch.equal(cast.cast_blocks_from_fp8(odd, e, dtype), cast.cast_blocks_from_fp8(c, e, dtype))
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+def test_empty(device):
+    x = torch.empty(0, 7, device=device)
+    codes, exps = cast.cast_blocks_to_fp8(x)
+    assert codes.shape == (0, 7) and exps.numel() == 0 and cast.cast_blocks_from_fp8(codes, exps, torch.bfloat16).shape == (0, 7)
+    y = K.gelu(x.requires_grad_(True), keep_fp8=True)
+    y.sum().backward()
+    assert x.grad.shape == (0, 7)
+
+
+def _slope(v):
+    c0, c1 = math.sqrt(2.0 / math.pi), 0.044715
+    t = torch.tanh(c0 * (v + c1 * v**3))
+    return 0.5 * (1 + t) + 0.5 * v * (1 - t * t) * c0 * (1 + 3 * c1 * v * v)
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape, offset', [((1, ), 0), ((33, ), 0), ((7, 100), 0), ((7, 100), 1), ((64, 512), 0), ((3, 5, 1000), 0)])
+def test_gelu(device, dtype, shape, offset):
+    n = math.prod(shape)
+    gen = torch.Generator().manual_seed(n)
+    x = (torch.randn(n + offset, generator=gen) * 3).to(dtype).to(device)[offset:].view(shape).requires_grad_(True)
+    dy = torch.randn(n + offset, generator=gen).to(dtype).to(device)[offset:].view(shape)
+    y = K.gelu(x, keep_fp8=True)
+    if offset == 0 or device == 'cpu':
+        assert torch.equal(y, K.gelu(x.detach()))    # the output does not know
+    dx, = torch.autograd.grad(y, x, dy)
+    v = cast.cast_blocks_from_fp8(*cast.cast_blocks_to_fp8(x.detach()), torch.float32).double()
+    want = dy.double() * _slope(v)
+    err = (dx.double() - want).abs()
+    tiny = torch.finfo(dtype).smallest_normal
+    assert (err <= want.abs() * torch.finfo(dtype).eps / 2 + dy.double().abs() * (1 + v.abs()) * 2.0**-18 + tiny).all()
+    # against differences of the function itself, at the kept values
+    h = 1e-4
+    c0, c1 = math.sqrt(2.0 / math.pi), 0.044715
+    f = lambda t: 0.5 * t * (1 + torch.tanh(c0 * (t + c1 * t**3)))    # noqa: E731
+    diff = dy.double() * (f(v + h) - f(v - h)) / (2 * h)
+    assert ((want - diff).abs() <= 1e-6 * (1 + dy.double().abs())).all()
+
+
+@pytest.mark.gpu
+def test_gelu_views_and_gradient_layouts():
+    x = torch.randn(40, 64, device='cuda').bfloat16().requires_grad_(True)
+    y = K.gelu(x, keep_fp8=True)
+    dy = torch.randn(64, 40, device='cuda').bfloat16().t()
+    a, = torch.autograd.grad(y, x, dy, retain_graph=True)
+    b, = torch.autograd.grad(y, x, dy.contiguous(), retain_graph=True)
+    c, = torch.autograd.grad(y.sum(), x)    # an expanded gradient
+    d, = torch.autograd.grad(K.gelu(x, keep_fp8=True), x, torch.ones_like(y))
+    assert torch.equal(a, b) and torch.equal(c, d)
+    t = torch.randn(64, 40, device='cuda').bfloat16()
+    u, v = t.t().detach().requires_grad_(True), t.t().contiguous().requires_grad_(True)
+    (gu, ), (gv, ) = torch.autograd.grad(K.gelu(u, keep_fp8=True), u, dy[:40, :64]), torch.autograd.grad(K.gelu(v, keep_fp8=True), v, dy[:40, :64])
+    assert torch.equal(gu, gv)
+
+
+def test_refusals():
+    c, e = cast.cast_blocks_to_fp8(torch.randn(70))
+    for bad in (lambda: cast.cast_blocks_to_fp8(torch.zeros(3, dtype=torch.float64)), lambda: cast.cast_blocks_to_fp8(torch.zeros(3, dtype=torch.int32)),
+                lambda: cast.cast_blocks_from_fp8(c, e, torch.float64), lambda: cast.cast_blocks_from_fp8(c.float(), e, torch.float32),
+                lambda: K.gelu(torch.zeros(3, dtype=torch.float64), keep_fp8=True), lambda: checkpoint_fp8(torch.sin, torch.zeros(3, dtype=torch.int64))):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: cast.cast_blocks_from_fp8(c, e[:-1], torch.float32), lambda: K.gelu_bwd_blocks(c, e, torch.randn(2, 35))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@pytest.mark.skipif(not native.available(), reason='kernel library not built')
+def test_entry_points_refuse():
+    """No launch: every call is refused by its arguments."""
+    lib, at = native.lib(), 1 << 20
+    assert lib.msamp_blocks_cast(None, None, at, at, 8, 0, None) == 1 and lib.msamp_blocks_cast(at, None, None, at, 8, 0, None) == 1
+    assert lib.msamp_blocks_cast(at, None, at, None, 8, 0, None) == 1 and lib.msamp_blocks_cast(at, None, at, at, 8, 7, None) == 2
+    assert lib.msamp_blocks_uncast(None, at, None, at, 8, 0, None) == 1 and lib.msamp_blocks_uncast(at, at, None, None, 8, 0, None) == 1
+    assert lib.msamp_blocks_cast(None, None, None, None, 0, 0, None) == 0 and lib.msamp_blocks_uncast(None, None, None, None, 0, 0, None) == 0
+
+
+# ------------------------------------------------------------------------------------------------------------- recomputation
+@pytest.mark.parametrize('device', CPU_GPU)
+def test_checkpoint_gradients_are_those_at_the_kept_input(device):
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(48, 40, device=device)
+    x = torch.randn(6, 48, device=device, requires_grad=True)
+    f = lambda t, s: torch.tanh(lin(t)) * s    # noqa: E731
+    y = checkpoint_fp8(f, x, 2.0)
+    assert torch.equal(y, f(x, 2.0))
+    dy = torch.randn_like(y)
+    y.backward(dy)
+    v = cast.cast_blocks_from_fp8(*cast.cast_blocks_to_fp8(x.detach()), x.dtype).requires_grad_(True)
+    wv, wb, wx = torch.autograd.grad(f(v, 2.0), (lin.weight, lin.bias, v), dy)
+    assert torch.equal(x.grad, wx) and torch.equal(lin.weight.grad, wv) and torch.equal(lin.bias.grad, wb)
+
+
+def test_checkpoint_dropout_tuple_and_frozen_input():
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(32, 32)
+    x = torch.ones(4, 32)    # exact in 8 bits, needs no gradient
+
+    def f(t):
+        z = torch.nn.functional.dropout(lin(t), 0.5)
+        return z, z.sum(), torch.arange(3)
+
+    z, total, count = checkpoint_fp8(f, x)
+    state = torch.get_rng_state()
+    (z.sum() + total).backward()
+    assert torch.equal(state, torch.get_rng_state()) and torch.equal(count, torch.arange(3))
+    kept = (z != 0).float()
+    assert torch.allclose(lin.weight.grad, 2 * (kept * 2.0).t() @ x) and x.grad is None
+    with torch.no_grad():
+        assert not checkpoint_fp8(f, x)[0].requires_grad
+
+
+def test_checkpoint_keeps_one_byte_per_element():
+    seen = []
+    lin = torch.nn.Linear(64, 64)
+    x = torch.randn(32, 64, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t) or t, lambda t: t):
+        checkpoint_fp8(lambda t: torch.tanh(lin(t)), x)
+    assert sum(t.numel() * t.element_size() for t in seen) == 32 * 64 + 64
+
+
+def test_public_names():
+    assert msamp.nn.checkpoint_fp8 is checkpoint_fp8 and 'checkpoint_fp8' in msamp.nn.__all__
