@@ -48,7 +48,16 @@ struct TcParams {
   int group;              // persistent kernels: (batch, head) pairs whose work items are taken together
   float scale;
   unsigned int* status;
+  // kernels with X only
+  int kv_heads, rep;       // key / value heads; query heads of each
+  const int* lengths;      // [batch] positions of a row that are not padding, or null: all
+  int parts;               // dK / dV: work items that share the query heads of a key / value head
+  float* partial;          // [parts][dK, dV][batch, kv_heads, seqlen, head_dim] when there are several
 };
+
+__device__ __forceinline__ int row_length(const TcParams& p, int b) { return p.lengths ? min(max(__ldg(p.lengths + b), 0), p.seqlen) : p.seqlen; }
+// The 128-row tile t of a sequence holds rows behind its end that are there in memory (rows behind seqlen are filled with zeros by TMA).
+__device__ __forceinline__ bool ends_inside(int t, int len, int seqlen) { return len < seqlen && (t + 1) * 128 > len; }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -76,6 +85,16 @@ __device__ __forceinline__ void mask_above(uint32_t (&r)[2][32], int last, uint3
 
 // Makes this thread's ordinary shared-memory writes visible to the async proxy (the MMA reads them).
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A warp clears rows first .. 127 of a 128-row tile (panels of 128 bytes a row).  A masked probability is exactly 0, but a product over
+// keys or queries multiplies it by what the padding holds, and 0 * inf is not 0.
+template <int PANELS>
+__device__ __forceinline__ void clear_rows(uint32_t tile, uint32_t panel, int first) {
+  const uint32_t from = (uint32_t)max(first, 0) * 128u + (threadIdx.x & 31) * 16u;
+  for (int pp = 0; pp < PANELS; ++pp)
+    for (uint32_t o = from; o < 128u * 128u; o += 512u) st_shared_v4(tile + (uint32_t)pp * panel + o, 0u, 0u, 0u, 0u);
+  fence_async_smem();
+}
 
 // 128 fp32 values of one row -> bf16 -> 256 contiguous bytes in global memory.
 __device__ __forceinline__ void st_row32(__nv_bfloat16* dst, const float (&v)[32]) {
@@ -1054,7 +1073,7 @@ struct Cfg {
   static constexpr uint32_t TILE = HP * PANEL;
   static constexpr uint32_t OFF_K = 2 * TILE, OFF_V = OFF_K + NK * TILE, OFF_BAR = OFF_V + NV * TILE;    // two Q tiles first
   static constexpr int B_Q = 0, B_QE = 2, B_KF = 4, B_KE = B_KF + NK, B_VF = B_KE + NK, B_VE = B_VF + NV, B_SF = B_VE + NV, B_SE = B_SF + 2,
-                       B_PF = B_SE + 1, B_OF = B_PF + 2, B_X = B_OF + 2, NBAR = B_X + 1;
+                       B_PF = B_SE + 1, B_OF = B_PF + 2, B_X = B_OF + 2, B_VL = B_X + 1, NBAR = B_VL + NV;
   static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16 + 1024;
   static_assert(SMEM <= 227 * 1024, "persistent forward kernel: shared memory");
 };
@@ -1073,13 +1092,17 @@ struct FwdItem {
   int qt, bh;
   int first, step, n_t;    // key tiles first, first + step, ... < n_t; n_t == 0: no item
   bool shared;
+  int len;                 // X: length of the row
 };
+// X: a row ends at its length, and a query tile behind it still takes one tile, all of it masked, which leaves zeros.
+template <bool X>
 struct FwdItems {
   int n_qt, n_items, bh_total, G, n_ctas, causal;
+  const TcParams* p;
   __device__ __forceinline__ FwdItem at(int w, int g) const {
     const int full = n_items / (2 * n_ctas), rem = n_items - full * 2 * n_ctas;
     const int c = (int)blockIdx.x;
-    FwdItem x{0, 0, 0, 1, 0, false};
+    FwdItem x{0, 0, 0, 1, 0, false, 0};
     // even waves upwards, odd waves downwards, so that the sums per worker stay within about a tile of each other
     int j = g * n_ctas + c;
     if (w & 1) j = 2 * n_ctas - 1 - j;
@@ -1105,6 +1128,10 @@ struct FwdItems {
     x.qt = n_qt - 1 - k / hg;
     x.bh = grp * G + k % hg;
     x.n_t = causal ? x.qt + 1 : n_qt;
+    if (X) {
+      x.len = row_length(*p, x.bh / p->heads);
+      x.n_t = x.qt * 128 >= x.len ? 1 : min(x.n_t, (x.len + 127) / 128);
+    }
     return x;
   }
 };
@@ -1115,7 +1142,8 @@ struct FwdStream {
   int g, w, t;           // stream, next wave, tile of the current item
   FwdItem item;          // n_t == 0: list exhausted
   uint32_t started;      // items so far (an item that is one shared tile leaves the second stream without any)
-  __device__ __forceinline__ void open(const FwdItems& items) {
+  template <bool X>
+  __device__ __forceinline__ void open(const FwdItems<X>& items) {
     item = items.at(w++, g);
     t = item.first;
     if (t >= item.n_t) item.n_t = 0;
@@ -1126,7 +1154,8 @@ struct FwdStream {
 };
 struct FwdSeq {
   FwdStream cur, other;
-  __device__ __forceinline__ FwdSeq(const FwdItems& items) {
+  template <bool X>
+  __device__ __forceinline__ FwdSeq(const FwdItems<X>& items) {
     cur.g = cur.w = other.w = 0;
     other.g = 1;
     cur.started = other.started = 0u;
@@ -1134,7 +1163,8 @@ struct FwdSeq {
     other.open(items);
   }
   __device__ __forceinline__ bool more() const { return cur.item.n_t > 0; }
-  __device__ __forceinline__ void advance(const FwdItems& items) {
+  template <bool X>
+  __device__ __forceinline__ void advance(const FwdItems<X>& items) {
     cur.t += cur.item.step;
     if (cur.t >= cur.item.n_t) cur.open(items);
     if (other.item.n_t > 0) {
@@ -1171,7 +1201,10 @@ struct FwdSeq {
 // Reuse: Q_g after the last score product of its item (B_QE); the score slot after B_SE (tiles in sequence order); P_g and
 // the accumulator after P V of the group's previous tile (B_OF); the accumulator of a finished item is read before the group
 // hands over its next P (B_PF), so the next item's first product cannot overtake it.
-template <int D>
+// X: query heads share key / value heads (only the coordinates of the K and V tiles know) and rows have lengths.  Scores of padded keys
+// and of padded queries are masked like those of later keys.  A V tile with rows behind the end of its sequence lands on a barrier of its
+// own (B_VL, one per slot, so that neither side can be a phase ahead); warp 3 clears those rows and then arrives on B_VF for it.
+template <int D, bool X>
 __global__ void __launch_bounds__(kPsThreads, 1)
 attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const TcParams p, int n_qt, int n_items) {
@@ -1191,7 +1224,7 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   auto wait_warp = [&](uint32_t br, uint32_t ph) { return __all_sync(0xffffffffu, wait(br, ph)) != 0; };
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const FwdItems items{n_qt, n_items, p.batch * p.heads, p.group, (int)gridDim.x, p.causal};
+  const FwdItems<X> items{n_qt, n_items, p.batch * p.heads, p.group, (int)gridDim.x, p.causal, &p};
 
   if (threadIdx.x == 0) {
     for (int g = 0; g < 2; ++g) {
@@ -1210,6 +1243,7 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     for (int s = 0; s < NV; ++s) {
       tc5::mbar_init(bar(C::B_VF + s), 1);
       tc5::mbar_init(bar(C::B_VE + s), 1);
+      if (X) tc5::mbar_init(bar(C::B_VL + s), 1);
     }
     *abort_flag = 0;
     tc5::mbar_fence_init();
@@ -1251,16 +1285,17 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
           tc5::mbar_arrive_expect_tx(bar(C::B_KF + kr.slot), TILE);
 #pragma unroll
           for (int pp = 0; pp < HP; ++pp)
-            tc5::tma_load_4d(base + OFF_K + kr.slot * TILE + pp * PANEL, &map_k, pp * 64, h, t * 128, b, bar(C::B_KF + kr.slot));
+            tc5::tma_load_4d(base + OFF_K + kr.slot * TILE + pp * PANEL, &map_k, pp * 64, X ? h / p.rep : h, t * 128, b, bar(C::B_KF + kr.slot));
           kr.next();
         }
         if (waiting == 2 || !more) {
           const int b = vbh0 / p.heads, h = vbh0 - b * p.heads;
           if (!wait(bar(C::B_VE + vr.slot), vr.phase ^ 1u)) break;
-          tc5::mbar_arrive_expect_tx(bar(C::B_VF + vr.slot), TILE);
+          const int landed = X && ends_inside(vt0, row_length(p, b), p.seqlen) ? C::B_VL + vr.slot : C::B_VF + vr.slot;
+          tc5::mbar_arrive_expect_tx(bar(landed), TILE);
 #pragma unroll
           for (int pp = 0; pp < HP; ++pp)
-            tc5::tma_load_4d(base + OFF_V + vr.slot * TILE + pp * PANEL, &map_v, pp * 64, h, vt0 * 128, b, bar(C::B_VF + vr.slot));
+            tc5::tma_load_4d(base + OFF_V + vr.slot * TILE + pp * PANEL, &map_v, pp * 64, X ? h / p.rep : h, vt0 * 128, b, bar(landed));
           vr.next();
           vt0 = vt1;
           vbh0 = vbh1;
@@ -1324,6 +1359,19 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         vr.next();
         v_ready = tc5::mbar_test(bar(C::B_VF + vr.slot), vr.phase);
       }
+    } else if (X && warp == 3 && p.lengths) {
+      // ---------------------------------------------------------------- V rows behind the end of their sequence
+      Ring<NV> vr;
+      uint32_t landed = 0u;    // bit s: parity of the next such tile in slot s
+      for (FwdSeq seq(items); seq.more(); seq.advance(items), vr.next()) {
+        const int t = seq.cur.t, len = seq.cur.item.len;
+        if (!ends_inside(t, len, p.seqlen)) continue;
+        if (!wait_warp(bar(C::B_VL + vr.slot), (landed >> vr.slot) & 1u)) break;
+        landed ^= 1u << vr.slot;
+        clear_rows<HP>(base + OFF_V + vr.slot * TILE, PANEL, len - t * 128);
+        __syncwarp();
+        if (lane == 0) tc5::mbar_arrive(bar(C::B_VF + vr.slot));
+      }
     }
   } else {
     regs_softmax<kFwdAux>();
@@ -1344,8 +1392,11 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const int b = bh / p.heads, h = bh - b * p.heads;
       const int q0 = qt * 128;
       const int grow = q0 + row;
-      const int lim = p.causal ? min(grow, p.seqlen - 1) : p.seqlen - 1;    // last visible column
-      const int wlim = p.causal ? min(q0 + qd * 32 + 31, p.seqlen - 1) : p.seqlen - 1;    // the same for the warp's last row
+      const int len = X ? item.len : p.seqlen;
+      int lim = p.causal ? min(grow, len - 1) : len - 1;    // last visible column
+      int wlim = p.causal ? min(q0 + qd * 32 + 31, len - 1) : len - 1;    // the same for the warp's last row
+      if (X && grow >= len) lim = -1;    // padding sees nothing
+      if (X && q0 + qd * 32 >= len) wlim = -1;
       float m[NA], l[NA];    // running maximum (log2 units) and row sum
 #pragma unroll
       for (int a = 0; a < NA; ++a) {
@@ -1363,7 +1414,7 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         __syncwarp();
         if (lane == 0) tc5::mbar_arrive(bar(C::B_SE));    // the score slot may take the next tile
         const int col0 = t * 128;
-        const bool need_mask = (p.causal && col0 + 127 > q0) || (col0 + 128 > p.seqlen);
+        const bool need_mask = (p.causal && col0 + 127 > q0) || (col0 + 128 > len) || (X && q0 + 128 > len);
         // 32-column chunks in which any row of this warp sees a key
         const int nch = need_mask ? min(4, (wlim - col0) / 32 + 1) : 4;
         const int rel = lim - col0;    // last visible column of this row
@@ -1503,6 +1554,10 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 #pragma unroll
             for (int i = 0; i < 64; ++i) v[i] = a ? fmaf(__uint_as_float(x[i >> 5][i & 31]), fa, v[i]) : __uint_as_float(x[i >> 5][i & 31]) * fa;
           }
+          if (X && lim < 0) {    // a row that sees nothing is zero, whatever the values hold
+#pragma unroll
+            for (int i = 0; i < 64; ++i) v[i] = 0.0f;
+          }
           st_rows64(dst + c, p.o_ss, rows, v);
         }
         tc5::fence_before_sync();    // the next item's first P is handed over after these reads
@@ -1544,6 +1599,10 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
               const float o0 = __uint_as_float(a0[i]) * g0;
               v[i] = fmaf(n_t > 1 ? __uint_as_float(a1[i]) : 0.0f, g1, a ? v[i] + o0 : o0);
             }
+          }
+          if (X && lim < 0) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
           }
           if (row < p.seqlen - q0) st_row32(dst + (int64_t)lane * p.o_ss + col, v);
         }
@@ -2613,7 +2672,7 @@ attn_bwd_dq_tm_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 // ============================================================================ dQ, persistent CTAs over the work items
 namespace dqk3 {
 using namespace dqk2;
-enum { B3_QE = NBAR, B3_OE = NBAR + 1, NBAR3 = NBAR + 2 };
+enum { B3_QE = NBAR, B3_OE = NBAR + 1, B3_KL = NBAR + 2, NBAR3 = B3_KL + NK };
 template <int D>
 struct Cfg {
   static constexpr int HP = D / 64;
@@ -2630,7 +2689,9 @@ struct Cfg {
 // its first score products issued while the softmax warps still store dQ of the current one.  B3_QE: the score products
 // of an item are complete, Q and dO may be overwritten; B3_OE: the softmax warps have read dQ, the accumulator may be
 // overwritten by the first product of the next item.
-template <int D>
+// X: shared key / value heads and row lengths as in the forward kernel; the K tiles with rows behind the end of their sequence land on
+// B3_KL and warp 3 clears those rows.  A query tile behind the end has no tiles: its rows are stored as zeros.
+template <int D, bool X>
 __global__ void __launch_bounds__(kPsThreads, 1)
 attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const TcParams p, int n_qt,
@@ -2658,8 +2719,10 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const int c = (w & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x;
     return w * (int)gridDim.x + c;
   };
-  auto tiles_of = [&](int qt) {
-    const int n_kv = p.causal ? min(2 * qt + 2, nk_all) : nk_all;
+  auto tiles_of = [&](int qt, int len) {
+    if (X && qt * 128 >= len) return 0;
+    const int n_len = X ? (len + 63) / 64 : nk_all;
+    const int n_kv = p.causal ? min(2 * qt + 2, n_len) : n_len;
     return (n_kv + 1) >> 1;
   };
 
@@ -2682,6 +2745,8 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     tc5::mbar_init(bar(B_ACC), 1);
     tc5::mbar_init(bar(B3_QE), 1);
     tc5::mbar_init(bar(B3_OE), 8);
+    if (X)
+      for (int s = 0; s < NK; ++s) tc5::mbar_init(bar(B3_KL + s), 1);
     *abort_flag = 0;
     tc5::mbar_fence_init();
     tc5::tma_prefetch_desc(&map_q);
@@ -2710,7 +2775,9 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         order.decode(item, level, bh);
         const int qt = n_qt - 1 - level;
         const int b = bh / p.heads, h = bh - b * p.heads;
-        const int n_t = tiles_of(qt);
+        const int len = X ? row_length(p, b) : 0;
+        const int n_t = tiles_of(qt, len);
+        if (X && n_t == 0) continue;
         if (it > 0 && !tc5::mbar_wait(bar(B3_QE), (uint32_t)(it - 1) & 1u, abort_flag, p.status, kStatusBit)) break;
         tc5::mbar_arrive_expect_tx(bar(B_Q), 2 * TILE);
 #pragma unroll
@@ -2721,13 +2788,14 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         for (int t = 0; t < n_t; ++t, ++gt) {
           const int ks = gt % NK, vs = gt % NV;
           if (!tc5::mbar_wait(bar(B_KE + ks), ((uint32_t)(gt / NK) & 1u) ^ 1u, abort_flag, p.status, kStatusBit)) { ok = false; break; }
-          tc5::mbar_arrive_expect_tx(bar(B_KF + ks), TILE);
+          const int landed = X && ends_inside(t, len, p.seqlen) ? B3_KL + ks : B_KF + ks;
+          tc5::mbar_arrive_expect_tx(bar(landed), TILE);
 #pragma unroll
-          for (int pp = 0; pp < HP; ++pp) tc5::tma_load_4d(base + OFF_K + ks * TILE + pp * PANEL, &map_k, pp * 64, h, t * 128, b, bar(B_KF + ks));
+          for (int pp = 0; pp < HP; ++pp) tc5::tma_load_4d(base + OFF_K + ks * TILE + pp * PANEL, &map_k, pp * 64, X ? h / p.rep : h, t * 128, b, bar(landed));
           if (!tc5::mbar_wait(bar(B_VE + vs), ((uint32_t)(gt / NV) & 1u) ^ 1u, abort_flag, p.status, kStatusBit)) { ok = false; break; }
           tc5::mbar_arrive_expect_tx(bar(B_VF + vs), TILE);
 #pragma unroll
-          for (int pp = 0; pp < HP; ++pp) tc5::tma_load_4d(base + OFF_V + vs * TILE + pp * PANEL, &map_v, pp * 64, h, t * 128, b, bar(B_VF + vs));
+          for (int pp = 0; pp < HP; ++pp) tc5::tma_load_4d(base + OFF_V + vs * TILE + pp * PANEL, &map_v, pp * 64, X ? h / p.rep : h, t * 128, b, bar(B_VF + vs));
         }
         ++it;
       }
@@ -2774,7 +2842,8 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         if (item >= n_items) continue;
         int level, bh;
         order.decode(item, level, bh);
-        const int n_t = tiles_of(n_qt - 1 - level);
+        const int n_t = tiles_of(n_qt - 1 - level, X ? row_length(p, bh / p.heads) : 0);
+        if (X && n_t == 0) continue;
         if (!tc5::mbar_wait(bar(B_Q), (uint32_t)it & 1u, abort_flag, p.status, kStatusBit)) { ok = false; break; }
         if (!issue_s(g0)) { ok = false; break; }
         if (n_t == 1) tc5::mma_commit(bar(B3_QE));
@@ -2802,6 +2871,27 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         g0 += n_t;
         ++it;
       }
+    } else if (X && warp == 3 && p.lengths) {
+      // K rows behind the end of their sequence
+      Ring<NK> kr;
+      uint32_t landed = 0u;    // bit s: parity of the next such tile in slot s
+      bool ok = true;
+      for (int w = 0; w < n_waves && ok; ++w) {
+        const int item = item_at(w);
+        if (item >= n_items) continue;
+        int level, bh;
+        order.decode(item, level, bh);
+        const int len = row_length(p, bh / p.heads);
+        const int n_t = tiles_of(n_qt - 1 - level, len);
+        for (int t = 0; t < n_t; ++t, kr.next()) {
+          if (!ends_inside(t, len, p.seqlen)) continue;
+          if (!wait_warp(bar(B3_KL + kr.slot), (landed >> kr.slot) & 1u)) { ok = false; break; }
+          landed ^= 1u << kr.slot;
+          clear_rows<HP>(base + OFF_K + kr.slot * TILE, PANEL, len - t * 128);
+          __syncwarp();
+          if (lane == 0) tc5::mbar_arrive(bar(B_KF + kr.slot));
+        }
+      }
     }
   } else {
     regs_softmax<88>();
@@ -2819,21 +2909,32 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       order.decode(item, level, bh);
       const int qt = n_qt - 1 - level;
       const int b = bh / p.heads, h = bh - b * p.heads;
-      const int n_t = tiles_of(qt);
+      const int len = X ? row_length(p, b) : p.seqlen;
+      const int n_t = tiles_of(qt, len);
       const int q0 = qt * 128;
       const int grow = q0 + row;
-      const bool in = grow < p.seqlen;
+      const bool in = grow < len;
+      if (X && n_t == 0) {
+        float v[64];
+#pragma unroll
+        for (int i = 0; i < 64; ++i) v[i] = 0.0f;
+        if (wg < HP)
+          st_rows64(p.dq + (int64_t)b * p.dq_sb + (int64_t)(q0 + qd * 32) * p.dq_ss + (int64_t)h * p.dq_sh + wg * 64, p.dq_ss,
+                    p.seqlen - q0 - qd * 32, v);
+        continue;
+      }
       const float lse2 = in ? p.lse[(int64_t)bh * p.seqlen + grow] * kLog2e : INFINITY;
       const float dlt = in ? p.delta[(int64_t)bh * p.seqlen + grow] : 0.0f;
       const uint64_t sl2 = f2_pack(sl, sl), nlse2 = f2_pack(-lse2, -lse2), ndlt2 = f2_pack(-dlt, -dlt);
-      const int lim = p.causal ? min(grow, p.seqlen - 1) : p.seqlen - 1;
+      int lim = p.causal ? min(grow, len - 1) : len - 1;
+      if (X && !in) lim = -1;
       for (int t = 0; t < n_t; ++t) {
         const int gt = g0 + t;
         const int col0 = (2 * t + wg) * 64;
         const uint32_t tdp = tlane + TM_DP + (uint32_t)(gt & 1) * 128u + (uint32_t)wg * 64u;
         if (!wait_warp(bar(B_SF), (uint32_t)gt & 1u)) { ok = false; break; }
         tc5::fence_after_sync();
-        const bool need_mask = (p.causal && col0 + 63 > q0) || (col0 + 64 > p.seqlen);
+        const bool need_mask = (p.causal && col0 + 63 > q0) || (col0 + 64 > len) || (X && q0 + 128 > len);
         uint32_t rs[2][32], rd[2][32];    // the scores become probabilities while dP is still being computed
         tc5::tmem_ld32(tlane + TM_S + (uint32_t)wg * 64u, rs[0]);
         tc5::tmem_ld32(tlane + TM_S + (uint32_t)wg * 64u + 32u, rs[1]);
@@ -2855,6 +2956,7 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         tc5::tmem_ld32(tdp, rd[0]);
         tc5::tmem_ld32(tdp + 32u, rd[1]);
         tc5::tmem_ld_wait();
+        if (X && need_mask) mask_above(rd, lim - col0, 0u);    // dP of padding may be anything
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
@@ -2886,7 +2988,7 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (mine) {
         float v[64];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i >> 5][i & 31]) * p.scale;
+        for (int i = 0; i < 64; ++i) v[i] = X && !in ? 0.0f : __uint_as_float(r[i >> 5][i & 31]) * p.scale;
         st_rows64(dq + wg * 64, p.dq_ss, p.seqlen - q0 - qd * 32, v);
       }
       g0 += n_t;
@@ -2922,7 +3024,7 @@ struct Cfg {
                             OFF_LSE = OFF_PT + (PT_TMEM ? 0 : NB * TILE_P), OFF_BAR = OFF_LSE + ND * 2 * 128 * 4;
   static constexpr int B_KV = 0, B_QF = 1, B_QE = B_QF + NQ, B_OF = B_QE + NQ, B_OE = B_OF + ND, B_SF = B_OE + ND, B_SE = B_SF + 1, B_DF = B_SE + 1,
                        B_PF = B_DF + NB, B_PP = B_PF + NB, B_PE = B_PP + NB, B_ACC = B_PE + NB, B3_KVE = B_ACC + 1, B3_OE = B3_KVE + 1,
-                       NBAR = B3_OE + 1;
+                       B3_QL = B3_OE + 1, B3_OL = B3_QL + NQ, NBAR = B3_OL + ND;
   static constexpr int SMEM = OFF_BAR + NBAR * 8 + 16;    // head size 128: 848 bytes below the limit, so the base has to be aligned
   static constexpr uint32_t TM_ST = 0, TM_DPT = 128, TM_DV = TM_DPT + NB * 128, TM_DK = TM_DV + D, TM_COLS = 512;
   static_assert(SMEM <= 227 * 1024, "persistent dK/dV kernel: shared memory");
@@ -2938,7 +3040,11 @@ struct Cfg {
 // exponential, one barrier for P^T and dS^T, and stores of one row per lane before).
 // B3_KVE: every S^T / dP^T product of an item is complete, K and V may be overwritten by the next item's; B3_OE: the softmax
 // warps have read dV and dK, the first products of the next item may overwrite the accumulators.
-template <int D>
+// X: an item takes the query tiles of all (or, in `parts`, of some) query heads of its key / value head one after the other into the same
+// accumulators, so the sum over the heads is in 32 bits; parts leave theirs in `partial`, which attn_bwd_join_kernel adds up in order.
+// Q and dO tiles with rows behind the end of their sequence land on B3_QL and B3_OL and warp 3 clears those rows.  Key rows behind the
+// end are stored as zeros.
+template <int D, bool X>
 __global__ void __launch_bounds__(kPsThreads, 1)
 attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const TcParams p, int n_kt,
@@ -2949,7 +3055,7 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   constexpr uint32_t PANEL = C::PANEL, TILE = C::TILE, TILE_P = C::TILE_P, OFF_K = 0, OFF_V = C::OFF_V, OFF_Q = C::OFF_Q, OFF_DO = C::OFF_DO,
                      OFF_PT = C::OFF_PT, OFF_LSE = C::OFF_LSE, OFF_BAR = C::OFF_BAR;
   constexpr int B_KV = C::B_KV, B_QF = C::B_QF, B_QE = C::B_QE, B_OF = C::B_OF, B_OE = C::B_OE, B_SF = C::B_SF, B_SE = C::B_SE, B_DF = C::B_DF, B_PF = C::B_PF, B_PP = C::B_PP, B_PE = C::B_PE,
-                B_ACC = C::B_ACC, B3_KVE = C::B3_KVE, B3_OE = C::B3_OE;
+                B_ACC = C::B_ACC, B3_KVE = C::B3_KVE, B3_OE = C::B3_OE, B3_QL = C::B3_QL, B3_OL = C::B3_OL;
   constexpr uint32_t TM_ST = C::TM_ST, TM_DPT = C::TM_DPT, TM_DV = C::TM_DV, TM_DK = C::TM_DK, TM_COLS = C::TM_COLS;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = tc5::smem_u32(smem);
@@ -2969,7 +3075,34 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int nq_all = (p.seqlen + 127) / 128;
-  const ItemOrder order{n_kt, p.batch * p.heads, p.group};
+  const ItemOrder order{n_kt, X ? p.batch * p.kv_heads * p.parts : p.batch * p.heads, p.group};
+  const int per_item = X ? p.rep / p.parts : 1;    // query heads of an item
+  // Work item -> its batch, first query head, key / value head and query tiles (n_q for each of the query heads)
+  struct Item {
+    int kt, b, h, hk, part, len, t_first, n_q, n_u;
+  };
+  auto open_item = [&](int item) {
+    Item x;
+    int idx;
+    order.decode(item, x.kt, idx);
+    if (X) {
+      const int bk = idx / p.parts;
+      x.part = idx - bk * p.parts;
+      x.b = bk / p.kv_heads;
+      x.hk = bk - x.b * p.kv_heads;
+      x.h = x.hk * p.rep + x.part * per_item;
+      x.len = row_length(p, x.b);
+    } else {
+      x.part = 0;
+      x.b = idx / p.heads;
+      x.h = x.hk = idx - x.b * p.heads;
+      x.len = p.seqlen;
+    }
+    x.t_first = p.causal ? x.kt : 0;
+    x.n_q = X ? (x.kt * 128 >= x.len ? 0 : (x.len + 127) / 128 - x.t_first) : nq_all - x.t_first;
+    x.n_u = X ? x.n_q * per_item : x.n_q;
+    return x;
+  };
   const int n_waves = (n_items + (int)gridDim.x - 1) / (int)gridDim.x;
   auto item_at = [&](int w) {
     const int c = (w & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x;
@@ -2997,6 +3130,10 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     tc5::mbar_init(bar(B_ACC), 1);
     tc5::mbar_init(bar(B3_KVE), 1);
     tc5::mbar_init(bar(B3_OE), 8);
+    if (X) {
+      for (int s = 0; s < NQ; ++s) tc5::mbar_init(bar(B3_QL + s), 1);
+      for (int s = 0; s < ND; ++s) tc5::mbar_init(bar(B3_OL + s), 1);
+    }
     *abort_flag = 0;
     tc5::mbar_fence_init();
     tc5::tma_prefetch_desc(&map_q);
@@ -3022,47 +3159,52 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     for (int w = 0; w < n_waves && ok; ++w) {
       const int item = item_at(w);
       if (item >= n_items) continue;
-      int kt, bh;
-      order.decode(item, kt, bh);
-      const int b = bh / p.heads, h = bh - b * p.heads;
-      const int k0 = kt * 128;
-      const int t_first = p.causal ? kt : 0;
-      const int n_q = nq_all - t_first;
+      const Item x = open_item(item);
+      const int b = x.b, k0 = x.kt * 128;
+      if (X && x.n_u == 0) continue;
       if (it > 0 && !__all_sync(0xffffffffu, tc5::mbar_wait(bar(B3_KVE), (uint32_t)(it - 1) & 1u, abort_flag, p.status, kStatusBit))) break;
       if (lane == 0) {
         tc5::mbar_arrive_expect_tx(bar(B_KV), 2 * TILE);
 #pragma unroll
         for (int pp = 0; pp < HP; ++pp) {
-          tc5::tma_load_4d(base + OFF_K + pp * PANEL, &map_k, pp * 64, h, k0, b, bar(B_KV));
-          tc5::tma_load_4d(base + OFF_V + pp * PANEL, &map_v, pp * 64, h, k0, b, bar(B_KV));
+          tc5::tma_load_4d(base + OFF_K + pp * PANEL, &map_k, pp * 64, x.hk, k0, b, bar(B_KV));
+          tc5::tma_load_4d(base + OFF_V + pp * PANEL, &map_v, pp * 64, x.hk, k0, b, bar(B_KV));
         }
       }
-      const float* glse = p.lse + (int64_t)bh * p.seqlen;
-      const float* gdelta = p.delta + (int64_t)bh * p.seqlen;
-      for (int t = 0; t < n_q; ++t, ++gq) {
+      int t = 0, h = x.h;    // query tile of its head, the head
+      for (int u = 0; u < x.n_u; ++u, ++gq) {
+        const float* glse = p.lse + ((int64_t)b * p.heads + h) * p.seqlen;
+        const float* gdelta = p.delta + ((int64_t)b * p.heads + h) * p.seqlen;
         const int s = gq % NQ, so = gq % ND;
-        const int qrow0 = (t_first + t) * 128;
+        const int qrow0 = (x.t_first + t) * 128;
         if (!__all_sync(0xffffffffu, tc5::mbar_wait(bar(B_QE + s), ((uint32_t)(gq / NQ) & 1u) ^ 1u, abort_flag, p.status, kStatusBit))) { ok = false; break; }
+        const bool clear = X && ends_inside(x.t_first + t, x.len, p.seqlen);
         if (lane == 0) {
-          tc5::mbar_arrive_expect_tx(bar(B_QF + s), TILE);
+          const int landed = clear ? B3_QL + s : B_QF + s;
+          tc5::mbar_arrive_expect_tx(bar(landed), TILE);
 #pragma unroll
-          for (int pp = 0; pp < HP; ++pp) tc5::tma_load_4d(base + OFF_Q + s * TILE + pp * PANEL, &map_q, pp * 64, h, qrow0, b, bar(B_QF + s));
+          for (int pp = 0; pp < HP; ++pp) tc5::tma_load_4d(base + OFF_Q + s * TILE + pp * PANEL, &map_q, pp * 64, h, qrow0, b, bar(landed));
         }
         if (!__all_sync(0xffffffffu, tc5::mbar_wait(bar(B_OE + so), ((uint32_t)(gq / ND) & 1u) ^ 1u, abort_flag, p.status, kStatusBit))) { ok = false; break; }
         if (lane == 0) {
-          tc5::mbar_arrive_expect_tx(bar(B_OF + so), TILE);
+          const int landed = clear ? B3_OL + so : B_OF + so;
+          tc5::mbar_arrive_expect_tx(bar(landed), TILE);
 #pragma unroll
-          for (int pp = 0; pp < HP; ++pp) tc5::tma_load_4d(base + OFF_DO + so * TILE + pp * PANEL, &map_do, pp * 64, h, qrow0, b, bar(B_OF + so));
+          for (int pp = 0; pp < HP; ++pp) tc5::tma_load_4d(base + OFF_DO + so * TILE + pp * PANEL, &map_do, pp * 64, h, qrow0, b, bar(landed));
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = lane + 32 * i;
-          const bool in = qrow0 + r < p.seqlen;
+          const bool in = qrow0 + r < x.len;
           s_lse[so * 128 + r] = in ? -(glse[qrow0 + r] * kLog2e) : -INFINITY;    // -inf makes the probability exactly zero
           s_delta[so * 128 + r] = in ? -gdelta[qrow0 + r] : 0.0f;
         }
         __syncwarp();
         if (lane == 0) tc5::mbar_arrive(bar(B_OF + so));
+        if (++t == x.n_q) {
+          t = 0;
+          ++h;
+        }
       }
       ++it;
     }
@@ -3129,9 +3271,9 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       for (int w = 0; w < n_waves && ok; ++w) {
         const int item = item_at(w);
         if (item >= n_items) continue;
-        int kt, bh;
-        order.decode(item, kt, bh);
-        const int n_q = nq_all - (p.causal ? kt : 0);
+        const Item x = open_item(item);
+        const int n_q = x.n_u;
+        if (X && n_q == 0) continue;
         if (!tc5::mbar_wait(bar(B_KV), (uint32_t)it & 1u, abort_flag, p.status, kStatusBit)) { ok = false; break; }
         if (!wait_for(B_QF + g0 % NQ, g0 / NQ)) { ok = false; break; }
         if (!PT_TMEM && g0 > 0 && !wait_for(B_SE, g0 - 1)) { ok = false; break; }
@@ -3181,6 +3323,32 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         g0 += n_q;
         ++it;
       }
+    } else if (X && warp == 3 && p.lengths) {
+      // ------------------------------------------------------------------ Q and dO rows behind the end of their sequence
+      int gq = 0;
+      uint32_t landed_q = 0u, landed_o = 0u;    // bit s: parity of the next such tile in slot s
+      bool ok = true;
+      for (int w = 0; w < n_waves && ok; ++w) {
+        const int item = item_at(w);
+        if (item >= n_items) continue;
+        const Item x = open_item(item);
+        const int last = x.t_first + x.n_q - 1;    // query tile
+        const bool ragged = x.n_u > 0 && ends_inside(last, x.len, p.seqlen);
+        for (int n = x.n_q; ragged && n <= x.n_u; n += x.n_q) {
+          const int s = (gq + n - 1) % NQ, so = (gq + n - 1) % ND;    // the last tile of a head
+          if (!wait_warp(bar(B3_QL + s), (landed_q >> s) & 1u)) { ok = false; break; }
+          landed_q ^= 1u << s;
+          clear_rows<HP>(base + OFF_Q + s * TILE, PANEL, x.len - last * 128);
+          __syncwarp();
+          if (lane == 0) tc5::mbar_arrive(bar(B_QF + s));
+          if (!wait_warp(bar(B3_OL + so), (landed_o >> so) & 1u)) { ok = false; break; }
+          landed_o ^= 1u << so;
+          clear_rows<HP>(base + OFF_DO + so * TILE, PANEL, x.len - last * 128);
+          __syncwarp();
+          if (lane == 0) tc5::mbar_arrive(bar(B_OF + so));
+        }
+        gq += x.n_u;
+      }
     }
   } else {
     regs_softmax<88>();
@@ -3191,6 +3359,15 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const uint32_t tlane = tmem_base + ((uint32_t)(qd * 32) << 16);
     const float sl = p.scale * kLog2e;
     const uint64_t sl2 = f2_pack(sl, sl);
+    // X: rows of a key tile behind the end of its sequence
+    auto store_zeros = [&](int item) {
+      const Item x = open_item(item);
+      const int r0 = x.kt * 128 + qd * 32;
+      const int64_t ss = wg == 0 ? p.dv_ss : p.dk_ss;
+      __nv_bfloat16* dst = wg == 0 ? p.dv + (int64_t)x.b * p.dv_sb + (int64_t)x.hk * p.dv_sh : p.dk + (int64_t)x.b * p.dk_sb + (int64_t)x.hk * p.dk_sh;
+      if (r0 + lane < p.seqlen)
+        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(dst + (r0 + lane) * ss + c) = make_uint4(0u, 0u, 0u, 0u);
+    };
     const uint32_t prow0 = base + OFF_PT + (uint32_t)wg * PANEL + (uint32_t)row * 128u;
     const uint32_t swz = (uint32_t)(row & 7);
     int g0 = 0, it = 0;
@@ -3198,17 +3375,26 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     for (int w = 0; w < n_waves && ok; ++w) {
       const int item = item_at(w);
       if (item >= n_items) continue;
-      int kt, bh;
-      order.decode(item, kt, bh);
-      const int b = bh / p.heads, h = bh - b * p.heads;
-      const int k0 = kt * 128;
+      int k0, n_q, t_first, n_head;    // n_q query tiles, n_head of each query head
+      {
+        const Item x = open_item(item);
+        k0 = x.kt * 128;
+        n_q = x.n_u;
+        t_first = x.t_first;
+        n_head = x.n_q;
+      }
+      if (X && n_q == 0) {    // padding only
+        if (p.parts == 1) store_zeros(item);
+        continue;
+      }
       const int grow = k0 + row;
-      const int t_first = p.causal ? kt : 0;
-      const int n_q = nq_all - t_first;
-      for (int t = 0; t < n_q; ++t) {
-        const int gq = g0 + t;
+      int t = 0;    // query tile of its head
+      for (int u = 0; u < n_q; ++u) {
+        const int gq = g0 + u;
         const int so = gq % ND;
         const int qrow0 = (t_first + t) * 128 + wg * 64;    // first query of this group's half
+        if (X && ++t == n_head) t = 0;
+        if (!X) ++t;
         if (!wait_warp(bar(B_OF + so), (uint32_t)(gq / ND) & 1u)) { ok = false; break; }
         if (!wait_warp(bar(B_SF), (uint32_t)gq & 1u)) { ok = false; break; }
         tc5::fence_after_sync();
@@ -3289,6 +3475,10 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       if (!ok || !wait_warp(bar(B_ACC), (uint32_t)it & 1u)) { ok = false; break; }
       tc5::fence_after_sync();
       // group 0 stores dV, group 1 stores dK: read the whole accumulator first, so that it is free for the next item
+      int again = item;
+      if (X) asm volatile("" : "+r"(again));    // what only the end of an item needs is worked out again, not held through its tiles
+      const Item x = open_item(again);
+      const int b = x.b, h = x.hk;
       __nv_bfloat16* dst = wg == 0 ? p.dv + (int64_t)b * p.dv_sb + (int64_t)(k0 + qd * 32) * p.dv_ss + (int64_t)h * p.dv_sh
                                    : p.dk + (int64_t)b * p.dk_sb + (int64_t)(k0 + qd * 32) * p.dk_ss + (int64_t)h * p.dk_sh;
       const float f = wg == 0 ? 1.0f : p.scale;
@@ -3300,15 +3490,28 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       tc5::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc5::mbar_arrive(bar(B3_OE));
+      g0 += n_q;
+      ++it;
+      const bool in = !X || grow < x.len;
+      if (X && p.parts > 1) {
+        if (in) {
+          float* out = p.partial + ((((int64_t)x.part * 2 + 1 - wg) * p.batch + b) * p.kv_heads + h) * p.seqlen * D + (int64_t)grow * D;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(out + c * 32 + i) = make_float4(__uint_as_float(acc[c][i]) * f, __uint_as_float(acc[c][i + 1]) * f,
+                                                                         __uint_as_float(acc[c][i + 2]) * f, __uint_as_float(acc[c][i + 3]) * f);
+        }
+        continue;
+      }
 #pragma unroll
       for (int c = 0; c < D / 32; c += 2) {
         float v[64];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(acc[c + (i >> 5)][i & 31]) * f;
+        for (int i = 0; i < 64; ++i) v[i] = in ? __uint_as_float(acc[c + (i >> 5)][i & 31]) * f : 0.0f;
         st_rows64(dst + c * 32, wg == 0 ? p.dv_ss : p.dk_ss, p.seqlen - k0 - qd * 32, v);
       }
-      g0 += n_q;
-      ++it;
     }
   }
 
@@ -3318,6 +3521,39 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   __syncthreads();
   tc5::fence_after_sync();
   if (warp == 1) tc5::tmem_dealloc(tmem_base, TM_COLS);
+}
+
+// dK and dV of the parts of a work item, added up in order: bound by memory.
+struct JoinParams {
+  const float* partial;
+  __nv_bfloat16 *dk, *dv;
+  int64_t dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
+  int parts, batch, kv_heads, seqlen;
+  const int* lengths;
+};
+template <int D>
+__global__ void __launch_bounds__(256) attn_bwd_join_kernel(const JoinParams p) {
+  constexpr int L = D / 8;    // threads of a row, eight elements each
+  const int64_t rows = (int64_t)p.batch * p.kv_heads * p.seqlen;
+  const int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  if (r >= 2 * rows) return;
+  const bool is_v = r >= rows;
+  const int64_t row = is_v ? r - rows : r;
+  const int c = (threadIdx.x % L) * 8;
+  const int s = (int)(row % p.seqlen);
+  const int64_t bh = row / p.seqlen;
+  const int h = (int)(bh % p.kv_heads);
+  const int64_t b = bh / p.kv_heads;
+  const int parts = p.lengths && s >= __ldg(p.lengths + b) ? 0 : p.parts;    // nothing was left for padding
+  float v[8] = {};
+  for (int k = 0; k < parts; ++k) {
+    const float4* src = reinterpret_cast<const float4*>(p.partial + ((int64_t)k * 2 * rows + r) * D + c);
+    const float4 a = src[0], b = src[1];
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+  __nv_bfloat16* dst = is_v ? p.dv + b * p.dv_sb + (int64_t)s * p.dv_ss + (int64_t)h * p.dv_sh : p.dk + b * p.dk_sb + (int64_t)s * p.dk_ss + (int64_t)h * p.dk_sh;
+  *reinterpret_cast<uint4*>(dst + c) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
 }
 
 // ---- host side -----------------------------------------------------------------------------------
@@ -3533,11 +3769,11 @@ MSAMP_API int msamp_attention_tc_fwd(const void* q, const void* k, const void* v
     return msamp_check_launch("attn_fwd_split_kernel");
   }
   if (head_dim == 128) {
-    if ((rc = set_smem(attn_fwd_ps_kernel<128>, fwd3::Cfg<128>::SMEM))) return rc;
-    attn_fwd_ps_kernel<128><<<ctas, kPsThreads, fwd3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
+    if ((rc = set_smem(attn_fwd_ps_kernel<128, false>, fwd3::Cfg<128>::SMEM))) return rc;
+    attn_fwd_ps_kernel<128, false><<<ctas, kPsThreads, fwd3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
   } else {
-    if ((rc = set_smem(attn_fwd_ps_kernel<64>, fwd3::Cfg<64>::SMEM))) return rc;
-    attn_fwd_ps_kernel<64><<<ctas, kPsThreads, fwd3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
+    if ((rc = set_smem(attn_fwd_ps_kernel<64, false>, fwd3::Cfg<64>::SMEM))) return rc;
+    attn_fwd_ps_kernel<64, false><<<ctas, kPsThreads, fwd3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
   }
   return msamp_check_launch("attn_fwd_ps_kernel");
 }
@@ -3608,15 +3844,135 @@ MSAMP_API int msamp_attention_tc_bwd(const void* q, const void* k, const void* v
     if ((rc = set_smem(attn_bwd_dq_tm_kernel, dqk2::SMEM))) return rc;
     attn_bwd_dq_tm_kernel<<<grid, kTcThreads, dqk2::SMEM, stream>>>(mq, mk, mv, mdo, p);
   } else if (head_dim == 128) {
-    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<128>, dkv3::Cfg<128>::SMEM))) return rc;
-    attn_bwd_dkdv_ps_kernel<128><<<ctas, kPsThreads, dkv3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
-    if ((rc = set_smem(attn_bwd_dq_ps_kernel<128>, dqk3::Cfg<128>::SMEM))) return rc;
-    attn_bwd_dq_ps_kernel<128><<<ctas, kPsThreads, dqk3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
+    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<128, false>, dkv3::Cfg<128>::SMEM))) return rc;
+    attn_bwd_dkdv_ps_kernel<128, false><<<ctas, kPsThreads, dkv3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
+    if ((rc = set_smem(attn_bwd_dq_ps_kernel<128, false>, dqk3::Cfg<128>::SMEM))) return rc;
+    attn_bwd_dq_ps_kernel<128, false><<<ctas, kPsThreads, dqk3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
   } else {
-    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<64>, dkv3::Cfg<64>::SMEM))) return rc;
-    attn_bwd_dkdv_ps_kernel<64><<<ctas, kPsThreads, dkv3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
-    if ((rc = set_smem(attn_bwd_dq_ps_kernel<64>, dqk3::Cfg<64>::SMEM))) return rc;
-    attn_bwd_dq_ps_kernel<64><<<ctas, kPsThreads, dqk3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
+    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<64, false>, dkv3::Cfg<64>::SMEM))) return rc;
+    attn_bwd_dkdv_ps_kernel<64, false><<<ctas, kPsThreads, dkv3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
+    if ((rc = set_smem(attn_bwd_dq_ps_kernel<64, false>, dqk3::Cfg<64>::SMEM))) return rc;
+    attn_bwd_dq_ps_kernel<64, false><<<ctas, kPsThreads, dqk3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
   }
   return msamp_check_launch("attn_bwd_tc kernels");
+}
+
+// ---- shared key / value heads and row lengths ----------------------------------------------------
+// Query heads h * rep .. h * rep + rep - 1 read key / value head h (heads == kv_heads * rep).  lengths [batch] (int32, or null): positions at or
+// behind a row's length are padding, as queries and as keys; their outputs and gradients are zero, their lse -inf, whatever they hold.
+// Strides as for the entry points above, those of k, v, dk and dv over kv_heads.
+static int shared_checks(const char* what, int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, const int64_t* strides, int n) {
+  MSAMP_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128 (got %d)", what, head_dim);
+  MSAMP_REQUIRE(batch > 0 && heads > 0 && kv_heads > 0 && seqlen > 0, "%s: empty problem", what);
+  MSAMP_REQUIRE(heads % kv_heads == 0, "%s: %d query heads do not share %d key / value heads evenly", what, heads, kv_heads);
+  MSAMP_REQUIRE(scale > 0.0f && scale <= 3.0e38f, "%s: the scale must be positive", what);
+  // work items and query tiles are counted in 32 bits
+  MSAMP_REQUIRE((int64_t)((seqlen + 127) / 128) * batch * heads <= (1 << 30), "%s: too many work items", what);
+  for (int i = 0; i < n; ++i) MSAMP_REQUIRE(strides[i] % 8 == 0, "%s: stride %d is not a multiple of 8 elements", what, i);
+  return MSAMP_OK;
+}
+
+MSAMP_API int msamp_attention_shared_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* lengths, const int64_t* strides,
+                                         int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, int causal, void* stream_) {
+  int rc = shared_checks("attention (shared heads)", batch, heads, kv_heads, seqlen, head_dim, scale, strides, 12);
+  if (rc) return rc;
+  MSAMP_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "attention (shared heads): q, k, v and o must be 16-byte aligned");
+  CUtensorMap mq, mk, mv;
+  if ((rc = make_map4(q, batch, heads, seqlen, head_dim, strides[0], strides[1], strides[2], 128, &mq))) return rc;
+  if ((rc = make_map4(k, batch, kv_heads, seqlen, head_dim, strides[3], strides[4], strides[5], 128, &mk))) return rc;
+  if ((rc = make_map4(v, batch, kv_heads, seqlen, head_dim, strides[6], strides[7], strides[8], 128, &mv))) return rc;
+  TcParams p = {};
+  p.o = (__nv_bfloat16*)o; p.lse = lse;
+  p.o_sb = strides[9]; p.o_ss = strides[10]; p.o_sh = strides[11];
+  p.batch = batch; p.heads = heads; p.seqlen = seqlen; p.causal = causal; p.scale = scale;
+  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.lengths = lengths;
+  p.status = msamp_device_status_ptr();
+  p.group = item_group(seqlen, head_dim);
+  const int n_qt = (seqlen + 127) / 128;
+  const int n_items = n_qt * batch * heads;
+  const int ctas = n_items < msamp_sm_count() ? n_items : msamp_sm_count();
+  cudaStream_t stream = (cudaStream_t)stream_;
+  if (head_dim == 128) {
+    if ((rc = set_smem(attn_fwd_ps_kernel<128, true>, fwd3::Cfg<128>::SMEM))) return rc;
+    attn_fwd_ps_kernel<128, true><<<ctas, kPsThreads, fwd3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
+  } else {
+    if ((rc = set_smem(attn_fwd_ps_kernel<64, true>, fwd3::Cfg<64>::SMEM))) return rc;
+    attn_fwd_ps_kernel<64, true><<<ctas, kPsThreads, fwd3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
+  }
+  return msamp_check_launch("attn_fwd_ps_kernel (shared heads)");
+}
+
+// Parts into which the query heads of a key / value head are cut for dK / dV: the smallest divisor of `rep` that gives every SM an item.
+MSAMP_API int msamp_attention_shared_parts(int batch, int heads, int kv_heads, int seqlen) {
+  const int rep = heads / kv_heads;
+  const int64_t items = (int64_t)((seqlen + 127) / 128) * batch * kv_heads;
+  for (int n = 1; n < rep; ++n)
+    if (rep % n == 0 && items * n >= msamp_sm_count()) return n;
+  return rep;
+}
+
+// partial: parts * 2 * batch * kv_heads * seqlen * head_dim floats when msamp_attention_shared_parts gives more than one part.
+MSAMP_API int msamp_attention_shared_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq,
+                                         void* dk, void* dv, float* delta, float* partial, const int* lengths, const int64_t* strides, int batch,
+                                         int heads, int kv_heads, int seqlen, int head_dim, float scale, int causal, void* stream_) {
+  int rc = shared_checks("attention (shared heads)", batch, heads, kv_heads, seqlen, head_dim, scale, strides, 24);
+  if (rc) return rc;
+  MSAMP_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(d_o) && aligned16(dq) && aligned16(dk) && aligned16(dv),
+                "attention (shared heads): q, k, v, o, dO and the gradients must be 16-byte aligned");
+  const int parts = msamp_attention_shared_parts(batch, heads, kv_heads, seqlen);
+  MSAMP_REQUIRE(parts == 1 || (partial && aligned16(partial)), "attention (shared heads): no workspace for %d parts", parts);
+  CUtensorMap mq, mk, mv, mdo;
+  if ((rc = make_map4(q, batch, heads, seqlen, head_dim, strides[0], strides[1], strides[2], 128, &mq))) return rc;
+  if ((rc = make_map4(k, batch, kv_heads, seqlen, head_dim, strides[3], strides[4], strides[5], 128, &mk))) return rc;
+  if ((rc = make_map4(v, batch, kv_heads, seqlen, head_dim, strides[6], strides[7], strides[8], 128, &mv))) return rc;
+  if ((rc = make_map4(d_o, batch, heads, seqlen, head_dim, strides[12], strides[13], strides[14], 128, &mdo))) return rc;
+  cudaStream_t stream = (cudaStream_t)stream_;
+  {
+    DeltaParams d = {};
+    d.o = (const __nv_bfloat16*)o; d.d_o = (const __nv_bfloat16*)d_o; d.delta = delta;
+    d.o_sb = strides[9]; d.o_ss = strides[10]; d.o_sh = strides[11];
+    d.do_sb = strides[12]; d.do_ss = strides[13]; d.do_sh = strides[14];
+    d.batch = batch; d.heads = heads; d.seqlen = seqlen;
+    const int64_t rows = (int64_t)batch * heads * seqlen;
+    const int per_cta = 2 * 256 / (head_dim / 8);
+    const unsigned blocks = (unsigned)((rows + per_cta - 1) / per_cta);
+    if (head_dim == 128) attn_delta_tc_kernel<128><<<blocks, 256, 0, stream>>>(d);
+    else                 attn_delta_tc_kernel<64><<<blocks, 256, 0, stream>>>(d);
+  }
+  TcParams p = {};
+  p.lse = const_cast<float*>(lse); p.delta = delta;
+  p.dq = (__nv_bfloat16*)dq; p.dk = (__nv_bfloat16*)dk; p.dv = (__nv_bfloat16*)dv;
+  p.dq_sb = strides[15]; p.dq_ss = strides[16]; p.dq_sh = strides[17];
+  p.dk_sb = strides[18]; p.dk_ss = strides[19]; p.dk_sh = strides[20];
+  p.dv_sb = strides[21]; p.dv_ss = strides[22]; p.dv_sh = strides[23];
+  p.batch = batch; p.heads = heads; p.seqlen = seqlen; p.causal = causal; p.scale = scale;
+  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.lengths = lengths; p.parts = parts; p.partial = partial;
+  p.status = msamp_device_status_ptr();
+  p.group = item_group(seqlen, head_dim);
+  const int n_t = (seqlen + 127) / 128;    // key tiles of dK / dV, query tiles of dQ
+  const int n_q = n_t * batch * heads, n_k = n_t * batch * kv_heads * parts;
+  const int sms = msamp_sm_count();
+  if (head_dim == 128) {
+    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<128, true>, dkv3::Cfg<128>::SMEM))) return rc;
+    if ((rc = set_smem(attn_bwd_dq_ps_kernel<128, true>, dqk3::Cfg<128>::SMEM))) return rc;
+    attn_bwd_dkdv_ps_kernel<128, true><<<n_k < sms ? n_k : sms, kPsThreads, dkv3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_k);
+    attn_bwd_dq_ps_kernel<128, true><<<n_q < sms ? n_q : sms, kPsThreads, dqk3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_q);
+  } else {
+    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<64, true>, dkv3::Cfg<64>::SMEM))) return rc;
+    if ((rc = set_smem(attn_bwd_dq_ps_kernel<64, true>, dqk3::Cfg<64>::SMEM))) return rc;
+    attn_bwd_dkdv_ps_kernel<64, true><<<n_k < sms ? n_k : sms, kPsThreads, dkv3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_k);
+    attn_bwd_dq_ps_kernel<64, true><<<n_q < sms ? n_q : sms, kPsThreads, dqk3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_q);
+  }
+  if (parts > 1) {
+    JoinParams j = {};
+    j.partial = partial; j.dk = p.dk; j.dv = p.dv;
+    j.dk_sb = p.dk_sb; j.dk_ss = p.dk_ss; j.dk_sh = p.dk_sh; j.dv_sb = p.dv_sb; j.dv_ss = p.dv_ss; j.dv_sh = p.dv_sh;
+    j.lengths = lengths; j.parts = parts; j.batch = batch; j.kv_heads = kv_heads; j.seqlen = seqlen;
+    const int64_t rows = 2 * (int64_t)batch * kv_heads * seqlen;
+    const int per_cta = 256 / (head_dim / 8);
+    const unsigned blocks = (unsigned)((rows + per_cta - 1) / per_cta);
+    if (head_dim == 128) attn_bwd_join_kernel<128><<<blocks, 256, 0, stream>>>(j);
+    else                 attn_bwd_join_kernel<64><<<blocks, 256, 0, stream>>>(j);
+  }
+  return msamp_check_launch("attention backward (shared heads)");
 }

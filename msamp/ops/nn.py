@@ -391,14 +391,178 @@ def attention_qkv(qkv, causal=True, scale=None):
     return attention(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], causal=causal, scale=scale)
 
 
-def attention(q, k, v, causal=True, scale=None, grad_layout='separate'):
+# Attention whose query heads share key / value heads, on rows that may end early.  ``q [B, S, heads, d]``, ``k`` and ``v [B, S, kv_heads, d]``
+# as strided views, ``lengths`` int32 ``[B]`` or None.
+def _map_strides(t):
+    """(batch, seq, head) element strides for a tensor map; the stride of an axis of extent 1 is never used and may be any number."""
+    return [s if n > 1 else t.shape[3] for s, n in zip(t.stride()[:3], t.shape[:3])]
+
+
+def _mappable(t):
+    """``t``, or a copy of it where it repeats a batch, position or head (a tensor map has no zero stride)."""
+    return t.contiguous() if any(s == 0 and n > 1 for s, n in zip(t.stride()[:3], t.shape[:3])) else t
+
+
+def _shared_fwd(q, k, v, causal, scale, lengths):
+    B, S, nh, d = q.shape
+    o = torch.empty((B, S, nh, d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, nh, S), dtype=torch.float32, device=q.device)
+    st = _map_strides(q) + _map_strides(k) + _map_strides(v) + _map_strides(o) + [0] * 12
+    with native.on_device(q):
+        native.check(
+            native.lib().msamp_attention_shared_fwd(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), native.addr(lengths), _i64x24(*st), B, nh, k.shape[2], S,
+                d, scale, int(causal), native.raw_stream()
+            ), 'attention_fwd'
+        )
+    return o, lse
+
+
+def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths):
+    B, S, nh, d = q.shape
+    nkv = k.shape[2]
+    o, d_o = _rows16(_mappable(o)), _rows16(_mappable(d_o))
+    st = [x for t in (q, k, v, o, d_o, dq, dk, dv) for x in _map_strides(t)]
+    with native.on_device(q):
+        parts = native.lib().msamp_attention_shared_parts(B, nh, nkv, S)
+        delta = torch.empty((B, nh, S), dtype=torch.float32, device=q.device)
+        partial = torch.empty(parts * 2 * B * nkv * S * d, dtype=torch.float32, device=q.device) if parts > 1 else None
+        native.check(
+            native.lib().msamp_attention_shared_bwd(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                delta.data_ptr(), native.addr(partial), native.addr(lengths), _i64x24(*st), B, nh, nkv, S, d, scale, int(causal),
+                native.raw_stream()
+            ), 'attention_bwd'
+        )
+
+
+class _AttentionSharedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, causal, scale, grad_layout, lengths):
+        o, lse = _shared_fwd(q, k, v, causal, scale, lengths)
+        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        ctx.causal, ctx.scale, ctx.grad_layout = causal, scale, grad_layout
+        return o
+
+    @staticmethod
+    def backward(ctx, d_o):
+        q, k, v, o, lse, lengths = ctx.saved_tensors
+        q, k, v = (_rows16(t) for t in (q, k, v))    # saved tensors may come back with other strides
+        B, S, nh, d = q.shape
+        if ctx.grad_layout == 'packed':
+            buf = torch.empty((B, S, nh + 2 * k.shape[2], d), dtype=q.dtype, device=q.device)
+            dq, dk, dv = buf.split([nh, k.shape[2], k.shape[2]], dim=2)
+        else:
+            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, ctx.causal, ctx.scale, lengths)
+        return dq, dk, dv, None, None, None, None
+
+
+def _attention_plain(q, k, v, causal, scale, lengths):
+    """The same in torch operations on any device (the CPU form)."""
+    B, S, nh, d = q.shape
+    nkv = k.shape[2]
+    if lengths is not None:
+        valid = torch.arange(S, device=q.device) < lengths.to(q.device)[:, None]
+        q, k, v = (torch.where(valid[:, :, None, None], t, torch.zeros((), dtype=t.dtype, device=t.device)) for t in (q, k, v))
+    qf, kf, vf = (t.float().permute(0, 2, 1, 3) for t in (q, k, v))
+    if nkv != nh:
+        kf, vf = (t.repeat_interleave(nh // nkv, dim=1) for t in (kf, vf))
+    s = (qf @ kf.transpose(-1, -2)) * scale
+    if causal:
+        s = s.masked_fill(torch.ones(S, S, dtype=torch.bool, device=q.device).triu(1), float('-inf'))
+    if lengths is not None:
+        s = s.masked_fill(~valid[:, None, None, :], float('-inf'))
+        seen = valid[:, None, :, None]
+        s = torch.where(seen, s, torch.zeros((), device=q.device))    # padding sees nothing: cleared below
+        p = torch.where(seen, torch.softmax(s, dim=-1), torch.zeros((), device=q.device))
+    else:
+        p = torch.softmax(s, dim=-1)
+    out = (p @ vf).permute(0, 2, 1, 3).to(q.dtype)
+    if lengths is not None:    # keeps what the gradient holds at padding out of the products of the backward pass
+        out = torch.where(valid[:, :, None, None], out, torch.zeros((), dtype=out.dtype, device=out.device))
+    return out.contiguous()
+
+
+def attention_shared_fwd_raw(q, k, v, causal=True, scale=None, lengths=None):
+    """Forward pass of :func:`attention` with shared key/value heads or row lengths, without autograd: ``(o, lse or None)``."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    if _use_native(q) and q.numel():
+        q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
+        return _shared_fwd(q, k, v, causal, scale, lengths)
+    _check_shared(q, k, v, scale, lengths)
+    with torch.no_grad():
+        return _attention_plain(q, k, v, causal, scale, lengths), None
+
+
+def attention_shared_bwd_raw(q, k, v, o, lse, d_o, dq, dk, dv, causal=True, scale=None, lengths=None):
+    """Its gradients, written into ``dq``, ``dk`` and ``dv`` (views with unit inner stride and 16-byte aligned rows)."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    if _use_native(q) and q.numel():
+        q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths)
+        return
+    with torch.enable_grad():
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+        grads = torch.autograd.grad(_attention_plain(*leaves, causal, scale, lengths), leaves, d_o)
+    for dst, g in zip((dq, dk, dv), grads):
+        dst.copy_(g)
+
+
+def _check_shared(q, k, v, scale, lengths):
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+        raise ValueError(f'attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together')
+    if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
+        raise ValueError(f'attention: {q.shape[2]} query heads do not share {k.shape[2]} key/value heads evenly')
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise ValueError('attention: q, k and v must have one dtype and one device')
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f'attention: scale must be positive (got {scale})')
+    if lengths is not None:
+        if tuple(lengths.shape) != (q.shape[0], ) or lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f'attention: lengths must be an int32 or int64 tensor [{q.shape[0]}] (got {lengths.dtype} {tuple(lengths.shape)})')
+        if lengths.device != q.device:
+            raise ValueError('attention: lengths must be on the device of q')
+
+
+def _shared_operands(q, k, v, scale, lengths):
+    """Checked operands of the CUDA kernels: mappable views, lengths in int32."""
+    _check_shared(q, k, v, scale, lengths)
+    d = q.shape[-1]
+    if q.dtype != torch.bfloat16 or d not in (64, 128):
+        raise RuntimeError(f'attention: CUDA kernel supports bf16 with head_dim 64/128 (got {q.dtype}, {d})')
+    q, k, v = (_mappable(t) for t in (q, k, v))
+    for t in (q, k, v):
+        if t.stride(3) != 1 or any(s % 8 for s in _map_strides(t)) or t.data_ptr() % 16:
+            raise RuntimeError('attention: operands must have unit inner stride and 16-byte aligned rows')
+    if lengths is not None:
+        lengths = lengths.to(torch.int32).contiguous()
+    return q, k, v, lengths
+
+
+def _attention_shared(q, k, v, causal, scale, grad_layout, lengths):
+    if not _use_native(q) or q.numel() == 0:
+        _check_shared(q, k, v, scale, lengths)
+        return _attention_plain(q, k, v, causal, scale, lengths)
+    q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
+    return _AttentionSharedFn.apply(q, k, v, bool(causal), float(scale), grad_layout, lengths)
+
+
+def attention(q, k, v, causal=True, scale=None, grad_layout='separate', lengths=None):
     """Softmax attention on ``[B, S, heads, head_dim]`` tensors; returns ``[B, S, heads, head_dim]``.
 
-    ``grad_layout='packed'`` makes backward return dq/dk/dv as views of one ``[B,S,3,heads,d]`` buffer
-    (use it when q, k, v are themselves views of a fused QKV tensor of that layout).
+    ``k`` and ``v`` may have fewer heads than ``q``: each of theirs then serves ``heads / kv_heads`` consecutive query heads, and its
+    gradient is the sum over those.  ``lengths`` (``[B]``, int32 or int64, on the device of ``q``) makes positions at or behind a row's
+    length padding: they are neither seen nor see, their outputs and gradients are zero, and whatever they hold stays out of every other
+    row; lengths outside ``0 .. S`` count as 0 or S.
+
+    ``grad_layout='packed'`` makes backward return dq/dk/dv as views of one ``[B,S,3,heads,d]`` buffer (``[B,S,heads + 2 kv_heads,d]`` with
+    shared heads or lengths; use it when q, k, v are themselves views of a fused QKV tensor of that layout).
     """
     d = q.shape[-1]
     scale = 1.0 / math.sqrt(d) if scale is None else scale
+    if lengths is not None or k.shape != q.shape:
+        return _attention_shared(q, k, v, causal, scale, grad_layout, lengths)
     if _use_native(q):
         if q.dtype != torch.bfloat16 or d not in (64, 128):
             raise RuntimeError(f'attention: CUDA kernel supports bf16 with head_dim 64/128 (got {q.dtype}, {d})')
@@ -406,13 +570,7 @@ def attention(q, k, v, causal=True, scale=None, grad_layout='separate'):
             if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
                 raise RuntimeError('attention: operands must have unit inner stride and 16-byte aligned rows')
         return _AttentionFn.apply(q, k, v, causal, scale, grad_layout)
-    qf, kf, vf = (t.float().permute(0, 2, 1, 3) for t in (q, k, v))
-    s = (qf @ kf.transpose(-1, -2)) * scale
-    if causal:
-        S = q.shape[1]
-        s = s.masked_fill(torch.ones(S, S, dtype=torch.bool, device=q.device).triu(1), float('-inf'))
-    out = torch.softmax(s, dim=-1) @ vf
-    return out.permute(0, 2, 1, 3).to(q.dtype).contiguous()
+    return _attention_plain(q, k, v, causal, scale, None)
 
 
 # ---------------------------------------------------------------------------------------- cross entropy
