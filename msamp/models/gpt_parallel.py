@@ -108,6 +108,8 @@ class ParallelGPT(nn.Module):
         self.tp = mpu.get_tensor_model_parallel_world_size()
         self.tp_rank = mpu.get_tensor_model_parallel_rank()
         self.sequence_parallel = sequence_parallel and self.tp > 1
+        if cfg.kv_heads != cfg.n_head or cfg.rotary_dim or cfg.keep_fp8 or cfg.recompute == 'fp8':
+            raise ValueError('ParallelGPT has a key/value head per query head, learned positions and no activations in 8 bits')
         if cfg.vocab_size % self.tp:
             raise ValueError('vocab_size must be divisible by the tensor-parallel size')
         self.wte = nn.Embedding(cfg.vocab_size, cfg.hidden, device=device, dtype=act_dtype)

@@ -133,7 +133,7 @@ class _LnLinearFn(torch.autograd.Function):
 class _MlpSublayerFn(torch.autograd.Function):
     """``x + fc2(gelu(fc1(layer_norm(x))))`` (without the ``x +`` when ``add_residual`` is false)."""
     @staticmethod
-    def forward(ctx, x, ln_weight, ln_bias, b1, b2, eps, w1, m1, w2, m2, add_residual=True):
+    def forward(ctx, x, ln_weight, ln_bias, b1, b2, eps, w1, m1, w2, m2, add_residual=True, keep_fp8=False):
         model_state.check_metas_in_flat(m1)
         model_state.check_metas_in_flat(m2)
         x = x.contiguous()
@@ -154,7 +154,9 @@ class _MlpSublayerFn(torch.autograd.Function):
             g_sinv = g_meta.scale_inv.clone()
         out = _g.gemm_fp8(g8, E4M3, g_sinv, w2_8, E4M3, w2_sinv, dt, bias=b2, residual=x if add_residual else None)
         ctx.add_residual = add_residual
-        ctx.save_for_backward(x, ln_weight, mean, rstd, y8, y_sinv, h, g8, g_sinv, w1_8, w1_sinv, w2_8, w2_sinv)
+        # the widest activation: the GeLU input, two bytes an element, or 1.03 as e4m3 blocks
+        kept = _k.cast_blocks_to_fp8(h) if keep_fp8 else (h, None)
+        ctx.save_for_backward(x, ln_weight, mean, rstd, y8, y_sinv, *kept, g8, g_sinv, w1_8, w1_sinv, w2_8, w2_sinv)
         ctx.w1, ctx.m1, ctx.w2, ctx.m2 = w1, m1, w2, m2
         ctx.has_ln_bias = ln_bias is not None
         ctx.b1_dtype = b1.dtype if b1 is not None else None
@@ -163,9 +165,11 @@ class _MlpSublayerFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        x, ln_weight, mean, rstd, y8, y_sinv, h, g8, g_sinv, w1_8, w1_sinv, w2_8, w2_sinv = ctx.saved_tensors
+        x, ln_weight, mean, rstd, y8, y_sinv, h, h_exp, g8, g_sinv, w1_8, w1_sinv, w2_8, w2_sinv = ctx.saved_tensors
         m1, m2 = ctx.m1, ctx.m2
         dt = x.dtype
+        if h_exp is not None:
+            h = _k.cast_blocks_from_fp8(h, h_exp, dt)
         g = g.contiguous()
         # fc2
         dy8, dy_sinv, db2 = _quantize_ograd(g, m2['ograd'], ctx.b2_dtype is not None, ctx.b2_dtype)
@@ -193,13 +197,24 @@ class _MlpSublayerFn(torch.autograd.Function):
         _deliver_wgrad(ctx.w1, m1, dh8, dh_sinv, y8, y_sinv, dt)
         dln = gemm_dgrad(dh8, dh_sinv, w1_8, w1_sinv, dt)
         dx, dgamma, dbeta = _ln_backward(dln, x, ln_weight, mean, rstd, ctx.has_ln_bias, g if ctx.add_residual else None)
-        return dx, dgamma, dbeta, db1, db2, None, None, None, None, None, None
+        return dx, dgamma, dbeta, db1, db2, None, None, None, None, None, None, None
+
+
+def _heads(qkv, batch, seq, n_head, n_kv):
+    """Views of a packed projection ``[tokens, (n_head + 2 n_kv) * d]``: query, key, value heads, and the first two together."""
+    x = qkv.view(batch, seq, n_head + 2 * n_kv, -1)
+    return x[:, :, :n_head], x[:, :, n_head:n_head + n_kv], x[:, :, n_head + n_kv:], x[:, :, :n_head + n_kv]
 
 
 class _AttnSublayerFn(torch.autograd.Function):
-    """``x + proj(attention(qkv(layer_norm(x))))`` with causal softmax attention on the packed QKV projection."""
+    """``x + proj(attention(qkv(layer_norm(x))))`` with softmax attention on the packed QKV projection.
+
+    ``rope`` (frequencies, positions, interleaved) turns the query and key heads where the projection left them, and their gradient
+    where the attention's backward pass left it.
+    """
     @staticmethod
-    def forward(ctx, x, ln_weight, ln_bias, b_qkv, b_proj, eps, w_qkv, m_qkv, w_proj, m_proj, batch, seq, n_head, causal):
+    def forward(ctx, x, ln_weight, ln_bias, b_qkv, b_proj, eps, w_qkv, m_qkv, w_proj, m_proj, batch, seq, n_head, causal, n_kv=None, rope=None,
+                lengths=None):
         model_state.check_metas_in_flat(m_qkv)
         model_state.check_metas_in_flat(m_proj)
         x = x.contiguous()
@@ -208,13 +223,20 @@ class _AttnSublayerFn(torch.autograd.Function):
         wq8, wq_sinv = weight_fp8(w_qkv)
         wp8, wp_sinv = weight_fp8(w_proj)
         qkv = _g.gemm_fp8(y8, E4M3, y_sinv, wq8, E4M3, wq_sinv, dt, bias=b_qkv)
-        head_dim = qkv.shape[1] // (3 * n_head)
-        qkv5 = qkv.view(batch, seq, 3, n_head, head_dim)
-        o, lse = _nn.attention_qkv_fwd_raw(qkv5, causal)
+        n_kv = n_head if n_kv is None else n_kv
+        head_dim = qkv.shape[1] // (n_head + 2 * n_kv)
+        q, k, v, turned = _heads(qkv, batch, seq, n_head, n_kv)
+        if rope is not None:
+            _nn.rotary_raw([turned], [turned], *rope, False)
+        if n_kv == n_head and lengths is None:
+            o, lse = _nn.attention_qkv_fwd_raw(qkv.view(batch, seq, 3, n_head, head_dim), causal)
+        else:
+            o, lse = _nn.attention_shared_fwd_raw(q, k, v, causal, lengths=lengths)
         o2 = o.view(batch * seq, n_head * head_dim)
         o8, o_sinv = _quantize(o2, m_proj['input'], E4M3)
         out = _g.gemm_fp8(o8, E4M3, o_sinv, wp8, E4M3, wp_sinv, dt, bias=b_proj, residual=x)
-        ctx.save_for_backward(x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv)
+        ctx.save_for_backward(x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths)
+        ctx.n_kv, ctx.rope = n_kv, rope
         ctx.w_qkv, ctx.m_qkv, ctx.w_proj, ctx.m_proj = w_qkv, m_qkv, w_proj, m_proj
         ctx.shape = (batch, seq, n_head, head_dim)
         ctx.causal = causal
@@ -225,9 +247,10 @@ class _AttnSublayerFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv = ctx.saved_tensors
+        x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths = ctx.saved_tensors
         m_qkv, m_proj = ctx.m_qkv, ctx.m_proj
         batch, seq, n_head, head_dim = ctx.shape
+        n_kv, rope = ctx.n_kv, ctx.rope
         dt = x.dtype
         g = g.contiguous()
         # proj
@@ -235,16 +258,25 @@ class _AttnSublayerFn(torch.autograd.Function):
         _deliver_wgrad(ctx.w_proj, m_proj, dy8, dy_sinv, o8, o_sinv, dt)
         d_o = gemm_dgrad(dy8, dy_sinv, wp8, wp_sinv, dt)
         # attention
-        dqkv = _nn.attention_qkv_bwd_raw(qkv.view(batch, seq, 3, n_head, head_dim), o, lse, d_o.view(batch, seq, n_head, head_dim), ctx.causal)
+        d_o = d_o.view(batch, seq, n_head, head_dim)
+        if n_kv == n_head and lengths is None:
+            dqkv = _nn.attention_qkv_bwd_raw(qkv.view(batch, seq, 3, n_head, head_dim), o, lse, d_o, ctx.causal)
+        else:
+            dqkv = torch.empty_like(qkv)
+            _nn.attention_shared_bwd_raw(*_heads(qkv, batch, seq, n_head, n_kv)[:3], o, lse, d_o, *_heads(dqkv, batch, seq, n_head, n_kv)[:3],
+                                         ctx.causal, lengths=lengths)
         del d_o
-        dqkv2 = dqkv.view(batch * seq, 3 * n_head * head_dim)
+        dqkv2 = dqkv.view(batch * seq, (n_head + 2 * n_kv) * head_dim)
+        if rope is not None:
+            turned = _heads(dqkv2, batch, seq, n_head, n_kv)[3]
+            _nn.rotary_raw([turned], [turned], *rope, True)
         # qkv
         dq8, dq_sinv, dbq = _quantize_ograd(dqkv2, m_qkv['ograd'], ctx.bq_dtype is not None, ctx.bq_dtype)
         del dqkv, dqkv2
         _deliver_wgrad(ctx.w_qkv, m_qkv, dq8, dq_sinv, y8, y_sinv, dt)
         dln = gemm_dgrad(dq8, dq_sinv, wq8, wq_sinv, dt)
         dx, dgamma, dbeta = _ln_backward(dln, x, ln_weight, mean, rstd, ctx.has_ln_bias, g)
-        return dx, dgamma, dbeta, dbq, dbp, None, None, None, None, None, None, None, None, None
+        return (dx, dgamma, dbeta, dbq, dbp) + (None, ) * 12
 
 
 def ln_linear(x, ln, linear):
@@ -253,11 +285,14 @@ def ln_linear(x, ln, linear):
     return _LnLinearFn.apply(x, ln.weight, ln.bias, linear.bias, ln.eps, linear.weight, linear.scaling_metas)
 
 
-def mlp_sublayer(x, ln, fc1, fc2, residual=True):
-    """``x + fc2(gelu(fc1(ln(x))))`` for FP8Linear ``fc1`` / ``fc2``, 2-D ``x``; ``residual=False`` drops the ``x +``."""
+def mlp_sublayer(x, ln, fc1, fc2, residual=True, keep_fp8=False):
+    """``x + fc2(gelu(fc1(ln(x))))`` for FP8Linear ``fc1`` / ``fc2``, 2-D ``x``; ``residual=False`` drops the ``x +``.
+
+    ``keep_fp8`` keeps the GeLU input for the backward pass as e4m3 with a power-of-two scale per 32 elements instead of 16 bits.
+    """
     model_state.ready_to_scale_tensor = True
     return _MlpSublayerFn.apply(x, ln.weight, ln.bias, fc1.bias, fc2.bias, ln.eps, fc1.weight, fc1.scaling_metas, fc2.weight,
-                                fc2.scaling_metas, bool(residual))
+                                fc2.scaling_metas, bool(residual), bool(keep_fp8))
 
 
 class ModuleView:
@@ -267,8 +302,12 @@ class ModuleView:
         self.weight, self.bias, self.eps, self.scaling_metas = weight, bias, eps, scaling_metas
 
 
-def attention_sublayer(x, ln, qkv, proj, batch, seq, n_head, causal=True):
-    """``x + proj(attention(qkv(ln(x))))`` for FP8Linear ``qkv`` (packed ``[3 * hidden, hidden]``) and ``proj``, 2-D ``x``."""
+def attention_sublayer(x, ln, qkv, proj, batch, seq, n_head, causal=True, n_kv_head=None, rope=None, lengths=None):
+    """``x + proj(attention(qkv(ln(x))))`` for FP8Linear ``qkv`` (packed ``[3 * hidden, hidden]``) and ``proj``, 2-D ``x``.
+
+    With ``n_kv_head`` key/value heads the projection is ``[(n_head + 2 * n_kv_head) * head_dim, hidden]``: query, key, value heads.
+    ``rope``: ``(freqs, positions or None, interleaved)`` of :func:`msamp.ops.nn.rotary`.  ``lengths``: see :func:`msamp.ops.nn.attention`.
+    """
     model_state.ready_to_scale_tensor = True
     return _AttnSublayerFn.apply(x, ln.weight, ln.bias, qkv.bias, proj.bias, ln.eps, qkv.weight, qkv.scaling_metas, proj.weight,
-                                 proj.scaling_metas, batch, seq, n_head, causal)
+                                 proj.scaling_metas, batch, seq, n_head, causal, n_kv_head, rope, lengths)

@@ -1,0 +1,225 @@
+"""Rotary positions, shared key/value heads, padded rows and activations in 8 bits together, as a GPT block uses them."""
+import math
+
+import pytest
+import torch
+
+import msamp
+from msamp.models import GPT, gpt_config
+from msamp.nn import LinearReplacer
+from msamp.nn import fused_layers as FL
+from msamp.ops import cast, native
+from msamp.ops import nn as K
+
+CPU_GPU = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+
+
+def _config(**kw):
+    return gpt_config('gpt-tiny', **{**dict(n_layer=2, n_head=4, hidden=256, ffn_hidden=512, vocab_size=512, max_seq=64), **kw})
+
+
+def _batch(device, batch=3, seq=24):
+    gen = torch.Generator().manual_seed(1)
+    tokens = torch.randint(0, 512, (batch, seq), generator=gen)
+    lengths = torch.tensor([seq, 7, 1][:batch])
+    labels = torch.where(torch.arange(seq) < lengths[:, None], tokens.roll(-1, 1), torch.tensor(-100))
+    return tokens.to(device), labels.to(device), lengths.to(device)
+
+
+def _model(device, **kw):
+    torch.manual_seed(0)
+    return GPT(_config(**kw), device=device, act_dtype=torch.bfloat16 if device == 'cuda' else torch.float32)
+
+
+LONG = dict(n_kv_head=2, rotary_dim=32, keep_fp8=True)
+
+
+def _plain_block(blk, x, batch, seq, freqs, valid):
+    """A block in torch operations: what the framework's form has to compute."""
+    h, d, n, m = x.shape[1], blk.head_dim, blk.n_head, blk.n_kv
+
+    def norm(ln, t):
+        return torch.nn.functional.layer_norm(t, (h, ), ln.weight, ln.bias, ln.eps)
+
+    qkv = torch.nn.functional.linear(norm(blk.ln1, x), blk.qkv.weight, blk.qkv.bias).view(batch, seq, n + 2 * m, d)
+    q, k, v = qkv.split([n, m, m], 2)
+    angle = torch.arange(seq, dtype=torch.float64)[:, None] * freqs
+    cos, sin = angle.cos().float()[:, None], angle.sin().float()[:, None]
+
+    def turn(t):
+        r = freqs.numel()
+        a, b = t[..., :r], t[..., r:2 * r]
+        return torch.cat([a * cos - b * sin, b * cos + a * sin, t[..., 2 * r:]], -1)
+
+    q, k = turn(q), turn(k).repeat_interleave(n // m, 2)
+    v = v.repeat_interleave(n // m, 2)
+    s = torch.einsum('bihd,bjhd->bhij', q, k) / d**0.5
+    see = valid[:, None, None, :] & torch.ones(seq, seq, dtype=torch.bool).tril()
+    p = torch.softmax(torch.where(see, s, torch.tensor(-1e30)), -1) * valid[:, None, :, None]
+    o = torch.einsum('bhij,bjhd->bihd', p, v).reshape(batch * seq, -1)
+    x = x + torch.nn.functional.linear(o, blk.proj.weight, blk.proj.bias)
+    f = torch.nn.functional.linear(norm(blk.ln2, x), blk.fc1.weight, blk.fc1.bias)
+    return x + torch.nn.functional.linear(torch.nn.functional.gelu(f, approximate='tanh'), blk.fc2.weight, blk.fc2.bias)
+
+
+def test_model_computes_the_plain_block():
+    """fp32 on the CPU: loss and gradients equal the plain form's up to 32-bit rounding (same matrices, other order of sums)."""
+    model = _model('cpu', n_kv_head=2, rotary_dim=32)
+    tokens, labels, lengths = _batch('cpu')
+    loss = model(tokens, labels, lengths=lengths)
+    loss.backward()
+    mine = {n: p.grad.clone() for n, p in model.named_parameters()}
+    model.zero_grad()
+    b, s = tokens.shape
+    valid = torch.arange(s) < lengths[:, None]
+    x = model.wte(tokens).view(b * s, -1)
+    for blk in model.blocks:
+        x = _plain_block(blk, x, b, s, model._freqs, valid)
+    ln = model.ln_f
+    logits = torch.nn.functional.layer_norm(x, (x.shape[1], ), ln.weight, ln.bias, ln.eps) @ model.lm_head.weight.t()
+    want = torch.nn.functional.cross_entropy(logits, labels.reshape(-1), ignore_index=-100)
+    want.backward()
+    assert abs(loss.item() - want.item()) <= 1e-5
+    for n, p in model.named_parameters():
+        assert (mine[n] - p.grad).norm() <= 1e-4 * p.grad.norm() + 1e-7, n
+
+
+def test_padding_does_not_change_a_row():
+    model = _model('cpu', **LONG)
+    tokens, _, lengths = _batch('cpu')
+    out = model(tokens, lengths=lengths)
+    other = tokens.clone()
+    other[torch.arange(tokens.shape[1]) >= lengths[:, None]] = 5
+    again = model(other, lengths=lengths)
+    short = model(tokens[1:2, :7])
+    assert torch.equal(out[1, :7], again[1, :7]) and torch.allclose(out[1, :7], short[0], rtol=1e-5, atol=1e-5)
+
+
+def test_positions_are_relative():
+    """Rotary scores depend on differences of positions only: a shifted context gives the same logits up to 32-bit rounding."""
+    model = _model('cpu', n_kv_head=1, rotary_dim=64, rotary_interleaved=True)
+    tokens, _, _ = _batch('cpu')
+    at = torch.arange(tokens.shape[1])
+    a, b, c = model(tokens), model(tokens, positions=at + 123456), model(tokens, positions=at * 2)
+    assert torch.allclose(a, b, rtol=1e-4, atol=1e-4) and not torch.allclose(a, c, rtol=1e-2, atol=1e-2)
+
+
+def _train_grads(device, opt, recompute=False, steps=1, **kw):
+    model = _model(device, recompute=recompute, **kw)
+    optimizer = torch.optim.AdamW(model.parameters(), lr=1e-3)
+    if opt:
+        model, optimizer = msamp.initialize(model, optimizer, opt)
+    tokens, labels, lengths = _batch(device)
+    for _ in range(steps):
+        optimizer.zero_grad()
+        loss = model(tokens, labels, lengths=lengths)
+        loss.backward()
+        grads = {n: (p.grad.float() if p.grad is not None else None) for n, p in model.named_parameters()}
+        optimizer.step()
+    return loss.item(), grads
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('opt', [None, 'O1', 'O2'])
+@pytest.mark.parametrize('recompute', [False, True, 'fp8'])
+def test_trains_with_every_option(device, opt, recompute):
+    if device == 'cuda' and opt is None:
+        pytest.skip('bf16 activations against fp32 linears: the model runs on CUDA after msamp.initialize')
+    loss, grads = _train_grads(device, opt, recompute, steps=3, rotary_scaling='parts', rotary_factor=2.0, rotary_trained=64, **LONG)
+    assert math.isfinite(loss)
+    for n, g in grads.items():
+        assert g is not None and torch.isfinite(g).all() and g.abs().sum() > 0, n
+    if device == 'cuda':
+        torch.cuda.synchronize()
+        assert native.device_status() == 0
+
+
+def test_fused_sublayers_compute_what_the_separate_calls_compute():
+    """FP8 on the CPU emulation: the attention sublayer with rope, shared heads and lengths against LayerNorm, FP8 linear, rotary, attention,
+    FP8 linear one by one; the same quantisation points, so the same values."""
+    torch.manual_seed(0)
+    h, n, m, d, b, s = 256, 4, 2, 64, 2, 12
+
+    class Parts(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            from msamp.models.gpt import LayerNorm
+            self.ln, self.qkv, self.proj = LayerNorm(h), torch.nn.Linear(h, (n + 2 * m) * d), torch.nn.Linear(h, h)
+
+    parts = LinearReplacer.replace(Parts())
+    x = torch.randn(b * s, h)
+    freqs, lengths = K.rotary_frequencies(d), torch.tensor([12, 5])
+    results = []
+    for fused in (True, False):
+        torch.manual_seed(1)
+        for meta in (parts.qkv, parts.proj):
+            for v in meta.scaling_metas.values():
+                v.amax.zero_()
+                v.scale.fill_(1.0)
+            meta.weight.grad = None
+        leaf = x.clone().requires_grad_(True)
+        if fused:
+            y = FL.attention_sublayer(leaf, parts.ln, parts.qkv, parts.proj, b, s, n, n_kv_head=m, rope=(freqs, None, False), lengths=lengths)
+        else:
+            q, k, v = parts.qkv(parts.ln(leaf)).view(b, s, -1, d).split([n, m, m], 2)
+            q, k = K.rotary(q, k, freqs)
+            y = leaf + parts.proj(K.attention(q, k, v, lengths=lengths).view(b * s, -1))
+        y.backward(torch.randn(b * s, h))
+        results.append((y.detach(), leaf.grad, parts.ln.weight.grad.clone(), parts.qkv.bias.grad.clone(), parts.proj.weight.grad.float()))
+        parts.zero_grad()
+    for a, c in zip(*results):
+        # a 32-bit sum in another order can move a value across a rounding border of e4m3 / e5m2 (a step of 2^-3 of it): rare, so small in norm
+        assert (a - c).norm() <= 1e-2 * c.norm()
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+def test_mlp_sublayer_keeps_the_gelu_input_in_8_bits(device):
+    torch.manual_seed(0)
+    dt = torch.bfloat16 if device == 'cuda' else torch.float32
+
+    class Parts(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            from msamp.models.gpt import LayerNorm
+            self.ln, self.fc1, self.fc2 = LayerNorm(128), torch.nn.Linear(128, 512), torch.nn.Linear(512, 128)
+
+    parts = LinearReplacer.replace(Parts().to(device))
+    x, dy = torch.randn(40, 128, device=device).to(dt), torch.randn(40, 128, device=device).to(dt)
+    seen, out = {}, {}
+    for keep in (False, True):
+        leaf, kept = x.clone().requires_grad_(True), []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+            y = FL.mlp_sublayer(leaf, parts.ln, parts.fc1, parts.fc2, keep_fp8=keep)
+        y.backward(dy)
+        seen[keep], out[keep] = sum(t.numel() * t.element_size() for t in kept), (y.detach(), leaf.grad)
+    assert torch.equal(out[False][0], out[True][0])
+    n = 40 * 512
+    assert seen[False] - seen[True] == n * dt.itemsize - n - n // 32
+    # the slope of GeLU moves by at most its second derivative (0.8) times 2^-4 of an input of order one, e = 0.05; a gradient moved by e
+    # crosses a border of e5m2 (steps of up to 1/4) with probability 4 e and then moves by a step: sqrt(e / 4) + e of the norm at most
+    a, c = out[False][1].float(), out[True][1].float()
+    assert 0 < (a - c).norm() <= 0.16 * a.norm()
+
+
+def test_options_refused():
+    with pytest.raises(ValueError):
+        GPT(_config(n_kv_head=3))
+    with pytest.raises(ValueError):
+        GPT(_config(recompute='fp4'))
+    with pytest.raises(ValueError):
+        GPT(_config(rotary_dim=33))
+    with pytest.raises(ValueError):
+        _model('cpu')(torch.zeros(1, 4, dtype=torch.int64), positions=torch.arange(4))
+
+
+def test_parameters_and_defaults():
+    for kw in ({}, LONG, dict(n_kv_head=1), dict(rotary_dim=64)):
+        model = GPT(_config(**kw))
+        assert sum(p.numel() for p in model.parameters()) == model.cfg.num_params()
+    plain = GPT(_config())
+    assert 'wpe.weight' in plain.state_dict() and plain.cfg.kv_heads == 4 and not any('freq' in n for n in plain.state_dict())
+    assert GPT(_config(rotary_dim=32)).bfloat16()._freqs.dtype == torch.float64
+
+
+def test_block_casts_are_in_the_public_module():
+    assert cast.cast_blocks_to_fp8(torch.zeros(3))[1].tolist() == [127]
