@@ -230,12 +230,13 @@ class _AttnSublayerFn(torch.autograd.Function):
             _nn.rotary_raw([turned], [turned], *rope, False)
         if n_kv == n_head and lengths is None:
             o, lse = _nn.attention_qkv_fwd_raw(qkv.view(batch, seq, 3, n_head, head_dim), causal)
+            plan = None
         else:
-            o, lse = _nn.attention_shared_fwd_raw(q, k, v, causal, lengths=lengths)
+            o, lse, plan = _nn.attention_shared_fwd_raw(q, k, v, causal, lengths=lengths)
         o2 = o.view(batch * seq, n_head * head_dim)
         o8, o_sinv = _quantize(o2, m_proj['input'], E4M3)
         out = _g.gemm_fp8(o8, E4M3, o_sinv, wp8, E4M3, wp_sinv, dt, bias=b_proj, residual=x)
-        ctx.save_for_backward(x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths)
+        ctx.save_for_backward(x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths, plan)
         ctx.n_kv, ctx.rope = n_kv, rope
         ctx.w_qkv, ctx.m_qkv, ctx.w_proj, ctx.m_proj = w_qkv, m_qkv, w_proj, m_proj
         ctx.shape = (batch, seq, n_head, head_dim)
@@ -247,7 +248,7 @@ class _AttnSublayerFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths = ctx.saved_tensors
+        x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths, plan = ctx.saved_tensors
         m_qkv, m_proj = ctx.m_qkv, ctx.m_proj
         batch, seq, n_head, head_dim = ctx.shape
         n_kv, rope = ctx.n_kv, ctx.rope
@@ -263,7 +264,7 @@ class _AttnSublayerFn(torch.autograd.Function):
             dqkv = _nn.attention_qkv_bwd_raw(qkv.view(batch, seq, 3, n_head, head_dim), o, lse, d_o, ctx.causal)
         else:
             dqkv = torch.empty_like(qkv)
-            _nn.attention_shared_bwd_raw(*_heads(qkv, batch, seq, n_head, n_kv)[:3], o, lse, d_o, *_heads(dqkv, batch, seq, n_head, n_kv)[:3],
+            _nn.attention_shared_bwd_raw(*_heads(qkv, batch, seq, n_head, n_kv)[:3], o, lse, plan, d_o, *_heads(dqkv, batch, seq, n_head, n_kv)[:3],
                                          ctx.causal, lengths=lengths)
         del d_o
         dqkv2 = dqkv.view(batch * seq, (n_head + 2 * n_kv) * head_dim)

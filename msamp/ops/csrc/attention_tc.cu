@@ -50,12 +50,20 @@ struct TcParams {
   unsigned int* status;
   // kernels with X only
   int kv_heads, rep;       // key / value heads; query heads of each
-  const int* lengths;      // [batch] positions of a row that are not padding, or null: all
+  const int* lengths;      // X == 2: [batch] positions of a row that are not padding
+  const int* plan;         // X == 2: the number of tiles that are not padding alone, then those tiles (see attn_plan_kernel)
   int parts;               // dK / dV: work items that share the query heads of a key / value head
   float* partial;          // [parts][dK, dV][batch, kv_heads, seqlen, head_dim] when there are several
 };
 
-__device__ __forceinline__ int row_length(const TcParams& p, int b) { return p.lengths ? min(max(__ldg(p.lengths + b), 0), p.seqlen) : p.seqlen; }
+__device__ __forceinline__ int row_length(const int* lengths, int b, int seqlen) { return min(max(__ldg(lengths + b), 0), seqlen); }
+__device__ __forceinline__ int row_length(const TcParams& p, int b) { return row_length(p.lengths, b, p.seqlen); }
+// The n-th tile of the plan: its batch and its number in the sequence
+__device__ __forceinline__ void planned_tile(const TcParams& p, int n, int n_tiles, int& b, int& i) {
+  const int code = __ldg(p.plan + 1 + n);
+  b = code / n_tiles;
+  i = code - b * n_tiles;
+}
 // The 128-row tile t of a sequence holds rows behind its end that are there in memory (rows behind seqlen are filled with zeros by TMA).
 __device__ __forceinline__ bool ends_inside(int t, int len, int seqlen) { return len < seqlen && (t + 1) * 128 > len; }
 
@@ -1092,10 +1100,10 @@ struct FwdItem {
   int qt, bh;
   int first, step, n_t;    // key tiles first, first + step, ... < n_t; n_t == 0: no item
   bool shared;
-  int len;                 // X: length of the row
+  int len;                 // X == 2: length of the row
 };
-// X: a row ends at its length, and a query tile behind it still takes one tile, all of it masked, which leaves zeros.
-template <bool X>
+// X == 2: the query tiles of the plan, longest first, each for all heads; a row ends at its length.
+template <int X>
 struct FwdItems {
   int n_qt, n_items, bh_total, G, n_ctas, causal;
   const TcParams* p;
@@ -1122,16 +1130,21 @@ struct FwdItems {
     // that the CTAs of a few consecutive waves work on the same heads: a head's K and V are read from HBM by its longest
     // rows and found in L2 by the others (with all heads of one query-tile level in a wave the kernel read K / V 3.9 times).
     const int item = w * 2 * n_ctas + j;
+    if (X == 2) {
+      const int n = item / p->heads;
+      int b;
+      planned_tile(*p, n, n_qt, b, x.qt);
+      x.bh = b * p->heads + item - n * p->heads;
+      x.len = row_length(*p, b);
+      x.n_t = causal ? x.qt + 1 : (x.len + 127) / 128;
+      return x;
+    }
     const int grp = item / (G * n_qt);
     const int hg = min(G, bh_total - grp * G);
     const int k = item - grp * G * n_qt;
     x.qt = n_qt - 1 - k / hg;
     x.bh = grp * G + k % hg;
     x.n_t = causal ? x.qt + 1 : n_qt;
-    if (X) {
-      x.len = row_length(*p, x.bh / p->heads);
-      x.n_t = x.qt * 128 >= x.len ? 1 : min(x.n_t, (x.len + 127) / 128);
-    }
     return x;
   }
 };
@@ -1142,7 +1155,7 @@ struct FwdStream {
   int g, w, t;           // stream, next wave, tile of the current item
   FwdItem item;          // n_t == 0: list exhausted
   uint32_t started;      // items so far (an item that is one shared tile leaves the second stream without any)
-  template <bool X>
+  template <int X>
   __device__ __forceinline__ void open(const FwdItems<X>& items) {
     item = items.at(w++, g);
     t = item.first;
@@ -1154,16 +1167,16 @@ struct FwdStream {
 };
 struct FwdSeq {
   FwdStream cur, other;
-  template <bool X>
+  template <int X>
   __device__ __forceinline__ FwdSeq(const FwdItems<X>& items) {
     cur.g = cur.w = other.w = 0;
     other.g = 1;
     cur.started = other.started = 0u;
-    cur.open(items);    // stream 0 has an item in every CTA
+    cur.open(items);    // where stream 0 has no item, stream 1 has none
     other.open(items);
   }
   __device__ __forceinline__ bool more() const { return cur.item.n_t > 0; }
-  template <bool X>
+  template <int X>
   __device__ __forceinline__ void advance(const FwdItems<X>& items) {
     cur.t += cur.item.step;
     if (cur.t >= cur.item.n_t) cur.open(items);
@@ -1201,10 +1214,10 @@ struct FwdSeq {
 // Reuse: Q_g after the last score product of its item (B_QE); the score slot after B_SE (tiles in sequence order); P_g and
 // the accumulator after P V of the group's previous tile (B_OF); the accumulator of a finished item is read before the group
 // hands over its next P (B_PF), so the next item's first product cannot overtake it.
-// X: query heads share key / value heads (only the coordinates of the K and V tiles know) and rows have lengths.  Scores of padded keys
-// and of padded queries are masked like those of later keys.  A V tile with rows behind the end of its sequence lands on a barrier of its
+// X >= 1: query heads share key / value heads; only the coordinates of the K and V tiles know.  X == 2: rows have lengths.  The work items
+// are those of the plan, scores of padded keys are masked like those of later keys, padded queries are not stored.  A V tile with rows behind the end of its sequence lands on a barrier of its
 // own (B_VL, one per slot, so that neither side can be a phase ahead); warp 3 clears those rows and then arrives on B_VF for it.
-template <int D, bool X>
+template <int D, int X>
 __global__ void __launch_bounds__(kPsThreads, 1)
 attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const TcParams p, int n_qt, int n_items) {
@@ -1224,7 +1237,7 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
   auto wait_warp = [&](uint32_t br, uint32_t ph) { return __all_sync(0xffffffffu, wait(br, ph)) != 0; };
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const FwdItems<X> items{n_qt, n_items, p.batch * p.heads, p.group, (int)gridDim.x, p.causal, &p};
+  const FwdItems<X> items{n_qt, X == 2 ? __ldg(p.plan) * p.heads : n_items, p.batch * p.heads, p.group, (int)gridDim.x, p.causal, &p};
 
   if (threadIdx.x == 0) {
     for (int g = 0; g < 2; ++g) {
@@ -1243,7 +1256,7 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     for (int s = 0; s < NV; ++s) {
       tc5::mbar_init(bar(C::B_VF + s), 1);
       tc5::mbar_init(bar(C::B_VE + s), 1);
-      if (X) tc5::mbar_init(bar(C::B_VL + s), 1);
+      if (X == 2) tc5::mbar_init(bar(C::B_VL + s), 1);
     }
     *abort_flag = 0;
     tc5::mbar_fence_init();
@@ -1291,7 +1304,7 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (waiting == 2 || !more) {
           const int b = vbh0 / p.heads, h = vbh0 - b * p.heads;
           if (!wait(bar(C::B_VE + vr.slot), vr.phase ^ 1u)) break;
-          const int landed = X && ends_inside(vt0, row_length(p, b), p.seqlen) ? C::B_VL + vr.slot : C::B_VF + vr.slot;
+          const int landed = X == 2 && ends_inside(vt0, row_length(p, b), p.seqlen) ? C::B_VL + vr.slot : C::B_VF + vr.slot;
           tc5::mbar_arrive_expect_tx(bar(landed), TILE);
 #pragma unroll
           for (int pp = 0; pp < HP; ++pp)
@@ -1359,7 +1372,7 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         vr.next();
         v_ready = tc5::mbar_test(bar(C::B_VF + vr.slot), vr.phase);
       }
-    } else if (X && warp == 3 && p.lengths) {
+    } else if (X == 2 && warp == 3) {
       // ---------------------------------------------------------------- V rows behind the end of their sequence
       Ring<NV> vr;
       uint32_t landed = 0u;    // bit s: parity of the next such tile in slot s
@@ -1392,11 +1405,9 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       const int b = bh / p.heads, h = bh - b * p.heads;
       const int q0 = qt * 128;
       const int grow = q0 + row;
-      const int len = X ? item.len : p.seqlen;
-      int lim = p.causal ? min(grow, len - 1) : len - 1;    // last visible column
-      int wlim = p.causal ? min(q0 + qd * 32 + 31, len - 1) : len - 1;    // the same for the warp's last row
-      if (X && grow >= len) lim = -1;    // padding sees nothing
-      if (X && q0 + qd * 32 >= len) wlim = -1;
+      const int len = X == 2 ? item.len : p.seqlen;
+      const int lim = p.causal ? min(grow, len - 1) : len - 1;    // last visible column
+      const int wlim = p.causal ? min(q0 + qd * 32 + 31, len - 1) : len - 1;    // the same for the warp's last row
       float m[NA], l[NA];    // running maximum (log2 units) and row sum
 #pragma unroll
       for (int a = 0; a < NA; ++a) {
@@ -1414,7 +1425,7 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         __syncwarp();
         if (lane == 0) tc5::mbar_arrive(bar(C::B_SE));    // the score slot may take the next tile
         const int col0 = t * 128;
-        const bool need_mask = (p.causal && col0 + 127 > q0) || (col0 + 128 > len) || (X && q0 + 128 > len);
+        const bool need_mask = (p.causal && col0 + 127 > q0) || (col0 + 128 > len);
         // 32-column chunks in which any row of this warp sees a key
         const int nch = need_mask ? min(4, (wlim - col0) / 32 + 1) : 4;
         const int rel = lim - col0;    // last visible column of this row
@@ -1529,7 +1540,7 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
       tc5::fence_after_sync();
       const int64_t lse_row = (int64_t)bh * p.seqlen + grow;
       __nv_bfloat16* dst = p.o + (int64_t)b * p.o_sb + (int64_t)(q0 + qd * 32) * p.o_ss + (int64_t)h * p.o_sh;    // the warp's first row
-      const int rows = p.seqlen - q0 - qd * 32;    // of which exist
+      const int rows = len - q0 - qd * 32;    // of which exist
       // the row's maximum and sum over its accumulators, and the factor of each
       float mr = m[0], lr = l[0], f[NA];
       f[0] = 1.0f;
@@ -1554,14 +1565,10 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
 #pragma unroll
             for (int i = 0; i < 64; ++i) v[i] = a ? fmaf(__uint_as_float(x[i >> 5][i & 31]), fa, v[i]) : __uint_as_float(x[i >> 5][i & 31]) * fa;
           }
-          if (X && lim < 0) {    // a row that sees nothing is zero, whatever the values hold
-#pragma unroll
-            for (int i = 0; i < 64; ++i) v[i] = 0.0f;
-          }
           st_rows64(dst + c, p.o_ss, rows, v);
         }
         tc5::fence_before_sync();    // the next item's first P is handed over after these reads
-        if (grow < p.seqlen) p.lse[lse_row] = lr > 0.0f ? mr * kLn2 + logf(lr) : -INFINITY;
+        if (grow < len) p.lse[lse_row] = lr > 0.0f ? mr * kLn2 + logf(lr) : -INFINITY;
       } else {
         // the last item of the CTA: maxima, sums and factors change hands through the P columns, which nothing uses any more
         uint32_t x[16] = {__float_as_uint(mr), __float_as_uint(lr), __float_as_uint(f[0]), __float_as_uint(f[NA - 1])}, y[16];
@@ -1600,13 +1607,9 @@ attn_fwd_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
               v[i] = fmaf(n_t > 1 ? __uint_as_float(a1[i]) : 0.0f, g1, a ? v[i] + o0 : o0);
             }
           }
-          if (X && lim < 0) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-          }
-          if (row < p.seqlen - q0) st_row32(dst + (int64_t)lane * p.o_ss + col, v);
+          if (row < len - q0) st_row32(dst + (int64_t)lane * p.o_ss + col, v);
         }
-        if (wg == 0 && grow < p.seqlen) p.lse[lse_row] = lt > 0.0f ? mm * kLn2 + logf(lt) : -INFINITY;
+        if (wg == 0 && grow < len) p.lse[lse_row] = lt > 0.0f ? mm * kLn2 + logf(lt) : -INFINITY;
       }
     }
   }
@@ -1627,12 +1630,17 @@ struct DeltaParams {
   float* delta;
   int64_t o_sb, o_ss, o_sh, do_sb, do_ss, do_sh;
   int batch, heads, seqlen;
+  // LEN only: gradients of padding are cleared here, so that the other kernels store rows of a sequence alone
+  const int* lengths;
+  __nv_bfloat16 *dq, *dk, *dv;
+  int64_t dq_sb, dq_ss, dq_sh, dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
+  int kv_heads;
 };
 
 // Bound by memory: one pass over O and dO.  D / 8 lanes read one row with 16-byte loads and rows are taken in the order of
 // their addresses ([batch, seq, head]), two per lane group, so that a warp keeps 2 KB of loads in flight.  A warp per row
 // in [batch, head, seq] order, 8 bytes a lane, took 50 us for 4 x 2048 x 32 heads of 128 (134 MB); this takes 35 us.
-template <int D>
+template <int D, bool LEN>
 __global__ void __launch_bounds__(256) attn_delta_tc_kernel(const DeltaParams p) {
   constexpr int L = D / 8;             // lanes of a row
   constexpr int ROWS = 256 / L;        // rows of a CTA and step
@@ -1650,6 +1658,15 @@ __global__ void __launch_bounds__(256) attn_delta_tc_kernel(const DeltaParams p)
       const int h = (int)(r % p.heads);
       const int64_t bs = r / p.heads;
       const int s = (int)(bs % p.seqlen), b = (int)(bs / p.seqlen);
+      if (LEN && s >= __ldg(p.lengths + b)) {
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(p.dq + (int64_t)b * p.dq_sb + (int64_t)s * p.dq_ss + (int64_t)h * p.dq_sh + sub * 8) = zero;
+        if (h < p.kv_heads) {
+          *reinterpret_cast<uint4*>(p.dk + (int64_t)b * p.dk_sb + (int64_t)s * p.dk_ss + (int64_t)h * p.dk_sh + sub * 8) = zero;
+          *reinterpret_cast<uint4*>(p.dv + (int64_t)b * p.dv_sb + (int64_t)s * p.dv_ss + (int64_t)h * p.dv_sh + sub * 8) = zero;
+        }
+        continue;
+      }
       a[k] = *reinterpret_cast<const Bytes16*>(p.o + (int64_t)b * p.o_sb + (int64_t)s * p.o_ss + (int64_t)h * p.o_sh + sub * 8);
       g[k] = *reinterpret_cast<const Bytes16*>(p.d_o + (int64_t)b * p.do_sb + (int64_t)s * p.do_ss + (int64_t)h * p.do_sh + sub * 8);
       out[k] = ((int64_t)b * p.heads + h) * p.seqlen + s;
@@ -2690,12 +2707,12 @@ struct Cfg {
 // of an item are complete, Q and dO may be overwritten; B3_OE: the softmax warps have read dQ, the accumulator may be
 // overwritten by the first product of the next item.
 // X: shared key / value heads and row lengths as in the forward kernel; the K tiles with rows behind the end of their sequence land on
-// B3_KL and warp 3 clears those rows.  A query tile behind the end has no tiles: its rows are stored as zeros.
-template <int D, bool X>
+// B3_KL and warp 3 clears those rows.
+template <int D, int X>
 __global__ void __launch_bounds__(kPsThreads, 1)
 attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const TcParams p, int n_qt,
-                      int n_items) {
+                      int max_items) {
   using namespace dqk3;
   constexpr int HP = Cfg<D>::HP;
   constexpr uint32_t TILE = Cfg<D>::TILE, OFF_DO = Cfg<D>::OFF_DO, OFF_K = Cfg<D>::OFF_K, OFF_V = Cfg<D>::OFF_V, OFF_BAR = Cfg<D>::OFF_BAR;
@@ -2714,14 +2731,30 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   const int lane = threadIdx.x & 31;
   const int nk_all = (p.seqlen + 63) / 64;
   const ItemOrder order{n_qt, p.batch * p.heads, p.group};
+  const int n_items = X == 2 ? __ldg(p.plan) * p.heads : max_items;
+  // Work item -> query tile, batch, head and the length of the row
+  auto open_item = [&](int item, int& qt, int& b, int& h, int& len) {
+    if (X == 2) {
+      const int n = item / p.heads;
+      planned_tile(p, n, n_qt, b, qt);
+      h = item - n * p.heads;
+      len = row_length(p, b);
+    } else {
+      int level, bh;
+      order.decode(item, level, bh);
+      qt = n_qt - 1 - level;
+      b = bh / p.heads;
+      h = bh - b * p.heads;
+      len = p.seqlen;
+    }
+  };
   const int n_waves = (n_items + (int)gridDim.x - 1) / (int)gridDim.x;
   auto item_at = [&](int w) {
     const int c = (w & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x;
     return w * (int)gridDim.x + c;
   };
   auto tiles_of = [&](int qt, int len) {
-    if (X && qt * 128 >= len) return 0;
-    const int n_len = X ? (len + 63) / 64 : nk_all;
+    const int n_len = X == 2 ? (len + 63) / 64 : nk_all;
     const int n_kv = p.causal ? min(2 * qt + 2, n_len) : n_len;
     return (n_kv + 1) >> 1;
   };
@@ -2745,7 +2778,7 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     tc5::mbar_init(bar(B_ACC), 1);
     tc5::mbar_init(bar(B3_QE), 1);
     tc5::mbar_init(bar(B3_OE), 8);
-    if (X)
+    if (X == 2)
       for (int s = 0; s < NK; ++s) tc5::mbar_init(bar(B3_KL + s), 1);
     *abort_flag = 0;
     tc5::mbar_fence_init();
@@ -2771,13 +2804,9 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       for (int w = 0; w < n_waves && ok; ++w) {
         const int item = item_at(w);
         if (item >= n_items) continue;
-        int level, bh;
-        order.decode(item, level, bh);
-        const int qt = n_qt - 1 - level;
-        const int b = bh / p.heads, h = bh - b * p.heads;
-        const int len = X ? row_length(p, b) : 0;
+        int qt, b, h, len;
+        open_item(item, qt, b, h, len);
         const int n_t = tiles_of(qt, len);
-        if (X && n_t == 0) continue;
         if (it > 0 && !tc5::mbar_wait(bar(B3_QE), (uint32_t)(it - 1) & 1u, abort_flag, p.status, kStatusBit)) break;
         tc5::mbar_arrive_expect_tx(bar(B_Q), 2 * TILE);
 #pragma unroll
@@ -2788,7 +2817,7 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         for (int t = 0; t < n_t; ++t, ++gt) {
           const int ks = gt % NK, vs = gt % NV;
           if (!tc5::mbar_wait(bar(B_KE + ks), ((uint32_t)(gt / NK) & 1u) ^ 1u, abort_flag, p.status, kStatusBit)) { ok = false; break; }
-          const int landed = X && ends_inside(t, len, p.seqlen) ? B3_KL + ks : B_KF + ks;
+          const int landed = X == 2 && ends_inside(t, len, p.seqlen) ? B3_KL + ks : B_KF + ks;
           tc5::mbar_arrive_expect_tx(bar(landed), TILE);
 #pragma unroll
           for (int pp = 0; pp < HP; ++pp) tc5::tma_load_4d(base + OFF_K + ks * TILE + pp * PANEL, &map_k, pp * 64, X ? h / p.rep : h, t * 128, b, bar(landed));
@@ -2840,10 +2869,9 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       for (int w = 0; w < n_waves && ok; ++w) {
         const int item = item_at(w);
         if (item >= n_items) continue;
-        int level, bh;
-        order.decode(item, level, bh);
-        const int n_t = tiles_of(n_qt - 1 - level, X ? row_length(p, bh / p.heads) : 0);
-        if (X && n_t == 0) continue;
+        int qt, b, h, len;
+        open_item(item, qt, b, h, len);
+        const int n_t = tiles_of(qt, len);
         if (!tc5::mbar_wait(bar(B_Q), (uint32_t)it & 1u, abort_flag, p.status, kStatusBit)) { ok = false; break; }
         if (!issue_s(g0)) { ok = false; break; }
         if (n_t == 1) tc5::mma_commit(bar(B3_QE));
@@ -2871,7 +2899,7 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         g0 += n_t;
         ++it;
       }
-    } else if (X && warp == 3 && p.lengths) {
+    } else if (X == 2 && warp == 3) {
       // K rows behind the end of their sequence
       Ring<NK> kr;
       uint32_t landed = 0u;    // bit s: parity of the next such tile in slot s
@@ -2879,10 +2907,9 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       for (int w = 0; w < n_waves && ok; ++w) {
         const int item = item_at(w);
         if (item >= n_items) continue;
-        int level, bh;
-        order.decode(item, level, bh);
-        const int len = row_length(p, bh / p.heads);
-        const int n_t = tiles_of(n_qt - 1 - level, len);
+        int qt, b, h, len;
+        open_item(item, qt, b, h, len);
+        const int n_t = tiles_of(qt, len);
         for (int t = 0; t < n_t; ++t, kr.next()) {
           if (!ends_inside(t, len, p.seqlen)) continue;
           if (!wait_warp(bar(B3_KL + kr.slot), (landed >> kr.slot) & 1u)) { ok = false; break; }
@@ -2905,36 +2932,24 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     for (int w = 0; w < n_waves && ok; ++w) {
       const int item = item_at(w);
       if (item >= n_items) continue;
-      int level, bh;
-      order.decode(item, level, bh);
-      const int qt = n_qt - 1 - level;
-      const int b = bh / p.heads, h = bh - b * p.heads;
-      const int len = X ? row_length(p, b) : p.seqlen;
+      int qt, b, h, len;
+      open_item(item, qt, b, h, len);
       const int n_t = tiles_of(qt, len);
       const int q0 = qt * 128;
       const int grow = q0 + row;
       const bool in = grow < len;
-      if (X && n_t == 0) {
-        float v[64];
-#pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = 0.0f;
-        if (wg < HP)
-          st_rows64(p.dq + (int64_t)b * p.dq_sb + (int64_t)(q0 + qd * 32) * p.dq_ss + (int64_t)h * p.dq_sh + wg * 64, p.dq_ss,
-                    p.seqlen - q0 - qd * 32, v);
-        continue;
-      }
-      const float lse2 = in ? p.lse[(int64_t)bh * p.seqlen + grow] * kLog2e : INFINITY;
-      const float dlt = in ? p.delta[(int64_t)bh * p.seqlen + grow] : 0.0f;
+      const int64_t at = ((int64_t)b * p.heads + h) * p.seqlen + grow;
+      const float lse2 = in ? p.lse[at] * kLog2e : INFINITY;
+      const float dlt = in ? p.delta[at] : 0.0f;
       const uint64_t sl2 = f2_pack(sl, sl), nlse2 = f2_pack(-lse2, -lse2), ndlt2 = f2_pack(-dlt, -dlt);
-      int lim = p.causal ? min(grow, len - 1) : len - 1;
-      if (X && !in) lim = -1;
+      const int lim = p.causal ? min(grow, len - 1) : len - 1;
       for (int t = 0; t < n_t; ++t) {
         const int gt = g0 + t;
         const int col0 = (2 * t + wg) * 64;
         const uint32_t tdp = tlane + TM_DP + (uint32_t)(gt & 1) * 128u + (uint32_t)wg * 64u;
         if (!wait_warp(bar(B_SF), (uint32_t)gt & 1u)) { ok = false; break; }
         tc5::fence_after_sync();
-        const bool need_mask = (p.causal && col0 + 63 > q0) || (col0 + 64 > len) || (X && q0 + 128 > len);
+        const bool need_mask = (p.causal && col0 + 63 > q0) || (col0 + 64 > len);
         uint32_t rs[2][32], rd[2][32];    // the scores become probabilities while dP is still being computed
         tc5::tmem_ld32(tlane + TM_S + (uint32_t)wg * 64u, rs[0]);
         tc5::tmem_ld32(tlane + TM_S + (uint32_t)wg * 64u + 32u, rs[1]);
@@ -2956,7 +2971,7 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         tc5::tmem_ld32(tdp, rd[0]);
         tc5::tmem_ld32(tdp + 32u, rd[1]);
         tc5::tmem_ld_wait();
-        if (X && need_mask) mask_above(rd, lim - col0, 0u);    // dP of padding may be anything
+        if (X == 2 && need_mask) mask_above(rd, lim - col0, 0u);    // dP of padding may be anything
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
@@ -2988,8 +3003,8 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (mine) {
         float v[64];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = X && !in ? 0.0f : __uint_as_float(r[i >> 5][i & 31]) * p.scale;
-        st_rows64(dq + wg * 64, p.dq_ss, p.seqlen - q0 - qd * 32, v);
+        for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i >> 5][i & 31]) * p.scale;
+        st_rows64(dq + wg * 64, p.dq_ss, len - q0 - qd * 32, v);
       }
       g0 += n_t;
       ++it;
@@ -3042,13 +3057,13 @@ struct Cfg {
 // warps have read dV and dK, the first products of the next item may overwrite the accumulators.
 // X: an item takes the query tiles of all (or, in `parts`, of some) query heads of its key / value head one after the other into the same
 // accumulators, so the sum over the heads is in 32 bits; parts leave theirs in `partial`, which attn_bwd_join_kernel adds up in order.
-// Q and dO tiles with rows behind the end of their sequence land on B3_QL and B3_OL and warp 3 clears those rows.  Key rows behind the
-// end are stored as zeros.
-template <int D, bool X>
+// X == 2: the key tiles of the plan, longest first.  Q and dO tiles with rows behind the end of their sequence land on B3_QL and B3_OL and
+// warp 3 clears those rows.
+template <int D, int X>
 __global__ void __launch_bounds__(kPsThreads, 1)
 attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const TcParams p, int n_kt,
-                        int n_items) {
+                        int max_items) {
   using C = dkv3::Cfg<D>;
   constexpr int HP = C::HP, NQ = C::NQ, ND = C::ND, NB = C::NB;
   constexpr bool PT_TMEM = C::PT_TMEM;
@@ -3083,26 +3098,36 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   };
   auto open_item = [&](int item) {
     Item x;
-    int idx;
-    order.decode(item, x.kt, idx);
+    int idx, n_len = nq_all;    // query tiles of the row
+    x.len = p.seqlen;
+    if (X == 2) {
+      const int per_tile = p.kv_heads * p.parts, n = item / per_tile;
+      int i;
+      planned_tile(p, n, n_kt, x.b, i);
+      idx = item - n * per_tile;
+      x.len = row_length(p, x.b);
+      n_len = (x.len + 127) / 128;
+      x.kt = p.causal ? n_len - 1 - i : i;    // as many query tiles as the i-th query tile has key tiles
+    } else {
+      order.decode(item, x.kt, idx);
+    }
     if (X) {
       const int bk = idx / p.parts;
       x.part = idx - bk * p.parts;
-      x.b = bk / p.kv_heads;
-      x.hk = bk - x.b * p.kv_heads;
+      if (X != 2) x.b = bk / p.kv_heads;
+      x.hk = X == 2 ? bk : bk - x.b * p.kv_heads;
       x.h = x.hk * p.rep + x.part * per_item;
-      x.len = row_length(p, x.b);
     } else {
       x.part = 0;
       x.b = idx / p.heads;
       x.h = x.hk = idx - x.b * p.heads;
-      x.len = p.seqlen;
     }
     x.t_first = p.causal ? x.kt : 0;
-    x.n_q = X ? (x.kt * 128 >= x.len ? 0 : (x.len + 127) / 128 - x.t_first) : nq_all - x.t_first;
+    x.n_q = n_len - x.t_first;
     x.n_u = X ? x.n_q * per_item : x.n_q;
     return x;
   };
+  const int n_items = X == 2 ? __ldg(p.plan) * p.kv_heads * p.parts : max_items;
   const int n_waves = (n_items + (int)gridDim.x - 1) / (int)gridDim.x;
   auto item_at = [&](int w) {
     const int c = (w & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x;
@@ -3130,7 +3155,7 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     tc5::mbar_init(bar(B_ACC), 1);
     tc5::mbar_init(bar(B3_KVE), 1);
     tc5::mbar_init(bar(B3_OE), 8);
-    if (X) {
+    if (X == 2) {
       for (int s = 0; s < NQ; ++s) tc5::mbar_init(bar(B3_QL + s), 1);
       for (int s = 0; s < ND; ++s) tc5::mbar_init(bar(B3_OL + s), 1);
     }
@@ -3161,7 +3186,6 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       if (item >= n_items) continue;
       const Item x = open_item(item);
       const int b = x.b, k0 = x.kt * 128;
-      if (X && x.n_u == 0) continue;
       if (it > 0 && !__all_sync(0xffffffffu, tc5::mbar_wait(bar(B3_KVE), (uint32_t)(it - 1) & 1u, abort_flag, p.status, kStatusBit))) break;
       if (lane == 0) {
         tc5::mbar_arrive_expect_tx(bar(B_KV), 2 * TILE);
@@ -3178,7 +3202,7 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const int s = gq % NQ, so = gq % ND;
         const int qrow0 = (x.t_first + t) * 128;
         if (!__all_sync(0xffffffffu, tc5::mbar_wait(bar(B_QE + s), ((uint32_t)(gq / NQ) & 1u) ^ 1u, abort_flag, p.status, kStatusBit))) { ok = false; break; }
-        const bool clear = X && ends_inside(x.t_first + t, x.len, p.seqlen);
+        const bool clear = X == 2 && ends_inside(x.t_first + t, x.len, p.seqlen);
         if (lane == 0) {
           const int landed = clear ? B3_QL + s : B_QF + s;
           tc5::mbar_arrive_expect_tx(bar(landed), TILE);
@@ -3273,7 +3297,6 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (item >= n_items) continue;
         const Item x = open_item(item);
         const int n_q = x.n_u;
-        if (X && n_q == 0) continue;
         if (!tc5::mbar_wait(bar(B_KV), (uint32_t)it & 1u, abort_flag, p.status, kStatusBit)) { ok = false; break; }
         if (!wait_for(B_QF + g0 % NQ, g0 / NQ)) { ok = false; break; }
         if (!PT_TMEM && g0 > 0 && !wait_for(B_SE, g0 - 1)) { ok = false; break; }
@@ -3323,7 +3346,7 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         g0 += n_q;
         ++it;
       }
-    } else if (X && warp == 3 && p.lengths) {
+    } else if (X == 2 && warp == 3) {
       // ------------------------------------------------------------------ Q and dO rows behind the end of their sequence
       int gq = 0;
       uint32_t landed_q = 0u, landed_o = 0u;    // bit s: parity of the next such tile in slot s
@@ -3333,7 +3356,7 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (item >= n_items) continue;
         const Item x = open_item(item);
         const int last = x.t_first + x.n_q - 1;    // query tile
-        const bool ragged = x.n_u > 0 && ends_inside(last, x.len, p.seqlen);
+        const bool ragged = ends_inside(last, x.len, p.seqlen);
         for (int n = x.n_q; ragged && n <= x.n_u; n += x.n_q) {
           const int s = (gq + n - 1) % NQ, so = (gq + n - 1) % ND;    // the last tile of a head
           if (!wait_warp(bar(B3_QL + s), (landed_q >> s) & 1u)) { ok = false; break; }
@@ -3359,15 +3382,6 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const uint32_t tlane = tmem_base + ((uint32_t)(qd * 32) << 16);
     const float sl = p.scale * kLog2e;
     const uint64_t sl2 = f2_pack(sl, sl);
-    // X: rows of a key tile behind the end of its sequence
-    auto store_zeros = [&](int item) {
-      const Item x = open_item(item);
-      const int r0 = x.kt * 128 + qd * 32;
-      const int64_t ss = wg == 0 ? p.dv_ss : p.dk_ss;
-      __nv_bfloat16* dst = wg == 0 ? p.dv + (int64_t)x.b * p.dv_sb + (int64_t)x.hk * p.dv_sh : p.dk + (int64_t)x.b * p.dk_sb + (int64_t)x.hk * p.dk_sh;
-      if (r0 + lane < p.seqlen)
-        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(dst + (r0 + lane) * ss + c) = make_uint4(0u, 0u, 0u, 0u);
-    };
     const uint32_t prow0 = base + OFF_PT + (uint32_t)wg * PANEL + (uint32_t)row * 128u;
     const uint32_t swz = (uint32_t)(row & 7);
     int g0 = 0, it = 0;
@@ -3382,10 +3396,6 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         n_q = x.n_u;
         t_first = x.t_first;
         n_head = x.n_q;
-      }
-      if (X && n_q == 0) {    // padding only
-        if (p.parts == 1) store_zeros(item);
-        continue;
       }
       const int grow = k0 + row;
       int t = 0;    // query tile of its head
@@ -3492,9 +3502,8 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       if (lane == 0) tc5::mbar_arrive(bar(B3_OE));
       g0 += n_q;
       ++it;
-      const bool in = !X || grow < x.len;
       if (X && p.parts > 1) {
-        if (in) {
+        if (grow < x.len) {
           float* out = p.partial + ((((int64_t)x.part * 2 + 1 - wg) * p.batch + b) * p.kv_heads + h) * p.seqlen * D + (int64_t)grow * D;
 #pragma unroll
           for (int c = 0; c < D / 32; ++c)
@@ -3509,8 +3518,8 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       for (int c = 0; c < D / 32; c += 2) {
         float v[64];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = in ? __uint_as_float(acc[c + (i >> 5)][i & 31]) * f : 0.0f;
-        st_rows64(dst + c * 32, wg == 0 ? p.dv_ss : p.dk_ss, p.seqlen - k0 - qd * 32, v);
+        for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(acc[c + (i >> 5)][i & 31]) * f;
+        st_rows64(dst + c * 32, wg == 0 ? p.dv_ss : p.dk_ss, x.len - k0 - qd * 32, v);
       }
     }
   }
@@ -3544,9 +3553,9 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const JoinParams p) 
   const int64_t bh = row / p.seqlen;
   const int h = (int)(bh % p.kv_heads);
   const int64_t b = bh / p.kv_heads;
-  const int parts = p.lengths && s >= __ldg(p.lengths + b) ? 0 : p.parts;    // nothing was left for padding
+  if (p.lengths && s >= __ldg(p.lengths + b)) return;    // padding: cleared before
   float v[8] = {};
-  for (int k = 0; k < parts; ++k) {
+  for (int k = 0; k < p.parts; ++k) {
     const float4* src = reinterpret_cast<const float4*>(p.partial + ((int64_t)k * 2 * rows + r) * D + c);
     const float4 a = src[0], b = src[1];
     v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
@@ -3554,6 +3563,48 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const JoinParams p) 
   }
   __nv_bfloat16* dst = is_v ? p.dv + b * p.dv_sb + (int64_t)s * p.dv_ss + (int64_t)h * p.dv_sh : p.dk + b * p.dk_sb + (int64_t)s * p.dk_ss + (int64_t)h * p.dk_sh;
   *reinterpret_cast<uint4*>(dst + c) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+// Row lengths of a padded batch: the list of 128-row tiles that hold rows of a sequence, longest work first, and zeros (lse: -inf) for the
+// output rows of padding.  plan[0]: number of tiles; plan[1 + rank]: b * n_tiles + i for tile i of batch b.  The work of tile i is i + 1 tiles
+// when causal, else those of its row; ties go by batch, then by tile.  A tile counts the tiles in front of it, O(batch) each, so that no
+// sort and no atomic is needed.  blockIdx.x: batch, blockIdx.y: share of its padding.
+struct PlanParams {
+  const int* lengths;
+  int* plan;
+  __nv_bfloat16* o;
+  float* lse;
+  int64_t o_sb, o_ss, o_sh;
+  int batch, heads, seqlen, head_dim, n_tiles, causal;
+};
+__global__ void __launch_bounds__(256) attn_plan_kernel(const PlanParams p) {
+  const int b = blockIdx.x;
+  const int len = row_length(p.lengths, b, p.seqlen), n = (len + 127) / 128;
+  if (blockIdx.y == 0) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      int rank = p.causal ? 0 : i;
+      for (int c = 0; c < p.batch; ++c) {
+        const int m = (row_length(p.lengths, c, p.seqlen) + 127) / 128;
+        if (p.causal) rank += max(0, m - i - 1) + (c < b && m > i ? 1 : 0);
+        else          rank += m > n || (m == n && c < b) ? m : 0;
+      }
+      p.plan[1 + rank] = b * p.n_tiles + i;
+    }
+    if (b == 0 && threadIdx.x == 0) {
+      int total = 0;
+      for (int c = 0; c < p.batch; ++c) total += (row_length(p.lengths, c, p.seqlen) + 127) / 128;
+      p.plan[0] = total;
+    }
+  }
+  const int per_head = p.head_dim / 8, per_row = p.heads * per_head;
+  const int64_t todo = (int64_t)(p.seqlen - len) * per_row;
+  for (int64_t k = (int64_t)blockIdx.y * blockDim.x + threadIdx.x; k < todo; k += (int64_t)gridDim.y * blockDim.x) {
+    const int64_t row = k / per_row;
+    const int r = (int)(k - row * per_row), h = r / per_head, c = r - h * per_head;
+    const int64_t s = len + row;
+    *reinterpret_cast<uint4*>(p.o + b * p.o_sb + s * p.o_ss + h * p.o_sh + c * 8) = make_uint4(0u, 0u, 0u, 0u);
+    if (c == 0) p.lse[((int64_t)b * p.heads + h) * p.seqlen + s] = -INFINITY;
+  }
 }
 
 // ---- host side -----------------------------------------------------------------------------------
@@ -3769,11 +3820,11 @@ MSAMP_API int msamp_attention_tc_fwd(const void* q, const void* k, const void* v
     return msamp_check_launch("attn_fwd_split_kernel");
   }
   if (head_dim == 128) {
-    if ((rc = set_smem(attn_fwd_ps_kernel<128, false>, fwd3::Cfg<128>::SMEM))) return rc;
-    attn_fwd_ps_kernel<128, false><<<ctas, kPsThreads, fwd3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
+    if ((rc = set_smem(attn_fwd_ps_kernel<128, 0>, fwd3::Cfg<128>::SMEM))) return rc;
+    attn_fwd_ps_kernel<128, 0><<<ctas, kPsThreads, fwd3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
   } else {
-    if ((rc = set_smem(attn_fwd_ps_kernel<64, false>, fwd3::Cfg<64>::SMEM))) return rc;
-    attn_fwd_ps_kernel<64, false><<<ctas, kPsThreads, fwd3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
+    if ((rc = set_smem(attn_fwd_ps_kernel<64, 0>, fwd3::Cfg<64>::SMEM))) return rc;
+    attn_fwd_ps_kernel<64, 0><<<ctas, kPsThreads, fwd3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
   }
   return msamp_check_launch("attn_fwd_ps_kernel");
 }
@@ -3817,8 +3868,8 @@ MSAMP_API int msamp_attention_tc_bwd(const void* q, const void* k, const void* v
     const int64_t rows = (int64_t)batch * heads * seqlen;
     const int per_cta = 2 * 256 / (head_dim / 8);
     const unsigned blocks = (unsigned)((rows + per_cta - 1) / per_cta);
-    if (head_dim == 128) attn_delta_tc_kernel<128><<<blocks, 256, 0, stream>>>(d);
-    else                 attn_delta_tc_kernel<64><<<blocks, 256, 0, stream>>>(d);
+    if (head_dim == 128) attn_delta_tc_kernel<128, false><<<blocks, 256, 0, stream>>>(d);
+    else                 attn_delta_tc_kernel<64, false><<<blocks, 256, 0, stream>>>(d);
   }
   TcParams p = {};
   p.lse = const_cast<float*>(lse); p.delta = delta;
@@ -3844,62 +3895,83 @@ MSAMP_API int msamp_attention_tc_bwd(const void* q, const void* k, const void* v
     if ((rc = set_smem(attn_bwd_dq_tm_kernel, dqk2::SMEM))) return rc;
     attn_bwd_dq_tm_kernel<<<grid, kTcThreads, dqk2::SMEM, stream>>>(mq, mk, mv, mdo, p);
   } else if (head_dim == 128) {
-    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<128, false>, dkv3::Cfg<128>::SMEM))) return rc;
-    attn_bwd_dkdv_ps_kernel<128, false><<<ctas, kPsThreads, dkv3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
-    if ((rc = set_smem(attn_bwd_dq_ps_kernel<128, false>, dqk3::Cfg<128>::SMEM))) return rc;
-    attn_bwd_dq_ps_kernel<128, false><<<ctas, kPsThreads, dqk3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
+    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<128, 0>, dkv3::Cfg<128>::SMEM))) return rc;
+    attn_bwd_dkdv_ps_kernel<128, 0><<<ctas, kPsThreads, dkv3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
+    if ((rc = set_smem(attn_bwd_dq_ps_kernel<128, 0>, dqk3::Cfg<128>::SMEM))) return rc;
+    attn_bwd_dq_ps_kernel<128, 0><<<ctas, kPsThreads, dqk3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
   } else {
-    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<64, false>, dkv3::Cfg<64>::SMEM))) return rc;
-    attn_bwd_dkdv_ps_kernel<64, false><<<ctas, kPsThreads, dkv3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
-    if ((rc = set_smem(attn_bwd_dq_ps_kernel<64, false>, dqk3::Cfg<64>::SMEM))) return rc;
-    attn_bwd_dq_ps_kernel<64, false><<<ctas, kPsThreads, dqk3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
+    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<64, 0>, dkv3::Cfg<64>::SMEM))) return rc;
+    attn_bwd_dkdv_ps_kernel<64, 0><<<ctas, kPsThreads, dkv3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
+    if ((rc = set_smem(attn_bwd_dq_ps_kernel<64, 0>, dqk3::Cfg<64>::SMEM))) return rc;
+    attn_bwd_dq_ps_kernel<64, 0><<<ctas, kPsThreads, dqk3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_items);
   }
   return msamp_check_launch("attn_bwd_tc kernels");
 }
 
 // ---- shared key / value heads and row lengths ----------------------------------------------------
 // Query heads h * rep .. h * rep + rep - 1 read key / value head h (heads == kv_heads * rep).  lengths [batch] (int32, or null): positions at or
-// behind a row's length are padding, as queries and as keys; their outputs and gradients are zero, their lse -inf, whatever they hold.
+// behind a row's length are padding, as queries and as keys; their outputs and gradients are zero, their lse -inf, whatever they hold.  With
+// lengths the forward pass writes `plan` (1 + batch * ceil(seqlen / 128) ints), which the backward pass of the same lengths reads.
 // Strides as for the entry points above, those of k, v, dk and dv over kv_heads.
-static int shared_checks(const char* what, int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, const int64_t* strides, int n) {
-  MSAMP_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128 (got %d)", what, head_dim);
-  MSAMP_REQUIRE(batch > 0 && heads > 0 && kv_heads > 0 && seqlen > 0, "%s: empty problem", what);
-  MSAMP_REQUIRE(heads % kv_heads == 0, "%s: %d query heads do not share %d key / value heads evenly", what, heads, kv_heads);
-  MSAMP_REQUIRE(scale > 0.0f && scale <= 3.0e38f, "%s: the scale must be positive", what);
+static int shared_checks(int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, const int* lengths, const int* plan,
+                         const int64_t* strides, int n) {
+  MSAMP_REQUIRE(head_dim == 64 || head_dim == 128, "attention (shared heads): head_dim must be 64 or 128 (got %d)", head_dim);
+  MSAMP_REQUIRE(batch > 0 && heads > 0 && kv_heads > 0 && seqlen > 0, "attention (shared heads): empty problem");
+  MSAMP_REQUIRE(heads % kv_heads == 0, "attention: %d query heads do not share %d key / value heads evenly", heads, kv_heads);
+  MSAMP_REQUIRE(scale > 0.0f && scale <= 3.0e38f, "attention (shared heads): the scale must be positive");
+  MSAMP_REQUIRE(!lengths || plan, "attention (shared heads): lengths without a plan");
   // work items and query tiles are counted in 32 bits
-  MSAMP_REQUIRE((int64_t)((seqlen + 127) / 128) * batch * heads <= (1 << 30), "%s: too many work items", what);
-  for (int i = 0; i < n; ++i) MSAMP_REQUIRE(strides[i] % 8 == 0, "%s: stride %d is not a multiple of 8 elements", what, i);
+  MSAMP_REQUIRE((int64_t)((seqlen + 127) / 128) * batch * heads <= (1 << 30), "attention (shared heads): too many work items");
+  for (int i = 0; i < n; ++i) MSAMP_REQUIRE(strides[i] % 8 == 0, "attention (shared heads): stride %d is not a multiple of 8 elements", i);
   return MSAMP_OK;
 }
 
-MSAMP_API int msamp_attention_shared_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* lengths, const int64_t* strides,
-                                         int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, int causal, void* stream_) {
-  int rc = shared_checks("attention (shared heads)", batch, heads, kv_heads, seqlen, head_dim, scale, strides, 12);
+template <int D, int X>
+static int launch_fwd(const CUtensorMap (&m)[3], const TcParams& p, int n_qt, int ctas, cudaStream_t stream) {
+  if (int rc = set_smem(attn_fwd_ps_kernel<D, X>, fwd3::Cfg<D>::SMEM)) return rc;
+  attn_fwd_ps_kernel<D, X><<<ctas, kPsThreads, fwd3::Cfg<D>::SMEM, stream>>>(m[0], m[1], m[2], p, n_qt, n_qt * p.batch * p.heads);
+  return MSAMP_OK;
+}
+template <int D, int X>
+static int launch_bwd(const CUtensorMap (&m)[4], const TcParams& p, int n_t, int sms, cudaStream_t stream) {
+  if (int rc = set_smem(attn_bwd_dkdv_ps_kernel<D, X>, dkv3::Cfg<D>::SMEM)) return rc;
+  if (int rc = set_smem(attn_bwd_dq_ps_kernel<D, X>, dqk3::Cfg<D>::SMEM)) return rc;
+  const int n_q = n_t * p.batch * p.heads, n_k = n_t * p.batch * p.kv_heads * p.parts;
+  attn_bwd_dkdv_ps_kernel<D, X><<<n_k < sms ? n_k : sms, kPsThreads, dkv3::Cfg<D>::SMEM, stream>>>(m[0], m[1], m[2], m[3], p, n_t, n_k);
+  attn_bwd_dq_ps_kernel<D, X><<<n_q < sms ? n_q : sms, kPsThreads, dqk3::Cfg<D>::SMEM, stream>>>(m[0], m[1], m[2], m[3], p, n_t, n_q);
+  return MSAMP_OK;
+}
+
+MSAMP_API int msamp_attention_shared_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* lengths, int* plan,
+                                         const int64_t* strides, int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale,
+                                         int causal, void* stream_) {
+  int rc = shared_checks(batch, heads, kv_heads, seqlen, head_dim, scale, lengths, plan, strides, 12);
   if (rc) return rc;
   MSAMP_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "attention (shared heads): q, k, v and o must be 16-byte aligned");
-  CUtensorMap mq, mk, mv;
-  if ((rc = make_map4(q, batch, heads, seqlen, head_dim, strides[0], strides[1], strides[2], 128, &mq))) return rc;
-  if ((rc = make_map4(k, batch, kv_heads, seqlen, head_dim, strides[3], strides[4], strides[5], 128, &mk))) return rc;
-  if ((rc = make_map4(v, batch, kv_heads, seqlen, head_dim, strides[6], strides[7], strides[8], 128, &mv))) return rc;
+  CUtensorMap m[3];
+  if ((rc = make_map4(q, batch, heads, seqlen, head_dim, strides[0], strides[1], strides[2], 128, &m[0]))) return rc;
+  if ((rc = make_map4(k, batch, kv_heads, seqlen, head_dim, strides[3], strides[4], strides[5], 128, &m[1]))) return rc;
+  if ((rc = make_map4(v, batch, kv_heads, seqlen, head_dim, strides[6], strides[7], strides[8], 128, &m[2]))) return rc;
   TcParams p = {};
   p.o = (__nv_bfloat16*)o; p.lse = lse;
   p.o_sb = strides[9]; p.o_ss = strides[10]; p.o_sh = strides[11];
   p.batch = batch; p.heads = heads; p.seqlen = seqlen; p.causal = causal; p.scale = scale;
-  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.lengths = lengths;
+  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.lengths = lengths; p.plan = plan;
   p.status = msamp_device_status_ptr();
   p.group = item_group(seqlen, head_dim);
   const int n_qt = (seqlen + 127) / 128;
-  const int n_items = n_qt * batch * heads;
-  const int ctas = n_items < msamp_sm_count() ? n_items : msamp_sm_count();
+  const int n_items = n_qt * batch * heads, sms = msamp_sm_count();
+  const int ctas = n_items < sms ? n_items : sms;
   cudaStream_t stream = (cudaStream_t)stream_;
-  if (head_dim == 128) {
-    if ((rc = set_smem(attn_fwd_ps_kernel<128, true>, fwd3::Cfg<128>::SMEM))) return rc;
-    attn_fwd_ps_kernel<128, true><<<ctas, kPsThreads, fwd3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
+  if (lengths) {
+    PlanParams w = {lengths, plan, p.o, lse, p.o_sb, p.o_ss, p.o_sh, batch, heads, seqlen, head_dim, n_qt, causal};
+    const int share = (4 * sms + batch - 1) / batch;
+    attn_plan_kernel<<<dim3((unsigned)batch, (unsigned)(share < 64 ? share : 64)), 256, 0, stream>>>(w);
+    rc = head_dim == 128 ? launch_fwd<128, 2>(m, p, n_qt, ctas, stream) : launch_fwd<64, 2>(m, p, n_qt, ctas, stream);
   } else {
-    if ((rc = set_smem(attn_fwd_ps_kernel<64, true>, fwd3::Cfg<64>::SMEM))) return rc;
-    attn_fwd_ps_kernel<64, true><<<ctas, kPsThreads, fwd3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, p, n_qt, n_items);
+    rc = head_dim == 128 ? launch_fwd<128, 1>(m, p, n_qt, ctas, stream) : launch_fwd<64, 1>(m, p, n_qt, ctas, stream);
   }
-  return msamp_check_launch("attn_fwd_ps_kernel (shared heads)");
+  return rc ? rc : msamp_check_launch("attention forward (shared heads)");
 }
 
 // Parts into which the query heads of a key / value head are cut for dK / dV: the smallest divisor of `rep` that gives every SM an item.
@@ -3913,32 +3985,21 @@ MSAMP_API int msamp_attention_shared_parts(int batch, int heads, int kv_heads, i
 
 // partial: parts * 2 * batch * kv_heads * seqlen * head_dim floats when msamp_attention_shared_parts gives more than one part.
 MSAMP_API int msamp_attention_shared_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq,
-                                         void* dk, void* dv, float* delta, float* partial, const int* lengths, const int64_t* strides, int batch,
-                                         int heads, int kv_heads, int seqlen, int head_dim, float scale, int causal, void* stream_) {
-  int rc = shared_checks("attention (shared heads)", batch, heads, kv_heads, seqlen, head_dim, scale, strides, 24);
+                                         void* dk, void* dv, float* delta, float* partial, const int* lengths, const int* plan,
+                                         const int64_t* strides, int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale,
+                                         int causal, void* stream_) {
+  int rc = shared_checks(batch, heads, kv_heads, seqlen, head_dim, scale, lengths, plan, strides, 24);
   if (rc) return rc;
   MSAMP_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(d_o) && aligned16(dq) && aligned16(dk) && aligned16(dv),
                 "attention (shared heads): q, k, v, o, dO and the gradients must be 16-byte aligned");
   const int parts = msamp_attention_shared_parts(batch, heads, kv_heads, seqlen);
   MSAMP_REQUIRE(parts == 1 || (partial && aligned16(partial)), "attention (shared heads): no workspace for %d parts", parts);
-  CUtensorMap mq, mk, mv, mdo;
-  if ((rc = make_map4(q, batch, heads, seqlen, head_dim, strides[0], strides[1], strides[2], 128, &mq))) return rc;
-  if ((rc = make_map4(k, batch, kv_heads, seqlen, head_dim, strides[3], strides[4], strides[5], 128, &mk))) return rc;
-  if ((rc = make_map4(v, batch, kv_heads, seqlen, head_dim, strides[6], strides[7], strides[8], 128, &mv))) return rc;
-  if ((rc = make_map4(d_o, batch, heads, seqlen, head_dim, strides[12], strides[13], strides[14], 128, &mdo))) return rc;
+  CUtensorMap m[4];
+  if ((rc = make_map4(q, batch, heads, seqlen, head_dim, strides[0], strides[1], strides[2], 128, &m[0]))) return rc;
+  if ((rc = make_map4(k, batch, kv_heads, seqlen, head_dim, strides[3], strides[4], strides[5], 128, &m[1]))) return rc;
+  if ((rc = make_map4(v, batch, kv_heads, seqlen, head_dim, strides[6], strides[7], strides[8], 128, &m[2]))) return rc;
+  if ((rc = make_map4(d_o, batch, heads, seqlen, head_dim, strides[12], strides[13], strides[14], 128, &m[3]))) return rc;
   cudaStream_t stream = (cudaStream_t)stream_;
-  {
-    DeltaParams d = {};
-    d.o = (const __nv_bfloat16*)o; d.d_o = (const __nv_bfloat16*)d_o; d.delta = delta;
-    d.o_sb = strides[9]; d.o_ss = strides[10]; d.o_sh = strides[11];
-    d.do_sb = strides[12]; d.do_ss = strides[13]; d.do_sh = strides[14];
-    d.batch = batch; d.heads = heads; d.seqlen = seqlen;
-    const int64_t rows = (int64_t)batch * heads * seqlen;
-    const int per_cta = 2 * 256 / (head_dim / 8);
-    const unsigned blocks = (unsigned)((rows + per_cta - 1) / per_cta);
-    if (head_dim == 128) attn_delta_tc_kernel<128><<<blocks, 256, 0, stream>>>(d);
-    else                 attn_delta_tc_kernel<64><<<blocks, 256, 0, stream>>>(d);
-  }
   TcParams p = {};
   p.lse = const_cast<float*>(lse); p.delta = delta;
   p.dq = (__nv_bfloat16*)dq; p.dk = (__nv_bfloat16*)dk; p.dv = (__nv_bfloat16*)dv;
@@ -3946,23 +4007,32 @@ MSAMP_API int msamp_attention_shared_bwd(const void* q, const void* k, const voi
   p.dk_sb = strides[18]; p.dk_ss = strides[19]; p.dk_sh = strides[20];
   p.dv_sb = strides[21]; p.dv_ss = strides[22]; p.dv_sh = strides[23];
   p.batch = batch; p.heads = heads; p.seqlen = seqlen; p.causal = causal; p.scale = scale;
-  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.lengths = lengths; p.parts = parts; p.partial = partial;
+  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.lengths = lengths; p.plan = plan; p.parts = parts; p.partial = partial;
   p.status = msamp_device_status_ptr();
   p.group = item_group(seqlen, head_dim);
-  const int n_t = (seqlen + 127) / 128;    // key tiles of dK / dV, query tiles of dQ
-  const int n_q = n_t * batch * heads, n_k = n_t * batch * kv_heads * parts;
-  const int sms = msamp_sm_count();
-  if (head_dim == 128) {
-    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<128, true>, dkv3::Cfg<128>::SMEM))) return rc;
-    if ((rc = set_smem(attn_bwd_dq_ps_kernel<128, true>, dqk3::Cfg<128>::SMEM))) return rc;
-    attn_bwd_dkdv_ps_kernel<128, true><<<n_k < sms ? n_k : sms, kPsThreads, dkv3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_k);
-    attn_bwd_dq_ps_kernel<128, true><<<n_q < sms ? n_q : sms, kPsThreads, dqk3::Cfg<128>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_q);
-  } else {
-    if ((rc = set_smem(attn_bwd_dkdv_ps_kernel<64, true>, dkv3::Cfg<64>::SMEM))) return rc;
-    if ((rc = set_smem(attn_bwd_dq_ps_kernel<64, true>, dqk3::Cfg<64>::SMEM))) return rc;
-    attn_bwd_dkdv_ps_kernel<64, true><<<n_k < sms ? n_k : sms, kPsThreads, dkv3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_k);
-    attn_bwd_dq_ps_kernel<64, true><<<n_q < sms ? n_q : sms, kPsThreads, dqk3::Cfg<64>::SMEM, stream>>>(mq, mk, mv, mdo, p, n_t, n_q);
+  {
+    DeltaParams d = {};
+    d.o = (const __nv_bfloat16*)o; d.d_o = (const __nv_bfloat16*)d_o; d.delta = delta;
+    d.o_sb = strides[9]; d.o_ss = strides[10]; d.o_sh = strides[11];
+    d.do_sb = strides[12]; d.do_ss = strides[13]; d.do_sh = strides[14];
+    d.batch = batch; d.heads = heads; d.seqlen = seqlen;
+    d.lengths = lengths; d.kv_heads = kv_heads;
+    d.dq = p.dq; d.dq_sb = p.dq_sb; d.dq_ss = p.dq_ss; d.dq_sh = p.dq_sh;
+    d.dk = p.dk; d.dk_sb = p.dk_sb; d.dk_ss = p.dk_ss; d.dk_sh = p.dk_sh;
+    d.dv = p.dv; d.dv_sb = p.dv_sb; d.dv_ss = p.dv_ss; d.dv_sh = p.dv_sh;
+    const int64_t rows = (int64_t)batch * heads * seqlen;
+    const int per_cta = 2 * 256 / (head_dim / 8);
+    const unsigned blocks = (unsigned)((rows + per_cta - 1) / per_cta);
+    if (head_dim == 128 && lengths) attn_delta_tc_kernel<128, true><<<blocks, 256, 0, stream>>>(d);
+    else if (head_dim == 128)       attn_delta_tc_kernel<128, false><<<blocks, 256, 0, stream>>>(d);
+    else if (lengths)               attn_delta_tc_kernel<64, true><<<blocks, 256, 0, stream>>>(d);
+    else                            attn_delta_tc_kernel<64, false><<<blocks, 256, 0, stream>>>(d);
   }
+  const int n_t = (seqlen + 127) / 128;    // key tiles of dK / dV, query tiles of dQ
+  const int sms = msamp_sm_count();
+  if (lengths) rc = head_dim == 128 ? launch_bwd<128, 2>(m, p, n_t, sms, stream) : launch_bwd<64, 2>(m, p, n_t, sms, stream);
+  else         rc = head_dim == 128 ? launch_bwd<128, 1>(m, p, n_t, sms, stream) : launch_bwd<64, 1>(m, p, n_t, sms, stream);
+  if (rc) return rc;
   if (parts > 1) {
     JoinParams j = {};
     j.partial = partial; j.dk = p.dk; j.dv = p.dv;

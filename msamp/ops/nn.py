@@ -407,18 +407,20 @@ def _shared_fwd(q, k, v, causal, scale, lengths):
     B, S, nh, d = q.shape
     o = torch.empty((B, S, nh, d), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, nh, S), dtype=torch.float32, device=q.device)
+    # with lengths: the tiles that are not padding, listed by the forward pass for both passes
+    plan = torch.empty(1 + B * ((S + 127) // 128), dtype=torch.int32, device=q.device) if lengths is not None else None
     st = _map_strides(q) + _map_strides(k) + _map_strides(v) + _map_strides(o) + [0] * 12
     with native.on_device(q):
         native.check(
             native.lib().msamp_attention_shared_fwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), native.addr(lengths), _i64x24(*st), B, nh, k.shape[2], S,
-                d, scale, int(causal), native.raw_stream()
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), native.addr(lengths), native.addr(plan), _i64x24(*st), B,
+                nh, k.shape[2], S, d, scale, int(causal), native.raw_stream()
             ), 'attention_fwd'
         )
-    return o, lse
+    return o, lse, plan
 
 
-def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths):
+def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths, plan):
     B, S, nh, d = q.shape
     nkv = k.shape[2]
     o, d_o = _rows16(_mappable(o)), _rows16(_mappable(d_o))
@@ -430,8 +432,8 @@ def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths):
         native.check(
             native.lib().msamp_attention_shared_bwd(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                delta.data_ptr(), native.addr(partial), native.addr(lengths), _i64x24(*st), B, nh, nkv, S, d, scale, int(causal),
-                native.raw_stream()
+                delta.data_ptr(), native.addr(partial), native.addr(lengths), native.addr(plan), _i64x24(*st), B, nh, nkv, S, d, scale,
+                int(causal), native.raw_stream()
             ), 'attention_bwd'
         )
 
@@ -439,14 +441,14 @@ def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths):
 class _AttentionSharedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, causal, scale, grad_layout, lengths):
-        o, lse = _shared_fwd(q, k, v, causal, scale, lengths)
-        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        o, lse, plan = _shared_fwd(q, k, v, causal, scale, lengths)
+        ctx.save_for_backward(q, k, v, o, lse, lengths, plan)
         ctx.causal, ctx.scale, ctx.grad_layout = causal, scale, grad_layout
         return o
 
     @staticmethod
     def backward(ctx, d_o):
-        q, k, v, o, lse, lengths = ctx.saved_tensors
+        q, k, v, o, lse, lengths, plan = ctx.saved_tensors
         q, k, v = (_rows16(t) for t in (q, k, v))    # saved tensors may come back with other strides
         B, S, nh, d = q.shape
         if ctx.grad_layout == 'packed':
@@ -454,7 +456,7 @@ class _AttentionSharedFn(torch.autograd.Function):
             dq, dk, dv = buf.split([nh, k.shape[2], k.shape[2]], dim=2)
         else:
             dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, ctx.causal, ctx.scale, lengths)
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, ctx.causal, ctx.scale, lengths, plan)
         return dq, dk, dv, None, None, None, None
 
 
@@ -485,22 +487,22 @@ def _attention_plain(q, k, v, causal, scale, lengths):
 
 
 def attention_shared_fwd_raw(q, k, v, causal=True, scale=None, lengths=None):
-    """Forward pass of :func:`attention` with shared key/value heads or row lengths, without autograd: ``(o, lse or None)``."""
+    """Forward pass of :func:`attention` with shared key/value heads or row lengths, without autograd: ``(o, lse, plan)`` for its gradients."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if _use_native(q) and q.numel():
         q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
         return _shared_fwd(q, k, v, causal, scale, lengths)
     _check_shared(q, k, v, scale, lengths)
     with torch.no_grad():
-        return _attention_plain(q, k, v, causal, scale, lengths), None
+        return _attention_plain(q, k, v, causal, scale, lengths), None, None
 
 
-def attention_shared_bwd_raw(q, k, v, o, lse, d_o, dq, dk, dv, causal=True, scale=None, lengths=None):
+def attention_shared_bwd_raw(q, k, v, o, lse, plan, d_o, dq, dk, dv, causal=True, scale=None, lengths=None):
     """Its gradients, written into ``dq``, ``dk`` and ``dv`` (views with unit inner stride and 16-byte aligned rows)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if _use_native(q) and q.numel():
         q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths)
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths, plan)
         return
     with torch.enable_grad():
         leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]

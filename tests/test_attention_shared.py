@@ -278,16 +278,17 @@ def test_entry_points_refuse():
     lib, at = native.lib(), 1 << 20
     good = [768, 256, 64] * 8
 
-    def fwd(ptrs=None, strides=good, sizes=(2, 4, 2, 3, 64), scale=0.125):
-        return lib.msamp_attention_shared_fwd(*(ptrs or [at] * 5), None, (ctypes.c_int64 * 24)(*strides), *sizes, scale, 1, None)
+    def fwd(ptrs=None, strides=good, sizes=(2, 4, 2, 3, 64), scale=0.125, lengths=None):
+        return lib.msamp_attention_shared_fwd(*(ptrs or [at] * 5), lengths, None, (ctypes.c_int64 * 24)(*strides), *sizes, scale, 1, None)
 
-    def bwd(ptrs=None, strides=good, sizes=(2, 4, 2, 3, 64), scale=0.125, partial=at):
-        return lib.msamp_attention_shared_bwd(*(ptrs or [at] * 10), partial, None, (ctypes.c_int64 * 24)(*strides), *sizes, scale, 1, None)
+    def bwd(ptrs=None, strides=good, sizes=(2, 4, 2, 3, 64), scale=0.125, partial=at, lengths=None):
+        return lib.msamp_attention_shared_bwd(*(ptrs or [at] * 10), partial, lengths, None, (ctypes.c_int64 * 24)(*strides), *sizes, scale, 1, None)
 
     odd = good[:4] + [260] + good[5:]
     for call in (fwd, bwd):
         assert call(strides=odd) == 1 and call(sizes=(2, 4, 2, 3, 96)) == 1 and call(sizes=(2, 4, 3, 3, 64)) == 1
         assert call(sizes=(0, 4, 2, 3, 64)) == 1 and call(sizes=(2, 4, 2, 0, 64)) == 1 and call(sizes=(2, 4, 0, 3, 64)) == 1
+        assert call(lengths=at) == 1    # without a plan
         assert call(scale=0.0) == 1 and call(scale=-1.0) == 1 and call(scale=float('nan')) == 1
         assert call(sizes=(1 << 14, 1 << 14, 1, 1 << 10, 64)) == 1
     for i in (0, 1, 2, 3):
