@@ -296,18 +296,27 @@ def _check_blocks(codes, exponents):
         raise ValueError(f'blocks: {codes.numel()} codes need {(codes.numel() + BLOCK - 1) // BLOCK} exponents (got {exponents.numel()})')
 
 
-def _blocks_cast(x, want_gelu):
-    """``(codes, exponents, gelu(x) or None)`` of a contiguous CUDA tensor in one pass."""
-    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
-    exponents = torch.empty((x.numel() + BLOCK - 1) // BLOCK, dtype=torch.uint8, device=x.device)
-    y = torch.empty_like(x) if want_gelu else None
+def _gelu_keep(x):
+    """GeLU of a contiguous CUDA tensor and, from the same read, its e4m3 blocks: ``(codes then exponents in one buffer, y)``."""
+    n = x.numel()
+    y = torch.empty_like(x)
+    kept = x.new_empty(n + (n + BLOCK - 1) // BLOCK, dtype=torch.uint8)
+    at = kept.data_ptr()
     with native.on_device(x):
+        native.check(native.lib().msamp_blocks_cast(x.data_ptr(), y.data_ptr(), at, at + n, n, native.dt(x.dtype), native.raw_stream()), 'gelu')
+    return kept, y
+
+
+def _gelu_keep_bwd(kept, dy):
+    """Its gradient for a contiguous ``dy``."""
+    n = dy.numel()
+    dx = torch.empty_like(dy)
+    at = kept.data_ptr()
+    with native.on_device(dy):
         native.check(
-            native.lib().msamp_blocks_cast(
-                x.data_ptr(), native.addr(y), codes.data_ptr(), exponents.data_ptr(), x.numel(), native.dt(x.dtype), native.raw_stream()
-            ), 'cast_blocks_to_fp8'
+            native.lib().msamp_blocks_uncast(at, at + n, dy.data_ptr(), dx.data_ptr(), n, native.dt(dy.dtype), native.raw_stream()), 'gelu_bwd'
         )
-    return codes, exponents, y
+    return dx
 
 
 def cast_blocks_to_fp8(x):
@@ -320,9 +329,17 @@ def cast_blocks_to_fp8(x):
     """
     if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f'cast_blocks_to_fp8: unsupported dtype {x.dtype}')
-    if x.is_cuda:
-        return _blocks_cast(x.contiguous(), False)[:2]
     n = x.numel()
+    if x.is_cuda:
+        x = x.contiguous()
+        codes = torch.empty_like(x, dtype=torch.uint8)
+        exponents = x.new_empty((n + BLOCK - 1) // BLOCK, dtype=torch.uint8)
+        with native.on_device(x):
+            native.check(
+                native.lib().msamp_blocks_cast(x.data_ptr(), None, codes.data_ptr(), exponents.data_ptr(), n, native.dt(x.dtype), native.raw_stream()),
+                'cast_blocks_to_fp8'
+            )
+        return codes, exponents
     rows = torch.nn.functional.pad(x.detach().float().reshape(-1), (0, -n % BLOCK)).view(-1, BLOCK)
     finite = torch.isfinite(rows)
     if n == 0:
@@ -342,7 +359,7 @@ def cast_blocks_from_fp8(codes, exponents, out_dtype):
     codes, exponents = codes.contiguous(), exponents.contiguous()
     n = codes.numel()
     if codes.is_cuda:
-        out = torch.empty(codes.shape, dtype=out_dtype, device=codes.device)
+        out = torch.empty_like(codes, dtype=out_dtype)
         with native.on_device(codes):
             native.check(
                 native.lib().msamp_blocks_uncast(

@@ -21,6 +21,7 @@
 // the device, now 44 + 107 us; 64 x 197 x 12 heads, 61 + 218 us, now 45 + 119 us.  Those kernels remain for views that a tensor map
 // cannot describe, for short rows (see short_rows) and as a cross-check (MSAMP_ATTN_IMPL=mma).
 #include <cstdlib>
+#include <initializer_list>
 #include <mutex>
 #include <unordered_map>
 
@@ -3942,9 +3943,50 @@ static int launch_bwd(const CUtensorMap (&m)[4], const TcParams& p, int n_t, int
   return MSAMP_OK;
 }
 
-MSAMP_API int msamp_attention_shared_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* lengths, int* plan,
-                                         const int64_t* strides, int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale,
-                                         int causal, void* stream_) {
+// The arguments of both passes come as one block of 64-bit fields, which a caller in Python packs several times faster than it passes
+// thirty arguments.
+struct SharedArgs {
+  int64_t batch, heads, kv_heads, seqlen, head_dim, causal;
+  double scale;
+};
+struct SharedFwdArgs {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;
+  const int* lengths;
+  int* plan;
+  SharedArgs n;
+  int64_t strides[12];    // (batch, seq, head) element strides of q, k, v, o
+};
+struct SharedBwdArgs {
+  const void *q, *k, *v, *o;
+  const float* lse;
+  const int *lengths, *plan;
+  const void* d_o;
+  void *dq, *dk, *dv;
+  float *delta, *partial;    // [batch, heads, seqlen]; see msamp_attention_shared_parts
+  SharedArgs n;
+  int64_t strides[24];    // of q, k, v, o, dO, dq, dk, dv
+};
+
+static int shared_sizes(const SharedArgs& n) {
+  for (int64_t v : {n.batch, n.heads, n.kv_heads, n.seqlen, n.head_dim})
+    MSAMP_REQUIRE(v >= 0 && v <= 0x7fffffff, "attention (shared heads): size %lld", (long long)v);
+  return MSAMP_OK;
+}
+
+MSAMP_API int msamp_attention_shared_fwd(const SharedFwdArgs* a, void* stream_) {
+  MSAMP_REQUIRE(a, "attention (shared heads): no arguments");
+  if (int e = shared_sizes(a->n)) return e;
+  const void *q = a->q, *k = a->k, *v = a->v;
+  void* o = a->o;
+  float* lse = a->lse;
+  const int* lengths = a->lengths;
+  int* plan = a->plan;
+  const int64_t* strides = a->strides;
+  const int batch = (int)a->n.batch, heads = (int)a->n.heads, kv_heads = (int)a->n.kv_heads, seqlen = (int)a->n.seqlen, head_dim = (int)a->n.head_dim;
+  const int causal = a->n.causal != 0;
+  const float scale = (float)a->n.scale;
   int rc = shared_checks(batch, heads, kv_heads, seqlen, head_dim, scale, lengths, plan, strides, 12);
   if (rc) return rc;
   MSAMP_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o), "attention (shared heads): q, k, v and o must be 16-byte aligned");
@@ -3984,10 +4026,18 @@ MSAMP_API int msamp_attention_shared_parts(int batch, int heads, int kv_heads, i
 }
 
 // partial: parts * 2 * batch * kv_heads * seqlen * head_dim floats when msamp_attention_shared_parts gives more than one part.
-MSAMP_API int msamp_attention_shared_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, void* dq,
-                                         void* dk, void* dv, float* delta, float* partial, const int* lengths, const int* plan,
-                                         const int64_t* strides, int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale,
-                                         int causal, void* stream_) {
+MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) {
+  MSAMP_REQUIRE(a, "attention (shared heads): no arguments");
+  if (int e = shared_sizes(a->n)) return e;
+  const void *q = a->q, *k = a->k, *v = a->v, *o = a->o, *d_o = a->d_o;
+  void *dq = a->dq, *dk = a->dk, *dv = a->dv;
+  const float* lse = a->lse;
+  float *delta = a->delta, *partial = a->partial;
+  const int *lengths = a->lengths, *plan = a->plan;
+  const int64_t* strides = a->strides;
+  const int batch = (int)a->n.batch, heads = (int)a->n.heads, kv_heads = (int)a->n.kv_heads, seqlen = (int)a->n.seqlen, head_dim = (int)a->n.head_dim;
+  const int causal = a->n.causal != 0;
+  const float scale = (float)a->n.scale;
   int rc = shared_checks(batch, heads, kv_heads, seqlen, head_dim, scale, lengths, plan, strides, 24);
   if (rc) return rc;
   MSAMP_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(d_o) && aligned16(dq) && aligned16(dk) && aligned16(dv),

@@ -5,6 +5,8 @@
 // The angle is taken in 64 bits, in turns, and reduced to (-1/2, 1/2] before it is rounded to 32 bits: at position 10^6 a 32-bit
 // angle is off by 0.06.  Sine and cosine belong to a token, not to a head, so a CTA computes those of its tokens once
 // (in shared memory) and takes all heads of both tensors through them.  Bound by memory: one read and one write of every head.
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace {
@@ -113,12 +115,30 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotParams p) {
 
 }    // namespace
 
-// x0 [batch, seq, heads0, dim] -> y0 and x1 [batch, seq, heads1, dim] -> y1 (heads1 may be 0).  strides: (batch, seq, head) element strides
-// of x0, y0, x1, y1.  y may be x itself with the same strides; otherwise the two must not overlap.  p_sb, p_ss: strides of the positions.
-MSAMP_API int msamp_rotary(const void* x0, void* y0, const void* x1, void* y1, const int64_t* strides, const double* freqs, const void* positions,
-                           int pos64, int64_t p_sb, int64_t p_ss, int batch, int seq, int heads0, int heads1, int dim, int part, int interleaved,
-                           int inverse, int dtype, void* stream_) {
-  MSAMP_REQUIRE(batch >= 0 && seq >= 0 && heads0 >= 0 && heads1 >= 0, "rotary: negative size");
+// x0 [batch, seq, heads0, dim] -> y0 and x1 [batch, seq, heads1, dim] -> y1 (heads1 may be 0).  y may be x itself with the same strides;
+// otherwise the two must not overlap.  The arguments come as one block of 64-bit fields, which a caller in Python packs several times faster
+// than it passes thirty arguments.
+struct RotaryArgs {
+  const void* x0;
+  void* y0;
+  const void* x1;
+  void* y1;
+  int64_t strides[12];    // (batch, seq, head) element strides of x0, y0, x1, y1
+  const double* freqs;
+  const void* positions;
+  int64_t pos64, p_sb, p_ss;    // positions are int64 (else int32); their strides
+  int64_t batch, seq, heads0, heads1, dim, part, interleaved, inverse, dtype;
+};
+MSAMP_API int msamp_rotary(const RotaryArgs* a, void* stream_) {
+  MSAMP_REQUIRE(a, "rotary: no arguments");
+  const void *x0 = a->x0, *x1 = a->x1;
+  void *y0 = a->y0, *y1 = a->y1;
+  const int64_t* strides = a->strides;
+  const double* freqs = a->freqs;
+  for (int64_t v : {a->batch, a->seq, a->heads0, a->heads1, a->dim, a->part}) MSAMP_REQUIRE(v >= 0 && v <= 0x7fffffff, "rotary: size %lld", (long long)v);
+  const int batch = (int)a->batch, seq = (int)a->seq, heads0 = (int)a->heads0, heads1 = (int)a->heads1, dim = (int)a->dim, part = (int)a->part;
+  const int dtype = (int)a->dtype;
+  const bool interleaved = a->interleaved != 0, inverse = a->inverse != 0;
   MSAMP_REQUIRE(part >= 2 && part % 2 == 0 && part <= dim && part <= kMaxPart, "rotary: part %d of a head of %d (even, at most %d)", part, dim, kMaxPart);
   MSAMP_REQUIRE(freqs, "rotary: no frequencies");
   if (batch == 0 || seq == 0 || heads0 + heads1 == 0) return MSAMP_OK;
@@ -140,7 +160,7 @@ MSAMP_API int msamp_rotary(const void* x0, void* y0, const void* x1, void* y1, c
     }
     p.t[i] = RotTensor{px[i], py[i], s[0], s[1], s[2], s[3], s[4], s[5], heads[i]};
   }
-  p.freqs = freqs; p.positions = positions; p.pos64 = pos64; p.p_sb = p_sb; p.p_ss = p_ss;
+  p.freqs = freqs; p.positions = a->positions; p.pos64 = a->pos64 != 0; p.p_sb = a->p_sb; p.p_ss = a->p_ss;
   p.batch = batch; p.seq = seq; p.dim = dim; p.part = part; p.sign = inverse ? -1.0f : 1.0f;
   const int half = part / 2;
   p.per_cta = half >= kThreads ? 1 : kThreads / half;

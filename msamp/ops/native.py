@@ -40,9 +40,9 @@ _ARGTYPES = {
     'msamp_attention_tc_fwd': [_P] * 6 + [_I] * 4 + [_F, _I, _P],
     'msamp_attention_bwd': [_P] * 11 + [_I] * 4 + [_F, _I, _P],
     'msamp_attention_tc_bwd': [_P] * 11 + [_I] * 4 + [_F, _I, _P],
-    'msamp_attention_shared_fwd': [_P] * 8 + [_I] * 5 + [_F, _I, _P],
-    'msamp_attention_shared_bwd': [_P] * 14 + [_I] * 5 + [_F, _I, _P],
-    'msamp_rotary': [_P] * 7 + [_I, _L, _L] + [_I] * 9 + [_P],
+    'msamp_attention_shared_fwd': [_P, _P],
+    'msamp_attention_shared_bwd': [_P, _P],
+    'msamp_rotary': [_P, _P],
     'msamp_blocks_cast': [_P] * 4 + [_L, _I, _P],
     'msamp_blocks_uncast': [_P] * 4 + [_L, _I, _P],
 }

@@ -6,6 +6,7 @@ torch math (the oracle the GPU tests compare against).
 import ctypes
 import math
 import os
+import struct
 
 import torch
 import torch.nn.functional as F
@@ -186,16 +187,19 @@ class _GeluKeepFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x):
         if x.is_cuda:
-            codes, exponents, y = _c._blocks_cast(x.contiguous(), True)
-        else:
-            codes, exponents = _c.cast_blocks_to_fp8(x)
-            y = F.gelu(x.float(), approximate='tanh').to(x.dtype)
-        ctx.save_for_backward(codes, exponents)
-        return y
+            kept, y = _c._gelu_keep(x.contiguous())
+            ctx.save_for_backward(kept)
+            return y
+        ctx.save_for_backward(*_c.cast_blocks_to_fp8(x))
+        return F.gelu(x.float(), approximate='tanh').to(x.dtype)
 
     @staticmethod
     def backward(ctx, dy):
-        return gelu_bwd_blocks(*ctx.saved_tensors, dy)
+        kept, *rest = ctx.saved_tensors
+        if rest:
+            return gelu_bwd_blocks(kept, rest[0], dy)
+        dy = dy.contiguous()
+        return _c._gelu_keep_bwd(kept, dy)
 
 
 def gelu_bwd_blocks(codes, exponents, dy):
@@ -392,48 +396,72 @@ def attention_qkv(qkv, causal=True, scale=None):
 
 
 # Attention whose query heads share key / value heads, on rows that may end early.  ``q [B, S, heads, d]``, ``k`` and ``v [B, S, kv_heads, d]``
-# as strided views, ``lengths`` int32 ``[B]`` or None.
+# as strided views, ``lengths`` int32 ``[B]`` or None.  The argument blocks of the native entry points: addresses, sizes and scale, strides.
+_pack_fwd, _pack_bwd = struct.Struct('7q').pack, struct.Struct('12q').pack
+_pack_one, _pack_sizes, _pack_st = struct.Struct('q').pack, struct.Struct('6qd').pack, [struct.Struct(f'{3 * n}q').pack for n in range(9)]
+
+
 def _map_strides(t):
     """(batch, seq, head) element strides for a tensor map; the stride of an axis of extent 1 is never used and may be any number."""
-    return [s if n > 1 else t.shape[3] for s, n in zip(t.stride()[:3], t.shape[:3])]
+    a, b, c, _ = t.stride()
+    if (a | b | c) & 7 == 0:
+        return a, b, c
+    return tuple(s if n > 1 else t.shape[3] for s, n in zip((a, b, c), t.shape))
+
+
+def _dense_strides(S, n, d):
+    """The same of a contiguous ``[B, S, n, d]`` tensor."""
+    return S * n * d, n * d, d
 
 
 def _mappable(t):
     """``t``, or a copy of it where it repeats a batch, position or head (a tensor map has no zero stride)."""
-    return t.contiguous() if any(s == 0 and n > 1 for s, n in zip(t.stride()[:3], t.shape[:3])) else t
+    a, b, c, _ = t.stride()
+    if a and b and c:
+        return t
+    return t.contiguous() if any(s == 0 and n > 1 for s, n in zip((a, b, c), t.shape)) else t
 
 
 def _shared_fwd(q, k, v, causal, scale, lengths):
+    """``(o, lse, plan, fields)``; the last are sizes and strides of q, k, v and o, which the backward pass has too."""
     B, S, nh, d = q.shape
-    o = torch.empty((B, S, nh, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, nh, S), dtype=torch.float32, device=q.device)
+    nkv = k.shape[2]
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((B, nh, S), dtype=torch.float32)
     # with lengths: the tiles that are not padding, listed by the forward pass for both passes
-    plan = torch.empty(1 + B * ((S + 127) // 128), dtype=torch.int32, device=q.device) if lengths is not None else None
-    st = _map_strides(q) + _map_strides(k) + _map_strides(v) + _map_strides(o) + [0] * 12
+    plan = q.new_empty(1 + B * ((S + 127) // 128), dtype=torch.int32) if lengths is not None else None
+    fields = _pack_sizes(B, nh, nkv, S, d, causal, scale) + _pack_st[4](*_map_strides(q), *_map_strides(k), *_map_strides(v),
+                                                                        *_dense_strides(S, nh, d))
     with native.on_device(q):
         native.check(
             native.lib().msamp_attention_shared_fwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), native.addr(lengths), native.addr(plan), _i64x24(*st), B,
-                nh, k.shape[2], S, d, scale, int(causal), native.raw_stream()
+                _pack_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+                          0 if plan is None else plan.data_ptr()) + fields, native.raw_stream()
             ), 'attention_fwd'
         )
-    return o, lse, plan
+    return o, lse, plan, fields
 
 
-def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths, plan):
-    B, S, nh, d = q.shape
-    nkv = k.shape[2]
-    o, d_o = _rows16(_mappable(o)), _rows16(_mappable(d_o))
-    st = [x for t in (q, k, v, o, d_o, dq, dk, dv) for x in _map_strides(t)]
+def _shared_workspace(B, nh, nkv, S, d):
+    """Floats of the backward pass's workspace, and of its first part: delta, then the partial sums of dK and dV where there are several."""
+    parts = native.lib().msamp_attention_shared_parts(B, nh, nkv, S)
+    first = (B * nh * S + 3) // 4 * 4
+    return first + (parts * 2 * B * nkv * S * d if parts > 1 else 0), first
+
+
+def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, work, grad_strides):
+    """Gradients into ``dq``, ``dk`` and ``dv``, whose packed strides are ``grad_strides``."""
+    if not d_o.is_contiguous() or d_o.data_ptr() % 16:
+        d_o = _rows16(_mappable(d_o))
+    total, first = work
+    space = q.new_empty(total, dtype=torch.float32)
+    at = space.data_ptr()
     with native.on_device(q):
-        parts = native.lib().msamp_attention_shared_parts(B, nh, nkv, S)
-        delta = torch.empty((B, nh, S), dtype=torch.float32, device=q.device)
-        partial = torch.empty(parts * 2 * B * nkv * S * d, dtype=torch.float32, device=q.device) if parts > 1 else None
         native.check(
             native.lib().msamp_attention_shared_bwd(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                delta.data_ptr(), native.addr(partial), native.addr(lengths), native.addr(plan), _i64x24(*st), B, nh, nkv, S, d, scale,
-                int(causal), native.raw_stream()
+                _pack_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+                          0 if plan is None else plan.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), at) +
+                _pack_one(at + 4 * first) + fields + _pack_st[1](*_map_strides(d_o)) + grad_strides, native.raw_stream()
             ), 'attention_bwd'
         )
 
@@ -441,23 +469,39 @@ def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths, plan):
 class _AttentionSharedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, causal, scale, grad_layout, lengths):
-        o, lse, plan = _shared_fwd(q, k, v, causal, scale, lengths)
+        o, lse, plan, ctx.fields = _shared_fwd(q, k, v, causal, scale, lengths)
         ctx.save_for_backward(q, k, v, o, lse, lengths, plan)
-        ctx.causal, ctx.scale, ctx.grad_layout = causal, scale, grad_layout
+        B, S, nh, d = q.shape
+        nkv = k.shape[2]
+        ctx.packed = grad_layout == 'packed'
+        if ctx.packed:
+            ctx.grad_strides = _pack_st[3](*_dense_strides(S, nh + 2 * nkv, d) * 3)
+        else:
+            ctx.grad_strides = _pack_st[3](*_dense_strides(S, nh, d), *_dense_strides(S, nkv, d) * 2)
+        ctx.work = _shared_workspace(B, nh, nkv, S, d)
+        ctx.args, ctx.places = (causal, scale), _places(q, k, v, o)
         return o
 
     @staticmethod
     def backward(ctx, d_o):
         q, k, v, o, lse, lengths, plan = ctx.saved_tensors
-        q, k, v = (_rows16(t) for t in (q, k, v))    # saved tensors may come back with other strides
-        B, S, nh, d = q.shape
-        if ctx.grad_layout == 'packed':
-            buf = torch.empty((B, S, nh + 2 * k.shape[2], d), dtype=q.dtype, device=q.device)
-            dq, dk, dv = buf.split([nh, k.shape[2], k.shape[2]], dim=2)
+        fields = ctx.fields
+        if _places(q, k, v, o) != ctx.places:    # saved tensors may come back with other strides (saved-tensor hooks)
+            q, k, v, o = (_rows16(_mappable(t)) for t in (q, k, v, o))
+            B, S, nh, d = q.shape
+            fields = _pack_sizes(B, nh, k.shape[2], S, d, *ctx.args) + _pack_st[4](*(s for t in (q, k, v, o) for s in _map_strides(t)))
+        if ctx.packed:
+            B, S, nh, d = q.shape
+            nkv = k.shape[2]
+            dq, dk, dv = q.new_empty((B, S, nh + 2 * nkv, d)).split([nh, nkv, nkv], dim=2)
         else:
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, ctx.causal, ctx.scale, lengths, plan)
+            dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, ctx.work, ctx.grad_strides)
         return dq, dk, dv, None, None, None, None
+
+
+def _places(*ts):
+    return tuple((t.stride(), t.data_ptr() & 15) for t in ts)
 
 
 def _attention_plain(q, k, v, causal, scale, lengths):
@@ -491,7 +535,7 @@ def attention_shared_fwd_raw(q, k, v, causal=True, scale=None, lengths=None):
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if _use_native(q) and q.numel():
         q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
-        return _shared_fwd(q, k, v, causal, scale, lengths)
+        return _shared_fwd(q, k, v, bool(causal), float(scale), lengths)[:3]
     _check_shared(q, k, v, scale, lengths)
     with torch.no_grad():
         return _attention_plain(q, k, v, causal, scale, lengths), None, None
@@ -502,7 +546,11 @@ def attention_shared_bwd_raw(q, k, v, o, lse, plan, d_o, dq, dk, dv, causal=True
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if _use_native(q) and q.numel():
         q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, causal, scale, lengths, plan)
+        o = _rows16(_mappable(o))
+        B, S, nh, d = q.shape
+        fields = _pack_sizes(B, nh, k.shape[2], S, d, bool(causal), float(scale)) + _pack_st[4](*(x for t in (q, k, v, o) for x in _map_strides(t)))
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, _shared_workspace(B, nh, k.shape[2], S, d),
+                    _pack_st[3](*(x for t in (dq, dk, dv) for x in _map_strides(t))))
         return
     with torch.enable_grad():
         leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
@@ -512,30 +560,33 @@ def attention_shared_bwd_raw(q, k, v, o, lse, plan, d_o, dq, dk, dv, causal=True
 
 
 def _check_shared(q, k, v, scale, lengths):
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
-        raise ValueError(f'attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together')
-    if k.shape[2] == 0 or q.shape[2] % k.shape[2]:
-        raise ValueError(f'attention: {q.shape[2]} query heads do not share {k.shape[2]} key/value heads evenly')
-    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+    shape, kv = q.shape, k.shape
+    if len(shape) != 4 or len(kv) != 4 or v.shape != kv or kv[:2] != shape[:2] or kv[3] != shape[3]:
+        raise ValueError(f'attention: q {tuple(shape)}, k {tuple(kv)} and v {tuple(v.shape)} do not fit together')
+    if kv[2] == 0 or shape[2] % kv[2]:
+        raise ValueError(f'attention: {shape[2]} query heads do not share {kv[2]} key/value heads evenly')
+    dtype, device = q.dtype, q.device
+    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
         raise ValueError('attention: q, k and v must have one dtype and one device')
     if not 0.0 < scale < 3e38:
         raise ValueError(f'attention: scale must be positive (got {scale})')
     if lengths is not None:
-        if tuple(lengths.shape) != (q.shape[0], ) or lengths.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f'attention: lengths must be an int32 or int64 tensor [{q.shape[0]}] (got {lengths.dtype} {tuple(lengths.shape)})')
-        if lengths.device != q.device:
+        if lengths.shape != shape[:1] or lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f'attention: lengths must be an int32 or int64 tensor [{shape[0]}] (got {lengths.dtype} {tuple(lengths.shape)})')
+        if lengths.device != device:
             raise ValueError('attention: lengths must be on the device of q')
 
 
 def _shared_operands(q, k, v, scale, lengths):
     """Checked operands of the CUDA kernels: mappable views, lengths in int32."""
     _check_shared(q, k, v, scale, lengths)
-    d = q.shape[-1]
+    d = q.shape[3]
     if q.dtype != torch.bfloat16 or d not in (64, 128):
         raise RuntimeError(f'attention: CUDA kernel supports bf16 with head_dim 64/128 (got {q.dtype}, {d})')
-    q, k, v = (_mappable(t) for t in (q, k, v))
+    q, k, v = _mappable(q), _mappable(k), _mappable(v)
     for t in (q, k, v):
-        if t.stride(3) != 1 or any(s % 8 for s in _map_strides(t)) or t.data_ptr() % 16:
+        a, b, c = _map_strides(t)
+        if t.stride(3) != 1 or (a | b | c) & 7 or t.data_ptr() & 15:
             raise RuntimeError('attention: operands must have unit inner stride and 16-byte aligned rows')
     if lengths is not None:
         lengths = lengths.to(torch.int32).contiguous()
@@ -543,11 +594,13 @@ def _shared_operands(q, k, v, scale, lengths):
 
 
 def _attention_shared(q, k, v, causal, scale, grad_layout, lengths):
-    if not _use_native(q) or q.numel() == 0:
+    if not q.is_cuda or q.numel() == 0:
         _check_shared(q, k, v, scale, lengths)
         return _attention_plain(q, k, v, causal, scale, lengths)
     q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
-    return _AttentionSharedFn.apply(q, k, v, bool(causal), float(scale), grad_layout, lengths)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _AttentionSharedFn.apply(q, k, v, bool(causal), float(scale), grad_layout, lengths)
+    return _shared_fwd(q, k, v, bool(causal), float(scale), lengths)[0]
 
 
 def attention(q, k, v, causal=True, scale=None, grad_layout='separate', lengths=None):

@@ -3,14 +3,12 @@
 CUDA tensors use the kernel in ``csrc/rotary.cu``; CPU tensors use plain torch math with the same 64-bit angles (the oracle of
 the GPU tests).
 """
-import ctypes
 import math
+import struct
 
 import torch
 
 from msamp.ops import native
-
-_i64x12 = ctypes.c_int64 * 12
 
 
 def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, trained=None, fast=32.0, slow=1.0, device=None):
@@ -46,30 +44,59 @@ def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, trained=None
     return f.to(device) if device is not None else f
 
 
-def _check(x, name, freqs, positions):
-    if x.dim() != 4:
-        raise ValueError(f'rotary: {name} must be [batch, seq, heads, head_dim] (got {tuple(x.shape)})')
-    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-        raise TypeError(f'rotary: unsupported dtype {x.dtype}')
-    if 2 * freqs.numel() > x.shape[3]:
-        raise ValueError(f'rotary: {freqs.numel()} pairs do not fit a head of {x.shape[3]}')
-    if freqs.device != x.device or (positions is not None and positions.device != x.device):
-        raise ValueError(f'rotary: {name}, frequencies and positions must be on one device')
+_TYPES = {torch.float32: native.DT_F32, torch.float16: native.DT_F16, torch.bfloat16: native.DT_BF16}
 
 
 def _check_all(q, k, freqs, positions):
+    if q.dim() != 4:
+        raise ValueError(f'rotary: q must be [batch, seq, heads, head_dim] (got {tuple(q.shape)})')
+    batch, seq, _, dim = q.shape
+    if q.dtype not in _TYPES:
+        raise TypeError(f'rotary: unsupported dtype {q.dtype}')
     if freqs.dtype != torch.float64 or freqs.dim() != 1 or not 1 <= freqs.numel() <= 512:
         raise ValueError(f'rotary: frequencies are a float64 vector of 1 to 512 pairs (got {freqs.dtype}, {tuple(freqs.shape)})')
-    _check(q, 'q', freqs, positions)
+    if 2 * freqs.numel() > dim:
+        raise ValueError(f'rotary: {freqs.numel()} pairs do not fit a head of {dim}')
+    if freqs.device != q.device:
+        raise ValueError('rotary: q and the frequencies must be on one device')
     if k is not None:
-        _check(k, 'k', freqs, positions)
-        if k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3] or k.dtype != q.dtype or k.device != q.device:
+        if k.dim() != 4 or k.shape[:2] != (batch, seq) or k.shape[3] != dim or k.dtype != q.dtype or k.device != q.device:
             raise ValueError(f'rotary: q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in more than their heads')
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f'rotary: positions must be int32 or int64 (got {positions.dtype})')
-        if tuple(positions.shape) not in ((q.shape[1], ), tuple(q.shape[:2])):
+        if tuple(positions.shape) not in ((seq, ), (batch, seq)):
             raise ValueError(f'rotary: positions {tuple(positions.shape)} are neither [seq] nor [batch, seq] of {tuple(q.shape)}')
+        if positions.device != q.device:
+            raise ValueError('rotary: q and the positions must be on one device')
+
+
+# The argument block of the native entry point: addresses and strides of the tensors, then what a call and its gradient share, then
+# inverse and dtype.
+_pack_tensors, _pack_common, _pack_end = struct.Struct('16q').pack, struct.Struct('12q').pack, struct.Struct('2q').pack
+
+
+def _common(freqs, positions, batch, seq, heads0, heads1, dim, interleaved):
+    """The fields that the rotation and its gradient share; ``freqs`` is contiguous."""
+    part = 2 * freqs.numel()
+    if positions is None:
+        return _pack_common(freqs.data_ptr(), 0, 0, 0, 0, batch, seq, heads0, heads1, dim, part, interleaved)
+    st = positions.stride()
+    return _pack_common(freqs.data_ptr(), positions.data_ptr(), positions.dtype == torch.int64, st[0] if len(st) == 2 else 0, st[-1], batch, seq,
+                        heads0, heads1, dim, part, interleaved)
+
+
+def _turn(x0, y0, x1, y1, common, inverse):
+    """One launch on one or two tensors whose inner strides are one."""
+    a, b = x0.stride(), y0.stride()
+    if x1 is None:
+        block = _pack_tensors(x0.data_ptr(), y0.data_ptr(), 0, 0, a[0], a[1], a[2], b[0], b[1], b[2], 0, 0, 0, 0, 0, 0)
+    else:
+        c, d = x1.stride(), y1.stride()
+        block = _pack_tensors(x0.data_ptr(), y0.data_ptr(), x1.data_ptr(), y1.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], c[0], c[1], c[2],
+                              d[0], d[1], d[2])
+    with native.on_device(x0):
+        native.check(native.lib().msamp_rotary(block + common + _pack_end(inverse, _TYPES[x0.dtype]), native.raw_stream()), 'rotary')
 
 
 def rotary_raw(xs, ys, freqs, positions, interleaved, inverse):
@@ -78,32 +105,14 @@ def rotary_raw(xs, ys, freqs, positions, interleaved, inverse):
     Inner strides are one; the others are free.  ``inverse`` turns back, which is also the gradient.
     """
     x = xs[0]
-    batch, seq, _, dim = x.shape
     if not x.is_cuda:
         for src, dst in zip(xs, ys):
             dst.copy_(_emulated(src, freqs, positions, interleaved, inverse))
         return
-    st, ptrs, heads = [], [], []
-    for src, dst in zip(xs, ys):
-        st += [*src.stride()[:3], *dst.stride()[:3]]
-        ptrs += [src.data_ptr(), dst.data_ptr()]
-        heads.append(src.shape[2])
-    if len(heads) == 1:
-        ptrs += [None, None]
-        heads.append(0)
     freqs = freqs.contiguous()
-    p_sb = p_ss = pos64 = 0
-    if positions is not None:
-        pos64 = int(positions.dtype == torch.int64)
-        p_ss = positions.stride(-1)
-        p_sb = positions.stride(0) if positions.dim() == 2 else 0
-    with native.on_device(x):
-        native.check(
-            native.lib().msamp_rotary(
-                *ptrs, _i64x12(*st), freqs.data_ptr(), native.addr(positions), pos64, p_sb, p_ss, batch, seq, *heads, dim, 2 * freqs.numel(),
-                int(interleaved), int(inverse), native.dt(x.dtype), native.raw_stream()
-            ), 'rotary'
-        )
+    two = len(xs) > 1
+    common = _common(freqs, positions, x.shape[0], x.shape[1], x.shape[2], xs[1].shape[2] if two else 0, x.shape[3], interleaved)
+    _turn(x, ys[0], xs[1] if two else None, ys[1] if two else None, common, inverse)
 
 
 def _emulated(x, freqs, positions, interleaved, inverse):
@@ -124,27 +133,53 @@ def _unit_inner(t):
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
+def _like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _forward(q, k, freqs, positions, interleaved):
+    """``(q', k' or None, fields)``; the last are what the gradient needs again on CUDA."""
+    if not q.is_cuda:
+        return (_emulated(q, freqs, positions, interleaved, False).contiguous(),
+                None if k is None else _emulated(k, freqs, positions, interleaved, False).contiguous(), None)
+    q = _unit_inner(q)
+    batch, seq, heads, dim = q.shape
+    if k is None:
+        common = _common(freqs, positions, batch, seq, heads, 0, dim, interleaved)
+        y = _like(q)
+        _turn(q, y, None, None, common, 0)
+        return y, None, common
+    k = _unit_inner(k)
+    common = _common(freqs, positions, batch, seq, heads, k.shape[2], dim, interleaved)
+    yq, yk = _like(q), _like(k)
+    _turn(q, yq, k, yk, common, 0)
+    return yq, yk, common
+
+
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, freqs, positions, interleaved):
         ctx.set_materialize_grads(False)
-        xs = [_unit_inner(t) for t in ((q, ) if k is None else (q, k))]
-        ys = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
-        rotary_raw(xs, ys, freqs, positions, interleaved, False)
+        yq, yk, ctx.common = _forward(q, k, freqs, positions, interleaved)
         ctx.save_for_backward(freqs, positions)
-        ctx.interleaved = interleaved
-        return tuple(ys)
+        ctx.interleaved, ctx.freqs_at, ctx.positions_at = interleaved, freqs.data_ptr(), 0 if positions is None else positions.data_ptr()
+        return yq if k is None else (yq, yk)
 
     @staticmethod
-    def backward(ctx, *grads):
+    def backward(ctx, gq, gk=None):
         freqs, positions = ctx.saved_tensors
-        xs = [_unit_inner(g) for g in grads if g is not None]
-        ys = [torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in xs]
-        if xs:
-            rotary_raw(xs, ys, freqs, positions, ctx.interleaved, True)
-        back = iter(ys)
-        out = [None if g is None else next(back) for g in grads]
-        return out[0], (out[1] if len(out) > 1 else None), None, None, None
+        if gq is not None and gk is not None and gq.is_cuda and gq.is_contiguous() and gk.is_contiguous() and freqs.data_ptr() == ctx.freqs_at and (
+                positions is None or positions.data_ptr() == ctx.positions_at):
+            # as a rule: both gradients, in the layout of the outputs, with the fields of the forward call
+            dq, dk = torch.empty_like(gq), torch.empty_like(gk)
+            _turn(gq, dq, gk, dk, ctx.common, 1)
+            return dq, dk, None, None, None
+        given = [_unit_inner(g) for g in (gq, gk) if g is not None]
+        out = [_like(g) for g in given]
+        if given:
+            rotary_raw(given, out, freqs, positions, ctx.interleaved, True)
+        back = iter(out)
+        return (None if gq is None else next(back)), (None if gk is None else next(back)), None, None, None
 
 
 def rotary(q, k, freqs, positions=None, interleaved=False):
@@ -156,5 +191,8 @@ def rotary(q, k, freqs, positions=None, interleaved=False):
     bf16; inputs may be strided views.  Returns new contiguous tensors, ``(q', k')`` or ``q'`` alone when ``k`` is None.
     """
     _check_all(q, k, freqs, positions)
-    out = _RotaryFn.apply(q, k, freqs, positions, bool(interleaved))
-    return out if k is not None else out[0]
+    freqs = freqs.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryFn.apply(q, k, freqs, positions, bool(interleaved))
+    yq, yk, _ = _forward(q, k, freqs, positions, bool(interleaved))
+    return yq if k is None else (yq, yk)

@@ -274,15 +274,16 @@ def test_refusals_on_cuda():
 @pytest.mark.skipif(not native.available(), reason='kernel library not built')
 def test_entry_points_refuse():
     """No launch and no driver call: every call is refused by its arguments."""
-    import ctypes
+    import struct
     lib, at = native.lib(), 1 << 20
     good = [768, 256, 64] * 8
 
-    def fwd(ptrs=None, strides=good, sizes=(2, 4, 2, 3, 64), scale=0.125, lengths=None):
-        return lib.msamp_attention_shared_fwd(*(ptrs or [at] * 5), lengths, None, (ctypes.c_int64 * 24)(*strides), *sizes, scale, 1, None)
+    def fwd(ptrs=None, strides=good, sizes=(2, 4, 2, 3, 64), scale=0.125, lengths=0):
+        return lib.msamp_attention_shared_fwd(struct.pack('7q6qd12q', *(ptrs or [at] * 5), lengths, 0, *sizes, 1, scale, *strides[:12]), None)
 
-    def bwd(ptrs=None, strides=good, sizes=(2, 4, 2, 3, 64), scale=0.125, partial=at, lengths=None):
-        return lib.msamp_attention_shared_bwd(*(ptrs or [at] * 10), partial, lengths, None, (ctypes.c_int64 * 24)(*strides), *sizes, scale, 1, None)
+    def bwd(ptrs=None, strides=good, sizes=(2, 4, 2, 3, 64), scale=0.125, partial=at, lengths=0):
+        p = ptrs or [at] * 9
+        return lib.msamp_attention_shared_bwd(struct.pack('13q6qd24q', *p[:5], lengths, 0, *p[5:], at, partial, *sizes, 1, scale, *strides), None)
 
     odd = good[:4] + [260] + good[5:]
     for call in (fwd, bwd):
@@ -290,11 +291,13 @@ def test_entry_points_refuse():
         assert call(sizes=(0, 4, 2, 3, 64)) == 1 and call(sizes=(2, 4, 2, 0, 64)) == 1 and call(sizes=(2, 4, 0, 3, 64)) == 1
         assert call(lengths=at) == 1    # without a plan
         assert call(scale=0.0) == 1 and call(scale=-1.0) == 1 and call(scale=float('nan')) == 1
-        assert call(sizes=(1 << 14, 1 << 14, 1, 1 << 10, 64)) == 1
+        assert call(sizes=(1 << 14, 1 << 14, 1, 1 << 10, 64)) == 1 and call(sizes=(2, 4, 2, 1 << 40, 64)) == 1 and call(sizes=(-2, 4, 2, 3, 64)) == 1
+    assert bwd(partial=0) == 1    # two parts of query heads and nowhere to leave them
+    assert lib.msamp_attention_shared_fwd(None, None) == 1 and lib.msamp_attention_shared_bwd(None, None) == 1
     for i in (0, 1, 2, 3):
         assert fwd([at + 8 * (j == i) for j in range(5)]) == 1
     for i in (0, 1, 2, 3, 5, 6, 7, 8):
-        assert bwd([at + 8 * (j == i) for j in range(10)]) == 1
+        assert bwd([at + 8 * (j == i) for j in range(9)]) == 1
 
 
 @pytest.mark.gpu

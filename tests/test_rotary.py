@@ -180,18 +180,17 @@ def test_refusals():
 @pytest.mark.skipif(not native.available(), reason='kernel library not built')
 def test_entry_point_refuses():
     """No launch: every call is refused by its arguments."""
-    import ctypes
+    import struct
     lib, at = native.lib(), 1 << 20
-    st = (ctypes.c_int64 * 12)(*([24, 8, 8] * 4))
-    other = (ctypes.c_int64 * 12)(*([24, 8, 8] + [48, 8, 8] + [24, 8, 8] * 2))
+    st, other = [24, 8, 8] * 4, [24, 8, 8] + [48, 8, 8] + [24, 8, 8] * 2
 
-    def call(x=at, y=at, strides=st, freqs=at, batch=1, part=8, dim=8):
-        return lib.msamp_rotary(x, y, None, None, strides, freqs, None, 0, 0, 0, batch, 3, 1, 0, dim, part, 0, 0, 0, None)
+    def call(x=at, y=at, strides=st, freqs=at, batch=1, part=8, dim=8, heads=1, dtype=0):
+        return lib.msamp_rotary(struct.pack('30q', x, y, 0, 0, *strides, freqs, 0, 0, 0, 0, batch, 3, heads, 0, dim, part, 0, 0, dtype), None)
 
-    for kw in (dict(x=None), dict(y=None), dict(freqs=None), dict(batch=-1), dict(part=7), dict(part=10), dict(part=0), dict(strides=other),
-               dict(part=2048, dim=2048)):
+    for kw in (dict(x=0), dict(y=0), dict(freqs=0), dict(batch=-1), dict(part=7), dict(part=10), dict(part=0), dict(strides=other),
+               dict(part=2048, dim=2048), dict(heads=-1), dict(batch=1 << 40)):
         assert call(**kw) == 1, kw
-    assert call(batch=0) == 0
+    assert call(dtype=5) == 2 and call(batch=0) == 0 and lib.msamp_rotary(None, None) == 1
 
 
 @pytest.mark.gpu
