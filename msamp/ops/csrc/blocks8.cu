@@ -68,55 +68,125 @@ __device__ __forceinline__ void cast_block_by_lane(const T* x, T* y, uint8_t* co
   if (lane == 0) exps[blk] = (uint8_t)(127 - k);
 }
 
-// VEC: every pointer aligned for whole vectors of 16 bytes of T; V elements a thread, L = 32 / V lanes a block.
+// A 16-byte vector of T: V elements, as 32-bit words of one or two.
+template <typename T>
+struct Vec {
+  static constexpr int V = 16 / sizeof(T), L = kBlock / V;    // elements of a vector, lanes of a block
+};
+// The two elements of a word of 16-bit T
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&t);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  __half2 t = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&t);
+}
+template <typename T>
+__device__ __forceinline__ void unpack(const Bytes16& raw, float (&v)[Vec<T>::V]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(raw.w[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack2(raw.w[j], T());
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ Bytes16 pack(const float (&v)[Vec<T>::V]) {
+  Bytes16 o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) o.w[j] = __float_as_uint(v[j]);
+    else                          o.w[j] = pack2(v[2 * j], v[2 * j + 1], T());
+  }
+  return o;
+}
+// Largest |x| of a vector as bits of fp32, from packed integer maxima (|x| as bits is monotone, with infinities and NaN on top)
+template <typename T>
+__device__ __forceinline__ uint32_t vector_amax(const Bytes16& raw) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (sizeof(T) == 4) m = max(m, raw.w[j] & 0x7fffffffu);
+    else                m = __vmaxu2(m, raw.w[j] & 0x7fff7fffu);
+  }
+  if constexpr (sizeof(T) == 4) {
+    return m;
+  } else {
+    m = max(m >> 16, m & 0xffffu);
+    return __float_as_uint(unpack2(m, T()).x);
+  }
+}
+
+// Bound by memory.  VEC: every pointer aligned for whole vectors; two vectors a thread and step are in flight, L lanes find the maximum of a
+// block with log2(L) shuffles.  A warp that sees an infinity or a NaN (its maxima are on top of all numbers) goes over its elements again.
 template <typename T, bool GELU, bool VEC>
 __global__ void __launch_bounds__(kThreads) blocks_cast_kernel(const T* __restrict__ x, T* __restrict__ y, uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ exps, int64_t n) {
-  const int64_t tid = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t threads = (int64_t)gridDim.x * kThreads;
   const int64_t full = VEC ? n / kBlock : 0;    // blocks taken by vectors
-  if (VEC) {
-    constexpr int V = 16 / sizeof(T), L = kBlock / V;
+  if constexpr (VEC) {
+    constexpr int V = Vec<T>::V, L = Vec<T>::L, U = 2;
     const int64_t nv = full * L;
-    const int64_t top = (nv + 31) / 32 * 32;    // whole warps go round, for the shuffles
-    for (int64_t i = tid; i < top; i += threads) {
-      Bytes16 raw = {};
-      if (i < nv) raw = reinterpret_cast<const Bytes16*>(x)[i];
-      const T* e = reinterpret_cast<const T*>(&raw);
-      float v[V];
-      uint32_t a = 0;
+    for (int64_t i0 = (int64_t)blockIdx.x * (kThreads * U) + threadIdx.x; i0 - threadIdx.x < nv; i0 += (int64_t)gridDim.x * (kThreads * U)) {
+      Bytes16 raw[U];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        v[j] = to_f32<T>(e[j]);
-        a = max(a, finite_bits(v[j]));
-      }
+      for (int u = 0; u < U; ++u) raw[u] = i0 + u * kThreads < nv ? reinterpret_cast<const Bytes16*>(x)[i0 + u * kThreads] : Bytes16{};
 #pragma unroll
-      for (int o = 1; o < L; o <<= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-      if (i >= nv) continue;
-      const int k = block_shift(a);
-      const float s = __uint_as_float((uint32_t)(k + 127) << 23);
-      uint32_t c[V / 4];
+      for (int u = 0; u < U; ++u) {
+        const int64_t i = i0 + u * kThreads;
+        float v[V];
+        unpack<T>(raw[u], v);
+        uint32_t a = vector_amax<T>(raw[u]);
+        float w[V];    // what is coded
 #pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        const uint32_t lo = f32x2_to_fp8x2<FMT_E4M3>(mul_keep(inf_to_nan(v[j]), s), mul_keep(inf_to_nan(v[j + 1]), s));
-        const uint32_t hi = f32x2_to_fp8x2<FMT_E4M3>(mul_keep(inf_to_nan(v[j + 2]), s), mul_keep(inf_to_nan(v[j + 3]), s));
-        c[j / 4] = lo | hi << 16;
-      }
-      if (V == 8) reinterpret_cast<uint2*>(codes)[i] = make_uint2(c[0], c[V / 4 - 1]);
-      else        reinterpret_cast<uint32_t*>(codes)[i] = c[0];
-      if (i % L == 0) exps[i / L] = (uint8_t)(127 - k);
-      if (GELU) {
-        Bytes16 out;
-        T* oe = reinterpret_cast<T*>(&out);
+        for (int j = 0; j < V; ++j) w[j] = v[j];
+        if (__any_sync(0xffffffffu, a >= 0x7f800000u)) {
+          a = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) oe[j] = from_f32<T>(gelu_f(v[j]));
-        reinterpret_cast<Bytes16*>(y)[i] = out;
+          for (int j = 0; j < V; ++j) {
+            a = max(a, finite_bits(v[j]));
+            w[j] = inf_to_nan(v[j]);
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < L; o <<= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+        if (i >= nv) continue;
+        const int k = block_shift(a);
+        const float s = __uint_as_float((uint32_t)(k + 127) << 23);
+        uint32_t c[V / 4];
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const uint32_t lo = f32x2_to_fp8x2<FMT_E4M3>(mul_keep(w[j], s), mul_keep(w[j + 1], s));
+          const uint32_t hi = f32x2_to_fp8x2<FMT_E4M3>(mul_keep(w[j + 2], s), mul_keep(w[j + 3], s));
+          c[j / 4] = lo | hi << 16;
+        }
+        if (V == 8) reinterpret_cast<uint2*>(codes)[i] = make_uint2(c[0], c[V / 4 - 1]);
+        else        reinterpret_cast<uint32_t*>(codes)[i] = c[0];
+        if (threadIdx.x % L == 0) exps[i / L] = (uint8_t)(127 - k);
+        if (GELU) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = gelu_f(v[j]);
+          reinterpret_cast<Bytes16*>(y)[i] = pack<T>(v);
+        }
       }
     }
   }
+  const int64_t tid = (int64_t)blockIdx.x * kThreads + threadIdx.x, threads = (int64_t)gridDim.x * kThreads;
   const int64_t blocks = (n + kBlock - 1) / kBlock;
   for (int64_t b = full + tid / 32; b < blocks; b += threads / 32) cast_block_by_lane<T, GELU>(x, y, codes, exps, n, b);
 }
+
+// From this exponent byte on a code can stand for more than the largest number of T (448 * 2^(byte - 127) in bf16 and fp32 from 2^120 on, in
+// fp16 from 2^8 on).
+template <typename T>
+__device__ __forceinline__ bool may_overflow(uint32_t byte) { return byte >= (sizeof(T) == 2 && largest<T>() < 65505.0f ? 135u : 247u); }
 
 template <typename T, bool GELU>
 __device__ __forceinline__ T uncast_one(float v, T dy) {
@@ -124,34 +194,58 @@ __device__ __forceinline__ T uncast_one(float v, T dy) {
   return from_f32<T>(in_range<T>(v));
 }
 
+// Bound by memory: two vectors a thread and step in flight.
 template <typename T, bool GELU, bool VEC>
 __global__ void __launch_bounds__(kThreads) blocks_uncast_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
                                                                  const T* __restrict__ dy, T* __restrict__ out, int64_t n) {
-  const int64_t tid = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t threads = (int64_t)gridDim.x * kThreads;
-  constexpr int V = 16 / sizeof(T), L = kBlock / V;
+  constexpr int V = Vec<T>::V, L = Vec<T>::L, U = 2;
   const int64_t nv = VEC ? n / V : 0;
-  if (VEC) {
-    for (int64_t i = tid; i < nv; i += threads) {
-      uint32_t c[2];
-      if (V == 8) {
-        const uint2 r = reinterpret_cast<const uint2*>(codes)[i];
-        c[0] = r.x;
-        c[1] = r.y;
-      } else {
-        c[0] = reinterpret_cast<const uint32_t*>(codes)[i];
-      }
-      Bytes16 g = {}, o;
-      if (GELU) g = reinterpret_cast<const Bytes16*>(dy)[i];
-      const float u = block_unit(exps[i / L]);
-      const T* ge = reinterpret_cast<const T*>(&g);
-      T* oe = reinterpret_cast<T*>(&o);
+  if constexpr (VEC) {
+    for (int64_t i0 = (int64_t)blockIdx.x * (kThreads * U) + threadIdx.x; i0 < nv; i0 += (int64_t)gridDim.x * (kThreads * U)) {
+      uint32_t c[U][V / 4], byte[U];
+      Bytes16 g[U];
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        oe[j] = uncast_one<T, GELU>(mul_keep(fp8_to_f32<FMT_E4M3>((uint8_t)(c[j / 4] >> (8 * (j & 3)))), u), ge[j]);
-      reinterpret_cast<Bytes16*>(out)[i] = o;
+      for (int u = 0; u < U; ++u) {
+        const int64_t i = i0 + u * kThreads;
+        g[u] = Bytes16{};
+        byte[u] = c[u][0] = c[u][V / 4 - 1] = 0;
+        if (i >= nv) continue;
+        if (V == 8) {
+          const uint2 r = reinterpret_cast<const uint2*>(codes)[i];
+          c[u][0] = r.x;
+          c[u][V / 4 - 1] = r.y;
+        } else {
+          c[u][0] = reinterpret_cast<const uint32_t*>(codes)[i];
+        }
+        byte[u] = exps[i / L];
+        if (GELU) g[u] = reinterpret_cast<const Bytes16*>(dy)[i];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t i = i0 + u * kThreads;
+        if (i >= nv) continue;
+        const float unit = block_unit(byte[u]);
+        float v[V], d[V];
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c[u][j / 4] >> (8 * (j & 2))), __NV_E4M3);
+          const float2 f = __half22float2(__half2(h));
+          v[j] = mul_keep(f.x, unit);
+          v[j + 1] = mul_keep(f.y, unit);
+        }
+        if (GELU) {
+          unpack<T>(g[u], d);
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = d[j] * gelu_grad_f(v[j]);
+        } else if (may_overflow<T>(byte[u])) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = in_range<T>(v[j]);
+        }
+        reinterpret_cast<Bytes16*>(out)[i] = pack<T>(v);
+      }
     }
   }
+  const int64_t tid = (int64_t)blockIdx.x * kThreads + threadIdx.x, threads = (int64_t)gridDim.x * kThreads;
   for (int64_t i = nv * V + tid; i < n; i += threads)
     out[i] = uncast_one<T, GELU>(mul_keep(fp8_to_f32<FMT_E4M3>(codes[i]), block_unit(exps[i / kBlock])), GELU ? dy[i] : T());
 }
@@ -165,7 +259,7 @@ MSAMP_API int msamp_blocks_cast(const void* x, void* y, void* codes, void* exps,
   cudaStream_t stream = (cudaStream_t)stream_;
   const bool vec = aligned16(x) && aligned16(codes) && (!y || aligned16(y));
   MSAMP_DISPATCH_HP(dtype, T, {
-    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 15) / 16 : n, kThreads, 8);
+    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 31) / 32 : n, kThreads, 8);
     if (vec && y)  blocks_cast_kernel<T, true, true><<<grid, kThreads, 0, stream>>>((const T*)x, (T*)y, (uint8_t*)codes, (uint8_t*)exps, n);
     else if (vec)  blocks_cast_kernel<T, false, true><<<grid, kThreads, 0, stream>>>((const T*)x, nullptr, (uint8_t*)codes, (uint8_t*)exps, n);
     else if (y)    blocks_cast_kernel<T, true, false><<<grid, kThreads, 0, stream>>>((const T*)x, (T*)y, (uint8_t*)codes, (uint8_t*)exps, n);
@@ -181,7 +275,7 @@ MSAMP_API int msamp_blocks_uncast(const void* codes, const void* exps, const voi
   cudaStream_t stream = (cudaStream_t)stream_;
   const bool vec = aligned16(codes) && aligned16(out) && (!dy || aligned16(dy));
   MSAMP_DISPATCH_HP(dtype, T, {
-    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 15) / 16 : n, kThreads, 8);
+    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 31) / 32 : n, kThreads, 8);
     const uint8_t *c = (const uint8_t*)codes, *e = (const uint8_t*)exps;
     if (vec && dy) blocks_uncast_kernel<T, true, true><<<grid, kThreads, 0, stream>>>(c, e, (const T*)dy, (T*)out, n);
     else if (vec)  blocks_uncast_kernel<T, false, true><<<grid, kThreads, 0, stream>>>(c, e, nullptr, (T*)out, n);
