@@ -16,6 +16,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 32;
+constexpr int kUnroll = 2;    // vectors of a thread in flight
+static inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 
 __device__ __forceinline__ float mul_keep(float a, float b) {
   float d;
@@ -68,11 +70,24 @@ __device__ __forceinline__ void cast_block_by_lane(const T* x, T* y, uint8_t* co
   if (lane == 0) exps[blk] = (uint8_t)(127 - k);
 }
 
-// A 16-byte vector of T: V elements, as 32-bit words of one or two.
+// A 32-byte vector of T: V elements, as 32-bit words of one or two.
 template <typename T>
 struct Vec {
-  static constexpr int V = 16 / sizeof(T), L = kBlock / V;    // elements of a vector, lanes of a block
+  static constexpr int V = 32 / sizeof(T), L = kBlock / V;    // elements of a vector, lanes of a block
 };
+struct alignas(32) Bytes32 { uint32_t w[8]; };
+__device__ __forceinline__ Bytes32 ld32(const void* p) {
+  Bytes32 r;
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+               : "l"(p));
+  return r;
+}
+__device__ __forceinline__ void st32(void* p, const Bytes32& r) {
+  asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]), "r"(r.w[4]),
+               "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7]), "l"(p)
+               : "memory");
+}
 // The two elements of a word of 16-bit T
 __device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 __device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
@@ -85,13 +100,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
   return *reinterpret_cast<uint32_t*>(&t);
 }
 template <typename T>
-__device__ __forceinline__ void unpack(const Bytes16& raw, float (&v)[Vec<T>::V]) {
+__device__ __forceinline__ void unpack(const Bytes32& raw, float (&v)[Vec<T>::V]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(raw.w[j]);
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw.w[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 8; ++j) {
       const float2 f = unpack2(raw.w[j], T());
       v[2 * j] = f.x;
       v[2 * j + 1] = f.y;
@@ -99,10 +114,10 @@ __device__ __forceinline__ void unpack(const Bytes16& raw, float (&v)[Vec<T>::V]
   }
 }
 template <typename T>
-__device__ __forceinline__ Bytes16 pack(const float (&v)[Vec<T>::V]) {
-  Bytes16 o;
+__device__ __forceinline__ Bytes32 pack(const float (&v)[Vec<T>::V]) {
+  Bytes32 o;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 8; ++j) {
     if constexpr (sizeof(T) == 4) o.w[j] = __float_as_uint(v[j]);
     else                          o.w[j] = pack2(v[2 * j], v[2 * j + 1], T());
   }
@@ -110,10 +125,10 @@ __device__ __forceinline__ Bytes16 pack(const float (&v)[Vec<T>::V]) {
 }
 // Largest |x| of a vector as bits of fp32, from packed integer maxima (|x| as bits is monotone, with infinities and NaN on top)
 template <typename T>
-__device__ __forceinline__ uint32_t vector_amax(const Bytes16& raw) {
+__device__ __forceinline__ uint32_t vector_amax(const Bytes32& raw) {
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 8; ++j) {
     if (sizeof(T) == 4) m = max(m, raw.w[j] & 0x7fffffffu);
     else                m = __vmaxu2(m, raw.w[j] & 0x7fff7fffu);
   }
@@ -125,19 +140,19 @@ __device__ __forceinline__ uint32_t vector_amax(const Bytes16& raw) {
   }
 }
 
-// Bound by memory.  VEC: every pointer aligned for whole vectors; two vectors a thread and step are in flight, L lanes find the maximum of a
-// block with log2(L) shuffles.  A warp that sees an infinity or a NaN (its maxima are on top of all numbers) goes over its elements again.
+// Bound by memory.  VEC: every pointer aligned for whole vectors of 32 bytes, so that a thread stores 16 codes at once and a warp 16 exponents;
+// two vectors a thread and step are in flight, L lanes find the maximum of a block with log2(L) shuffles.  A warp that sees an infinity or a NaN (its maxima are on top of all numbers) goes over its elements again.
 template <typename T, bool GELU, bool VEC>
 __global__ void __launch_bounds__(kThreads) blocks_cast_kernel(const T* __restrict__ x, T* __restrict__ y, uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ exps, int64_t n) {
   const int64_t full = VEC ? n / kBlock : 0;    // blocks taken by vectors
   if constexpr (VEC) {
-    constexpr int V = Vec<T>::V, L = Vec<T>::L, U = 2;
+    constexpr int V = Vec<T>::V, L = Vec<T>::L, U = kUnroll;
     const int64_t nv = full * L;
     for (int64_t i0 = (int64_t)blockIdx.x * (kThreads * U) + threadIdx.x; i0 - threadIdx.x < nv; i0 += (int64_t)gridDim.x * (kThreads * U)) {
-      Bytes16 raw[U];
+      Bytes32 raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = i0 + u * kThreads < nv ? reinterpret_cast<const Bytes16*>(x)[i0 + u * kThreads] : Bytes16{};
+      for (int u = 0; u < U; ++u) raw[u] = i0 + u * kThreads < nv ? ld32(x + (i0 + u * kThreads) * V) : Bytes32{};
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t i = i0 + u * kThreads;
@@ -167,13 +182,13 @@ __global__ void __launch_bounds__(kThreads) blocks_cast_kernel(const T* __restri
           const uint32_t hi = f32x2_to_fp8x2<FMT_E4M3>(mul_keep(w[j + 2], s), mul_keep(w[j + 3], s));
           c[j / 4] = lo | hi << 16;
         }
-        if (V == 8) reinterpret_cast<uint2*>(codes)[i] = make_uint2(c[0], c[V / 4 - 1]);
-        else        reinterpret_cast<uint32_t*>(codes)[i] = c[0];
+        if constexpr (V == 16) reinterpret_cast<uint4*>(codes)[i] = make_uint4(c[0], c[1], c[2], c[3]);
+        else                   reinterpret_cast<uint2*>(codes)[i] = make_uint2(c[0], c[1]);
         if (threadIdx.x % L == 0) exps[i / L] = (uint8_t)(127 - k);
         if (GELU) {
 #pragma unroll
           for (int j = 0; j < V; ++j) v[j] = gelu_f(v[j]);
-          reinterpret_cast<Bytes16*>(y)[i] = pack<T>(v);
+          st32(y + i * V, pack<T>(v));
         }
       }
     }
@@ -198,27 +213,29 @@ __device__ __forceinline__ T uncast_one(float v, T dy) {
 template <typename T, bool GELU, bool VEC>
 __global__ void __launch_bounds__(kThreads) blocks_uncast_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
                                                                  const T* __restrict__ dy, T* __restrict__ out, int64_t n) {
-  constexpr int V = Vec<T>::V, L = Vec<T>::L, U = 2;
+  constexpr int V = Vec<T>::V, L = Vec<T>::L, U = kUnroll;
   const int64_t nv = VEC ? n / V : 0;
   if constexpr (VEC) {
     for (int64_t i0 = (int64_t)blockIdx.x * (kThreads * U) + threadIdx.x; i0 < nv; i0 += (int64_t)gridDim.x * (kThreads * U)) {
       uint32_t c[U][V / 4], byte[U];
-      Bytes16 g[U];
+      Bytes32 g[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t i = i0 + u * kThreads;
-        g[u] = Bytes16{};
-        byte[u] = c[u][0] = c[u][V / 4 - 1] = 0;
         if (i >= nv) continue;
-        if (V == 8) {
+        if constexpr (V == 16) {
+          const uint4 r = reinterpret_cast<const uint4*>(codes)[i];
+          c[u][0] = r.x;
+          c[u][1] = r.y;
+          c[u][2] = r.z;
+          c[u][3] = r.w;
+        } else {
           const uint2 r = reinterpret_cast<const uint2*>(codes)[i];
           c[u][0] = r.x;
-          c[u][V / 4 - 1] = r.y;
-        } else {
-          c[u][0] = reinterpret_cast<const uint32_t*>(codes)[i];
+          c[u][1] = r.y;
         }
         byte[u] = exps[i / L];
-        if (GELU) g[u] = reinterpret_cast<const Bytes16*>(dy)[i];
+        if (GELU) g[u] = ld32(dy + i * V);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -241,7 +258,7 @@ __global__ void __launch_bounds__(kThreads) blocks_uncast_kernel(const uint8_t* 
 #pragma unroll
           for (int j = 0; j < V; ++j) v[j] = in_range<T>(v[j]);
         }
-        reinterpret_cast<Bytes16*>(out)[i] = pack<T>(v);
+        st32(out + i * V, pack<T>(v));
       }
     }
   }
@@ -257,9 +274,9 @@ MSAMP_API int msamp_blocks_cast(const void* x, void* y, void* codes, void* exps,
   if (n <= 0) return MSAMP_OK;
   MSAMP_REQUIRE(x && codes && exps, "blocks_cast: null pointer");
   cudaStream_t stream = (cudaStream_t)stream_;
-  const bool vec = aligned16(x) && aligned16(codes) && (!y || aligned16(y));
+  const bool vec = aligned32(x) && aligned32(codes) && (!y || aligned32(y));
   MSAMP_DISPATCH_HP(dtype, T, {
-    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 31) / 32 : n, kThreads, 8);
+    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 32 * kUnroll - 1) / (32 * kUnroll) : n, kThreads, 8);
     if (vec && y)  blocks_cast_kernel<T, true, true><<<grid, kThreads, 0, stream>>>((const T*)x, (T*)y, (uint8_t*)codes, (uint8_t*)exps, n);
     else if (vec)  blocks_cast_kernel<T, false, true><<<grid, kThreads, 0, stream>>>((const T*)x, nullptr, (uint8_t*)codes, (uint8_t*)exps, n);
     else if (y)    blocks_cast_kernel<T, true, false><<<grid, kThreads, 0, stream>>>((const T*)x, (T*)y, (uint8_t*)codes, (uint8_t*)exps, n);
@@ -273,9 +290,9 @@ MSAMP_API int msamp_blocks_uncast(const void* codes, const void* exps, const voi
   if (n <= 0) return MSAMP_OK;
   MSAMP_REQUIRE(codes && exps && out, "blocks_uncast: null pointer");
   cudaStream_t stream = (cudaStream_t)stream_;
-  const bool vec = aligned16(codes) && aligned16(out) && (!dy || aligned16(dy));
+  const bool vec = aligned32(codes) && aligned32(out) && (!dy || aligned32(dy));
   MSAMP_DISPATCH_HP(dtype, T, {
-    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 31) / 32 : n, kThreads, 8);
+    const int grid = msamp_grid_for(vec ? (n * (int64_t)sizeof(T) + 32 * kUnroll - 1) / (32 * kUnroll) : n, kThreads, 8);
     const uint8_t *c = (const uint8_t*)codes, *e = (const uint8_t*)exps;
     if (vec && dy) blocks_uncast_kernel<T, true, true><<<grid, kThreads, 0, stream>>>(c, e, (const T*)dy, (T*)out, n);
     else if (vec)  blocks_uncast_kernel<T, false, true><<<grid, kThreads, 0, stream>>>(c, e, nullptr, (T*)out, n);
