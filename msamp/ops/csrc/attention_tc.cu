@@ -1122,7 +1122,7 @@ struct FwdItems {
         j = c;
         x.first = g;
         x.step = 2;
-      } else {
+      } else if (!X || !(w & 1)) {    // an odd last wave goes downwards as well: the shortest sums take its longest items
         j = g * n_ctas + c;
       }
       if (j >= rem) return x;
