@@ -37,7 +37,7 @@ constexpr unsigned int kStatusBit = 4u;
 struct TcParams {
   __nv_bfloat16* o;
   float* lse;             // [b, h, s] natural-log sum-exp of the scaled scores
-  const float* delta;     // [b, h, s] rowsum(dO * O)
+  float* delta;           // [b, h, s] rowsum(dO * O)
   __nv_bfloat16* dq;
   __nv_bfloat16* dk;
   __nv_bfloat16* dv;
@@ -52,16 +52,16 @@ struct TcParams {
   // kernels with X only
   int kv_heads, rep;       // key / value heads; query heads of each
   const int* lengths;      // X == 2: [batch] positions of a row that are not padding
-  const int* plan;         // X == 2: the number of tiles that are not padding alone, then those tiles (see attn_plan_kernel)
-  int parts;               // dK / dV: work items that share the query heads of a key / value head
-  float* partial;          // [parts][dK, dV][batch, kv_heads, seqlen, head_dim] when there are several
+  const int* plan;         // X == 2: the number of tiles that are not padding alone, parts, then those tiles (see attn_plan_kernel)
+  int parts;               // X == 1, dK / dV: work items that share the query heads of a key / value head
+  float* partial;          // [item][dK, dV][head_dim / 4][128 rows][4] when there are several
 };
 
 __device__ __forceinline__ int row_length(const int* lengths, int b, int seqlen) { return min(max(__ldg(lengths + b), 0), seqlen); }
 __device__ __forceinline__ int row_length(const TcParams& p, int b) { return row_length(p.lengths, b, p.seqlen); }
 // The n-th tile of the plan: its batch and its number in the sequence
 __device__ __forceinline__ void planned_tile(const TcParams& p, int n, int n_tiles, int& b, int& i) {
-  const int code = __ldg(p.plan + 1 + n);
+  const int code = __ldg(p.plan + 2 + n);
   b = code / n_tiles;
   i = code - b * n_tiles;
 }
@@ -2690,13 +2690,14 @@ attn_bwd_dq_tm_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 // ============================================================================ dQ, persistent CTAs over the work items
 namespace dqk3 {
 using namespace dqk2;
-enum { B3_QE = NBAR, B3_OE = NBAR + 1, B3_KL = NBAR + 2, NBAR3 = B3_KL + NK };
+enum { B3_QE = NBAR, B3_OE = NBAR + 1, B3_KL = NBAR + 2, B3_DX = B3_KL + NK, NBAR3 = B3_DX + 1 };
 template <int D>
 struct Cfg {
   static constexpr int HP = D / 64;
   static constexpr uint32_t TILE = HP * PANEL;    // 128 rows of one head
   static constexpr uint32_t OFF_DO = TILE, OFF_K = 2 * TILE, OFF_V = OFF_K + NK * TILE, OFF_BAR = OFF_V + NV * TILE;
   static constexpr int SMEM = OFF_BAR + NBAR3 * 8 + 16 + 1024;
+  static_assert(SMEM <= 227 * 1024, "persistent dQ kernel: shared memory");
 };
 }    // namespace dqk3
 
@@ -2708,7 +2709,10 @@ struct Cfg {
 // of an item are complete, Q and dO may be overwritten; B3_OE: the softmax warps have read dQ, the accumulator may be
 // overwritten by the first product of the next item.
 // X: shared key / value heads and row lengths as in the forward kernel; the K tiles with rows behind the end of their sequence land on
-// B3_KL and warp 3 clears those rows.
+// B3_KL and warp 3 clears those rows.  A query tile whose keys are one tile does not take delta from the rounded output but as
+// sum P dP, in 32 bits from the tile itself (the two groups' halves meet at B3_DX), and leaves it for the dK / dV kernel, which
+// therefore comes after this one: with few keys a row's dS is a small difference, and the rounding of O and of the P in it put
+// the gradients of rows of 2 to 16 keys up to 0.8 % off in norm, three times the rounding of dS.
 template <int D, int X>
 __global__ void __launch_bounds__(kPsThreads, 1)
 attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -2779,6 +2783,7 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     tc5::mbar_init(bar(B_ACC), 1);
     tc5::mbar_init(bar(B3_QE), 1);
     tc5::mbar_init(bar(B3_OE), 8);
+    if (X) tc5::mbar_init(bar(B3_DX), 8);
     if (X == 2)
       for (int s = 0; s < NK; ++s) tc5::mbar_init(bar(B3_KL + s), 1);
     *abort_flag = 0;
@@ -2928,6 +2933,7 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const int row = qd * 32 + lane;
     const uint32_t tlane = tmem_base + ((uint32_t)(qd * 32) << 16);
     const float sl = p.scale * kLog2e;
+    uint32_t n_dx = 0;    // items of one key tile so far
     int g0 = 0, it = 0;
     bool ok = true;
     for (int w = 0; w < n_waves && ok; ++w) {
@@ -2942,7 +2948,8 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       const int64_t at = ((int64_t)b * p.heads + h) * p.seqlen + grow;
       const float lse2 = in ? p.lse[at] * kLog2e : INFINITY;
       const float dlt = in ? p.delta[at] : 0.0f;
-      const uint64_t sl2 = f2_pack(sl, sl), nlse2 = f2_pack(-lse2, -lse2), ndlt2 = f2_pack(-dlt, -dlt);
+      const uint64_t sl2 = f2_pack(sl, sl), nlse2 = f2_pack(-lse2, -lse2);
+      uint64_t ndlt2 = f2_pack(-dlt, -dlt);
       const int lim = p.causal ? min(grow, len - 1) : len - 1;
       for (int t = 0; t < n_t; ++t) {
         const int gt = g0 + t;
@@ -2973,6 +2980,27 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         tc5::tmem_ld32(tdp + 32u, rd[1]);
         tc5::tmem_ld_wait();
         if (X == 2 && need_mask) mask_above(rd, lim - col0, 0u);    // dP of padding may be anything
+        if (X && n_t == 1) {
+          uint64_t a2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+#pragma unroll
+          for (int i = 0; i < 64; i += 2)
+            a2[(i >> 1) & 1] = f2_fma(f2_pack(__uint_as_float(rs[i >> 5][i & 31]), __uint_as_float(rs[i >> 5][(i & 31) + 1])),
+                                      f2_pack(__uint_as_float(rd[i >> 5][i & 31]), __uint_as_float(rd[i >> 5][(i & 31) + 1])), a2[(i >> 1) & 1]);
+          const float2 a = f2_unpack(f2_add(a2[0], a2[1]));
+          // through the columns of the dP tile that dS leaves free; dP of a later tile comes after dQ of this one, which comes after both
+          const float mine = a.x + a.y;
+          tc5::tmem_st1(tdp + 32u, __float_as_uint(mine));
+          tc5::tmem_st_wait();
+          tc5::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc5::mbar_arrive(bar(B3_DX));
+          if (!wait_warp(bar(B3_DX), n_dx & 1u)) { ok = false; break; }
+          ++n_dx;
+          tc5::fence_after_sync();
+          const float sum = mine + __uint_as_float(tc5::tmem_ld1(wg ? tdp - 32u : tdp + 96u));
+          ndlt2 = f2_pack(-sum, -sum);
+          if (wg == 0 && in) p.delta[at] = sum;
+        }
         uint32_t pk[32];
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
@@ -3057,7 +3085,8 @@ struct Cfg {
 // B3_KVE: every S^T / dP^T product of an item is complete, K and V may be overwritten by the next item's; B3_OE: the softmax
 // warps have read dV and dK, the first products of the next item may overwrite the accumulators.
 // X: an item takes the query tiles of all (or, in `parts`, of some) query heads of its key / value head one after the other into the same
-// accumulators, so the sum over the heads is in 32 bits; parts leave theirs in `partial`, which attn_bwd_join_kernel adds up in order.
+// accumulators, so the sum over the heads is in 32 bits; parts leave theirs in `partial` (four columns of 128 rows at a time, which is how
+// the threads hold them), which attn_bwd_join_kernel adds up in order.
 // X == 2: the key tiles of the plan, longest first.  Q and dO tiles with rows behind the end of their sequence land on B3_QL and B3_OL and
 // warp 3 clears those rows.
 template <int D, int X>
@@ -3091,8 +3120,9 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int nq_all = (p.seqlen + 127) / 128;
-  const ItemOrder order{n_kt, X ? p.batch * p.kv_heads * p.parts : p.batch * p.heads, p.group};
-  const int per_item = X ? p.rep / p.parts : 1;    // query heads of an item
+  const int parts = X == 2 ? __ldg(p.plan + 1) : X ? p.parts : 1;
+  const ItemOrder order{n_kt, X ? p.batch * p.kv_heads * parts : p.batch * p.heads, p.group};
+  const int per_item = X ? p.rep / parts : 1;    // query heads of an item
   // Work item -> its batch, first query head, key / value head and query tiles (n_q for each of the query heads)
   struct Item {
     int kt, b, h, hk, part, len, t_first, n_q, n_u;
@@ -3102,7 +3132,7 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     int idx, n_len = nq_all;    // query tiles of the row
     x.len = p.seqlen;
     if (X == 2) {
-      const int per_tile = p.kv_heads * p.parts, n = item / per_tile;
+      const int per_tile = p.kv_heads * parts, n = item / per_tile;
       int i;
       planned_tile(p, n, n_kt, x.b, i);
       idx = item - n * per_tile;
@@ -3113,8 +3143,8 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       order.decode(item, x.kt, idx);
     }
     if (X) {
-      const int bk = idx / p.parts;
-      x.part = idx - bk * p.parts;
+      const int bk = idx / parts;
+      x.part = idx - bk * parts;
       if (X != 2) x.b = bk / p.kv_heads;
       x.hk = X == 2 ? bk : bk - x.b * p.kv_heads;
       x.h = x.hk * p.rep + x.part * per_item;
@@ -3128,7 +3158,7 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     x.n_u = X ? x.n_q * per_item : x.n_q;
     return x;
   };
-  const int n_items = X == 2 ? __ldg(p.plan) * p.kv_heads * p.parts : max_items;
+  const int n_items = X == 2 ? __ldg(p.plan) * p.kv_heads * parts : max_items;
   const int n_waves = (n_items + (int)gridDim.x - 1) / (int)gridDim.x;
   auto item_at = [&](int w) {
     const int c = (w & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x;
@@ -3503,15 +3533,15 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
       if (lane == 0) tc5::mbar_arrive(bar(B3_OE));
       g0 += n_q;
       ++it;
-      if (X && p.parts > 1) {
+      if (X && parts > 1) {
+        const int slot = X == 2 ? again : ((b * p.kv_heads + h) * n_kt + x.kt) * parts + x.part;
         if (grow < x.len) {
-          float* out = p.partial + ((((int64_t)x.part * 2 + 1 - wg) * p.batch + b) * p.kv_heads + h) * p.seqlen * D + (int64_t)grow * D;
+          float4* out = reinterpret_cast<float4*>(p.partial) + ((int64_t)slot * 2 + 1 - wg) * (D / 4 * 128) + row;
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(out + c * 32 + i) = make_float4(__uint_as_float(acc[c][i]) * f, __uint_as_float(acc[c][i + 1]) * f,
-                                                                         __uint_as_float(acc[c][i + 2]) * f, __uint_as_float(acc[c][i + 3]) * f);
+          for (int c = 0; c < D / 4; ++c) {
+            const uint32_t* v = &acc[c / 8][c % 8 * 4];
+            out[c * 128] = make_float4(__uint_as_float(v[0]) * f, __uint_as_float(v[1]) * f, __uint_as_float(v[2]) * f, __uint_as_float(v[3]) * f);
+          }
         }
         continue;
       }
@@ -3533,41 +3563,81 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   if (warp == 1) tc5::tmem_dealloc(tmem_base, TM_COLS);
 }
 
-// dK and dV of the parts of a work item, added up in order: bound by memory.
+// dK and dV of the parts of a key tile, added up in order; a CTA takes 16 columns of 128 rows of one of them.  Bound by memory.
 struct JoinParams {
-  const float* partial;
-  __nv_bfloat16 *dk, *dv;
-  int64_t dk_sb, dk_ss, dk_sh, dv_sb, dv_ss, dv_sh;
-  int parts, batch, kv_heads, seqlen;
-  const int* lengths;
+  TcParams p;
+  int n_kt;
 };
-template <int D>
-__global__ void __launch_bounds__(256) attn_bwd_join_kernel(const JoinParams p) {
-  constexpr int L = D / 8;    // threads of a row, eight elements each
-  const int64_t rows = (int64_t)p.batch * p.kv_heads * p.seqlen;
-  const int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (r >= 2 * rows) return;
-  const bool is_v = r >= rows;
-  const int64_t row = is_v ? r - rows : r;
-  const int c = (threadIdx.x % L) * 8;
-  const int s = (int)(row % p.seqlen);
-  const int64_t bh = row / p.seqlen;
-  const int h = (int)(bh % p.kv_heads);
-  const int64_t b = bh / p.kv_heads;
-  if (p.lengths && s >= __ldg(p.lengths + b)) return;    // padding: cleared before
-  float v[8] = {};
-  for (int k = 0; k < p.parts; ++k) {
-    const float4* src = reinterpret_cast<const float4*>(p.partial + ((int64_t)k * 2 * rows + r) * D + c);
-    const float4 a = src[0], b = src[1];
-    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+template <int D, int X>
+__global__ void __launch_bounds__(128) attn_bwd_join_kernel(const JoinParams j) {
+  const TcParams& p = j.p;
+  const int parts = X == 2 ? __ldg(p.plan + 1) : p.parts;
+  if (X == 2 && parts == 1) return;
+  const int c = blockIdx.x % (D / 16), which = blockIdx.x / (D / 16) & 1;
+  const int tile = blockIdx.x / (D / 8);    // n * kv_heads + head of the plan, or (batch * kv_heads + head) * n_kt + key tile
+  int b, h, kt, len = p.seqlen;
+  if (X == 2) {
+    const int n = tile / p.kv_heads;
+    if (n >= __ldg(p.plan)) return;
+    int i;
+    planned_tile(p, n, j.n_kt, b, i);
+    h = tile - n * p.kv_heads;
+    len = row_length(p, b);
+    kt = p.causal ? (len + 127) / 128 - 1 - i : i;
+  } else {
+    const int bh = tile / j.n_kt;
+    kt = tile - bh * j.n_kt;
+    b = bh / p.kv_heads;
+    h = bh - b * p.kv_heads;
   }
-  __nv_bfloat16* dst = is_v ? p.dv + b * p.dv_sb + (int64_t)s * p.dv_ss + (int64_t)h * p.dv_sh : p.dk + b * p.dk_sb + (int64_t)s * p.dk_ss + (int64_t)h * p.dk_sh;
-  *reinterpret_cast<uint4*>(dst + c) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  const int s = kt * 128 + threadIdx.x;
+  if (s >= len) return;
+  const float4* src = reinterpret_cast<const float4*>(p.partial) + ((int64_t)tile * parts * 2 + which) * (D / 4 * 128) + c * 4 * 128 + threadIdx.x;
+  float v[16] = {};
+  for (int k = 0; k < parts; ++k, src += 2 * (D / 4 * 128)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 a = src[i * 128];
+      v[4 * i] += a.x;
+      v[4 * i + 1] += a.y;
+      v[4 * i + 2] += a.z;
+      v[4 * i + 3] += a.w;
+    }
+  }
+  __nv_bfloat16* dst = which ? p.dv + (int64_t)b * p.dv_sb + (int64_t)s * p.dv_ss + (int64_t)h * p.dv_sh
+                             : p.dk + (int64_t)b * p.dk_sb + (int64_t)s * p.dk_ss + (int64_t)h * p.dk_sh;
+  uint4* d4 = reinterpret_cast<uint4*>(dst + c * 16);
+  d4[0] = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+  d4[1] = make_uint4(pack_bf16(v[8], v[9]), pack_bf16(v[10], v[11]), pack_bf16(v[12], v[13]), pack_bf16(v[14], v[15]));
+}
+
+// Into how many parts the query heads of a key / value head are cut for dK / dV, a divisor of their number.  Time is counted in tiles of
+// 128 x 128 (1.8 us): the longest item, or the mean over the SMs where that is more (items of one size: whole waves of them); parts add
+// the launch that joins them, two, and the writing and reading of their sums, one for 50 items of head size 128.  items: key tiles times
+// key / value heads; units: tiles of all of them; longest: tiles of the longest row.
+// Backward pass of 1 x 4096 x 16 / 1 heads of 128, causal, in 1, 2, 4, 8 and 16 parts: 1048, 591, 362, 249 and 259 us (8 chosen);
+// 2 x 1000 x 12 / 4 of 64 in 1 and 3: 73 and 54 (3); 2 x 2048 x 16 / 4 of 128 in 1, 2 and 4: 204, 156 and 169 (2); 4 x 2048 x 32 / 8 of 128
+// in 1, 2 and 4: 499, 542 and 579 (1); 2 x 2048 x 16 / 4 of 128, not causal: 247, 261 and 278 (1).
+constexpr int kPartSlots = 3;    // items in parts at most, for each SM (their workspace is 128 KB each at head size 128)
+__host__ __device__ __forceinline__ int choose_parts(int rep, int64_t items, int64_t units, int longest, int head_dim, int sms, bool one_size) {
+  const float mean = (float)units / (float)sms;
+  int best = 1;
+  float least = 0.0f;
+  for (int n = 1; n <= rep; ++n) {
+    if (rep % n != 0 || (n > 1 && items * n > (int64_t)kPartSlots * sms)) continue;
+    const int64_t waves = one_size ? (items * n + sms - 1) / sms : 1;
+    float t = fmaxf((float)waves * (float)longest * (float)(rep / n), mean);
+    if (n > 1) t += 2.0f + 0.02f * (float)(items * n) * (float)head_dim / 128.0f;
+    if (n == 1 || t < least) {
+      least = t;
+      best = n;
+    }
+  }
+  return best;
 }
 
 // Row lengths of a padded batch: the list of 128-row tiles that hold rows of a sequence, longest work first, and zeros (lse: -inf) for the
-// output rows of padding.  plan[0]: number of tiles; plan[1 + rank]: b * n_tiles + i for tile i of batch b.  The work of tile i is i + 1 tiles
+// output rows of padding.  plan[0]: number of tiles; plan[1]: parts (choose_parts); plan[2 + rank]: b * n_tiles + i for tile i of batch b.  The work of tile i is i + 1 tiles
 // when causal, else those of its row; ties go by batch, then by tile.  A tile counts the tiles in front of it, O(batch) each, so that no
 // sort and no atomic is needed.  blockIdx.x: batch, blockIdx.y: share of its padding.
 struct PlanParams {
@@ -3576,7 +3646,7 @@ struct PlanParams {
   __nv_bfloat16* o;
   float* lse;
   int64_t o_sb, o_ss, o_sh;
-  int batch, heads, seqlen, head_dim, n_tiles, causal;
+  int batch, heads, kv_heads, seqlen, head_dim, n_tiles, causal, sms;
 };
 __global__ void __launch_bounds__(256) attn_plan_kernel(const PlanParams p) {
   const int b = blockIdx.x;
@@ -3589,12 +3659,27 @@ __global__ void __launch_bounds__(256) attn_plan_kernel(const PlanParams p) {
         if (p.causal) rank += max(0, m - i - 1) + (c < b && m > i ? 1 : 0);
         else          rank += m > n || (m == n && c < b) ? m : 0;
       }
-      p.plan[1 + rank] = b * p.n_tiles + i;
+      p.plan[2 + rank] = b * p.n_tiles + i;
     }
-    if (b == 0 && threadIdx.x == 0) {
-      int total = 0;
-      for (int c = 0; c < p.batch; ++c) total += (row_length(p.lengths, c, p.seqlen) + 127) / 128;
-      p.plan[0] = total;
+    if (b == 0) {
+      __shared__ int s_total, s_longest;
+      __shared__ unsigned long long s_units;
+      if (threadIdx.x == 0) {
+        s_total = s_longest = 0;
+        s_units = 0;
+      }
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.batch; c += blockDim.x) {
+        const int m = (row_length(p.lengths, c, p.seqlen) + 127) / 128;
+        atomicAdd(&s_total, m);
+        atomicMax(&s_longest, m);
+        atomicAdd(&s_units, (unsigned long long)(p.causal ? (int64_t)m * (m + 1) / 2 : (int64_t)m * m) * p.heads);
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        p.plan[0] = s_total;
+        p.plan[1] = choose_parts(p.heads / p.kv_heads, (int64_t)s_total * p.kv_heads, (int64_t)s_units, s_longest, p.head_dim, p.sms, false);
+      }
     }
   }
   const int per_head = p.head_dim / 8, per_row = p.heads * per_head;
@@ -3912,7 +3997,7 @@ MSAMP_API int msamp_attention_tc_bwd(const void* q, const void* k, const void* v
 // ---- shared key / value heads and row lengths ----------------------------------------------------
 // Query heads h * rep .. h * rep + rep - 1 read key / value head h (heads == kv_heads * rep).  lengths [batch] (int32, or null): positions at or
 // behind a row's length are padding, as queries and as keys; their outputs and gradients are zero, their lse -inf, whatever they hold.  With
-// lengths the forward pass writes `plan` (1 + batch * ceil(seqlen / 128) ints), which the backward pass of the same lengths reads.
+// lengths the forward pass writes `plan` (2 + batch * ceil(seqlen / 128) ints), which the backward pass of the same lengths reads.
 // Strides as for the entry points above, those of k, v, dk and dv over kv_heads.
 static int shared_checks(int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, const int* lengths, const int* plan,
                          const int64_t* strides, int n) {
@@ -3937,9 +4022,10 @@ template <int D, int X>
 static int launch_bwd(const CUtensorMap (&m)[4], const TcParams& p, int n_t, int sms, cudaStream_t stream) {
   if (int rc = set_smem(attn_bwd_dkdv_ps_kernel<D, X>, dkv3::Cfg<D>::SMEM)) return rc;
   if (int rc = set_smem(attn_bwd_dq_ps_kernel<D, X>, dqk3::Cfg<D>::SMEM)) return rc;
-  const int n_q = n_t * p.batch * p.heads, n_k = n_t * p.batch * p.kv_heads * p.parts;
-  attn_bwd_dkdv_ps_kernel<D, X><<<n_k < sms ? n_k : sms, kPsThreads, dkv3::Cfg<D>::SMEM, stream>>>(m[0], m[1], m[2], m[3], p, n_t, n_k);
+  // with lengths the number of parts is known on the device only: as many CTAs as any number of them needs
+  const int n_q = n_t * p.batch * p.heads, n_k = n_t * p.batch * p.kv_heads * (X == 2 ? p.rep : p.parts);
   attn_bwd_dq_ps_kernel<D, X><<<n_q < sms ? n_q : sms, kPsThreads, dqk3::Cfg<D>::SMEM, stream>>>(m[0], m[1], m[2], m[3], p, n_t, n_q);
+  attn_bwd_dkdv_ps_kernel<D, X><<<n_k < sms ? n_k : sms, kPsThreads, dkv3::Cfg<D>::SMEM, stream>>>(m[0], m[1], m[2], m[3], p, n_t, n_k);
   return MSAMP_OK;
 }
 
@@ -3964,7 +4050,7 @@ struct SharedBwdArgs {
   const int *lengths, *plan;
   const void* d_o;
   void *dq, *dk, *dv;
-  float *delta, *partial;    // [batch, heads, seqlen]; see msamp_attention_shared_parts
+  float *delta, *partial;    // [batch, heads, seqlen]; msamp_attention_shared_partial floats
   SharedArgs n;
   int64_t strides[24];    // of q, k, v, o, dO, dq, dk, dv
 };
@@ -4006,7 +4092,7 @@ MSAMP_API int msamp_attention_shared_fwd(const SharedFwdArgs* a, void* stream_) 
   const int ctas = n_items < sms ? n_items : sms;
   cudaStream_t stream = (cudaStream_t)stream_;
   if (lengths) {
-    PlanParams w = {lengths, plan, p.o, lse, p.o_sb, p.o_ss, p.o_sh, batch, heads, seqlen, head_dim, n_qt, causal};
+    PlanParams w = {lengths, plan, p.o, lse, p.o_sb, p.o_ss, p.o_sh, batch, heads, kv_heads, seqlen, head_dim, n_qt, causal, sms};
     const int share = (4 * sms + batch - 1) / batch;
     attn_plan_kernel<<<dim3((unsigned)batch, (unsigned)(share < 64 ? share : 64)), 256, 0, stream>>>(w);
     rc = head_dim == 128 ? launch_fwd<128, 2>(m, p, n_qt, ctas, stream) : launch_fwd<64, 2>(m, p, n_qt, ctas, stream);
@@ -4016,16 +4102,26 @@ MSAMP_API int msamp_attention_shared_fwd(const SharedFwdArgs* a, void* stream_) 
   return rc ? rc : msamp_check_launch("attention forward (shared heads)");
 }
 
-// Parts into which the query heads of a key / value head are cut for dK / dV: the smallest divisor of `rep` that gives every SM an item.
-MSAMP_API int msamp_attention_shared_parts(int batch, int heads, int kv_heads, int seqlen) {
-  const int rep = heads / kv_heads;
-  const int64_t items = (int64_t)((seqlen + 127) / 128) * batch * kv_heads;
-  for (int n = 1; n < rep; ++n)
-    if (rep % n == 0 && items * n >= msamp_sm_count()) return n;
-  return rep;
+// Parts of dK / dV without lengths.
+static int uniform_parts(int batch, int heads, int kv_heads, int seqlen, int head_dim, int causal) {
+  const int64_t n = (seqlen + 127) / 128, items = n * batch * kv_heads;
+  return choose_parts(heads / kv_heads, items, (causal ? n * (n + 1) / 2 : n * n) * batch * heads, (int)n, head_dim, msamp_sm_count(),
+                      !causal);
+}
+// Floats of the workspace `partial` (0: none).  With lengths the parts are chosen on the device, up to kPartSlots items for each SM.
+MSAMP_API int64_t msamp_attention_shared_partial(int batch, int heads, int kv_heads, int seqlen, int head_dim, int causal, int lengths) {
+  if (batch <= 0 || kv_heads <= 0 || heads <= kv_heads || seqlen <= 0) return 0;
+  const int64_t items = (int64_t)((seqlen + 127) / 128) * batch * kv_heads, rep = heads / kv_heads;
+  int64_t slots;
+  if (lengths) {
+    slots = items * rep < (int64_t)kPartSlots * msamp_sm_count() ? items * rep : (int64_t)kPartSlots * msamp_sm_count();
+  } else {
+    const int parts = uniform_parts(batch, heads, kv_heads, seqlen, head_dim, causal);
+    slots = parts > 1 ? items * parts : 0;
+  }
+  return slots * 2 * 128 * head_dim;
 }
 
-// partial: parts * 2 * batch * kv_heads * seqlen * head_dim floats when msamp_attention_shared_parts gives more than one part.
 MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) {
   MSAMP_REQUIRE(a, "attention (shared heads): no arguments");
   if (int e = shared_sizes(a->n)) return e;
@@ -4042,8 +4138,9 @@ MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) 
   if (rc) return rc;
   MSAMP_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(d_o) && aligned16(dq) && aligned16(dk) && aligned16(dv),
                 "attention (shared heads): q, k, v, o, dO and the gradients must be 16-byte aligned");
-  const int parts = msamp_attention_shared_parts(batch, heads, kv_heads, seqlen);
-  MSAMP_REQUIRE(parts == 1 || (partial && aligned16(partial)), "attention (shared heads): no workspace for %d parts", parts);
+  const int parts = lengths ? 1 : uniform_parts(batch, heads, kv_heads, seqlen, head_dim, causal);
+  const bool join = lengths ? heads > kv_heads : parts > 1;
+  MSAMP_REQUIRE(!join || (partial && aligned16(partial)), "attention (shared heads): no workspace for partial sums");
   CUtensorMap m[4];
   if ((rc = make_map4(q, batch, heads, seqlen, head_dim, strides[0], strides[1], strides[2], 128, &m[0]))) return rc;
   if ((rc = make_map4(k, batch, kv_heads, seqlen, head_dim, strides[3], strides[4], strides[5], 128, &m[1]))) return rc;
@@ -4060,7 +4157,7 @@ MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) 
   p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.lengths = lengths; p.plan = plan; p.parts = parts; p.partial = partial;
   p.status = msamp_device_status_ptr();
   p.group = item_group(seqlen, head_dim);
-  {
+  if (lengths || seqlen > 128) {    // rows of one key tile: the dQ kernel finds delta itself
     DeltaParams d = {};
     d.o = (const __nv_bfloat16*)o; d.d_o = (const __nv_bfloat16*)d_o; d.delta = delta;
     d.o_sb = strides[9]; d.o_ss = strides[10]; d.o_sh = strides[11];
@@ -4083,16 +4180,14 @@ MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) 
   if (lengths) rc = head_dim == 128 ? launch_bwd<128, 2>(m, p, n_t, sms, stream) : launch_bwd<64, 2>(m, p, n_t, sms, stream);
   else         rc = head_dim == 128 ? launch_bwd<128, 1>(m, p, n_t, sms, stream) : launch_bwd<64, 1>(m, p, n_t, sms, stream);
   if (rc) return rc;
-  if (parts > 1) {
-    JoinParams j = {};
-    j.partial = partial; j.dk = p.dk; j.dv = p.dv;
-    j.dk_sb = p.dk_sb; j.dk_ss = p.dk_ss; j.dk_sh = p.dk_sh; j.dv_sb = p.dv_sb; j.dv_ss = p.dv_ss; j.dv_sh = p.dv_sh;
-    j.lengths = lengths; j.parts = parts; j.batch = batch; j.kv_heads = kv_heads; j.seqlen = seqlen;
-    const int64_t rows = 2 * (int64_t)batch * kv_heads * seqlen;
-    const int per_cta = 256 / (head_dim / 8);
-    const unsigned blocks = (unsigned)((rows + per_cta - 1) / per_cta);
-    if (head_dim == 128) attn_bwd_join_kernel<128><<<blocks, 256, 0, stream>>>(j);
-    else                 attn_bwd_join_kernel<64><<<blocks, 256, 0, stream>>>(j);
+  if (join) {
+    const JoinParams j = {p, n_t};
+    const int tiles = n_t * batch * kv_heads, most = kPartSlots * sms / 2;    // more of them are not cut
+    const unsigned blocks = (unsigned)(tiles < most ? tiles : most) * (unsigned)(head_dim / 8);
+    if (head_dim == 128 && lengths) attn_bwd_join_kernel<128, 2><<<blocks, 128, 0, stream>>>(j);
+    else if (head_dim == 128)       attn_bwd_join_kernel<128, 1><<<blocks, 128, 0, stream>>>(j);
+    else if (lengths)               attn_bwd_join_kernel<64, 2><<<blocks, 128, 0, stream>>>(j);
+    else                            attn_bwd_join_kernel<64, 1><<<blocks, 128, 0, stream>>>(j);
   }
   return msamp_check_launch("attention backward (shared heads)");
 }

@@ -42,6 +42,7 @@ _ARGTYPES = {
     'msamp_attention_tc_bwd': [_P] * 11 + [_I] * 4 + [_F, _I, _P],
     'msamp_attention_shared_fwd': [_P, _P],
     'msamp_attention_shared_bwd': [_P, _P],
+    'msamp_attention_shared_partial': [_I] * 7,
     'msamp_rotary': [_P, _P],
     'msamp_blocks_cast': [_P] * 4 + [_L, _I, _P],
     'msamp_blocks_uncast': [_P] * 4 + [_L, _I, _P],
@@ -85,6 +86,7 @@ def lib():
                 handle.msamp_last_error.restype = ctypes.c_char_p
                 for name, types in _ARGTYPES.items():
                     getattr(handle, name).argtypes = types
+                handle.msamp_attention_shared_partial.restype = _L
                 _lib = handle
     return _lib
 

@@ -429,7 +429,7 @@ def _shared_fwd(q, k, v, causal, scale, lengths):
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((B, nh, S), dtype=torch.float32)
     # with lengths: the tiles that are not padding, listed by the forward pass for both passes
-    plan = q.new_empty(1 + B * ((S + 127) // 128), dtype=torch.int32) if lengths is not None else None
+    plan = q.new_empty(2 + B * ((S + 127) // 128), dtype=torch.int32) if lengths is not None else None
     fields = _pack_sizes(B, nh, nkv, S, d, causal, scale) + _pack_st[4](*_map_strides(q), *_map_strides(k), *_map_strides(v),
                                                                         *_dense_strides(S, nh, d))
     with native.on_device(q):
@@ -442,11 +442,10 @@ def _shared_fwd(q, k, v, causal, scale, lengths):
     return o, lse, plan, fields
 
 
-def _shared_workspace(B, nh, nkv, S, d):
+def _shared_workspace(B, nh, nkv, S, d, causal, lengths):
     """Floats of the backward pass's workspace, and of its first part: delta, then the partial sums of dK and dV where there are several."""
-    parts = native.lib().msamp_attention_shared_parts(B, nh, nkv, S)
     first = (B * nh * S + 3) // 4 * 4
-    return first + (parts * 2 * B * nkv * S * d if parts > 1 else 0), first
+    return first + native.lib().msamp_attention_shared_partial(B, nh, nkv, S, d, causal, lengths is not None), first
 
 
 def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, work, grad_strides):
@@ -478,7 +477,7 @@ class _AttentionSharedFn(torch.autograd.Function):
             ctx.grad_strides = _pack_st[3](*_dense_strides(S, nh + 2 * nkv, d) * 3)
         else:
             ctx.grad_strides = _pack_st[3](*_dense_strides(S, nh, d), *_dense_strides(S, nkv, d) * 2)
-        ctx.work = _shared_workspace(B, nh, nkv, S, d)
+        ctx.work = _shared_workspace(B, nh, nkv, S, d, causal, lengths)
         ctx.args, ctx.places = (causal, scale), _places(q, k, v, o)
         return o
 
@@ -549,7 +548,7 @@ def attention_shared_bwd_raw(q, k, v, o, lse, plan, d_o, dq, dk, dv, causal=True
         o = _rows16(_mappable(o))
         B, S, nh, d = q.shape
         fields = _pack_sizes(B, nh, k.shape[2], S, d, bool(causal), float(scale)) + _pack_st[4](*(x for t in (q, k, v, o) for x in _map_strides(t)))
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, _shared_workspace(B, nh, k.shape[2], S, d),
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, _shared_workspace(B, nh, k.shape[2], S, d, bool(causal), lengths),
                     _pack_st[3](*(x for t in (dq, dk, dv) for x in _map_strides(t))))
         return
     with torch.enable_grad():
