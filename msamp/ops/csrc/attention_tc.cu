@@ -1640,25 +1640,26 @@ struct DeltaParams {
 
 // Bound by memory: one pass over O and dO.  D / 8 lanes read one row with 16-byte loads and rows are taken in the order of
 // their addresses ([batch, seq, head]), two per lane group, so that a warp keeps 2 KB of loads in flight.  A warp per row
-// in [batch, head, seq] order, 8 bytes a lane, took 50 us for 4 x 2048 x 32 heads of 128 (134 MB); this takes 35 us.
+// in [batch, head, seq] order, 8 bytes a lane, took 50 us for 4 x 2048 x 32 heads of 128 (134 MB); this takes 26.5 us.
 template <int D, bool LEN>
 __global__ void __launch_bounds__(256) attn_delta_tc_kernel(const DeltaParams p) {
   constexpr int L = D / 8;             // lanes of a row
   constexpr int ROWS = 256 / L;        // rows of a CTA and step
   const int sub = threadIdx.x % L;
-  const int64_t total = (int64_t)p.batch * p.heads * p.seqlen;
-  const int64_t r0 = (int64_t)blockIdx.x * (2 * ROWS) + threadIdx.x / L;
+  // rows and their parts in 32 bits (2^32 rows of a head would fill the memory several times): a 64-bit division for each of the three parts
+  // took 8 us more
+  const uint32_t heads = (uint32_t)p.heads, seqlen = (uint32_t)p.seqlen, total = (uint32_t)p.batch * heads * seqlen;
+  const uint32_t r0 = blockIdx.x * (uint32_t)(2 * ROWS) + threadIdx.x / L;
   Bytes16 a[2], g[2];
   int64_t out[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int64_t r = r0 + k * ROWS;
+    const uint32_t r = r0 + k * ROWS;
     a[k] = g[k] = Bytes16{};
     out[k] = -1;
     if (r < total) {
-      const int h = (int)(r % p.heads);
-      const int64_t bs = r / p.heads;
-      const int s = (int)(bs % p.seqlen), b = (int)(bs / p.seqlen);
+      const uint32_t bs = r / heads, b_ = bs / seqlen;
+      const int h = (int)(r - bs * heads), s = (int)(bs - b_ * seqlen), b = (int)b_;
       if (LEN && s >= __ldg(p.lengths + b)) {
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
         *reinterpret_cast<uint4*>(p.dq + (int64_t)b * p.dq_sb + (int64_t)s * p.dq_ss + (int64_t)h * p.dq_sh + sub * 8) = zero;
@@ -2999,7 +3000,9 @@ attn_bwd_dq_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           tc5::fence_after_sync();
           const float sum = mine + __uint_as_float(tc5::tmem_ld1(wg ? tdp - 32u : tdp + 96u));
           ndlt2 = f2_pack(-sum, -sum);
-          if (wg == 0 && in) p.delta[at] = sum;
+          int again = h;
+          asm volatile("" : "+r"(again));    // the address is worked out again, not held through the tiles of other items
+          if (wg == 0 && grow < len) p.delta[((int64_t)b * p.heads + again) * p.seqlen + grow] = sum;
         }
         uint32_t pk[32];
 #pragma unroll
@@ -3682,14 +3685,13 @@ __global__ void __launch_bounds__(256) attn_plan_kernel(const PlanParams p) {
       }
     }
   }
-  const int per_head = p.head_dim / 8, per_row = p.heads * per_head;
-  const int64_t todo = (int64_t)(p.seqlen - len) * per_row;
-  for (int64_t k = (int64_t)blockIdx.y * blockDim.x + threadIdx.x; k < todo; k += (int64_t)gridDim.y * blockDim.x) {
-    const int64_t row = k / per_row;
-    const int r = (int)(k - row * per_row), h = r / per_head, c = r - h * per_head;
-    const int64_t s = len + row;
-    *reinterpret_cast<uint4*>(p.o + b * p.o_sb + s * p.o_ss + h * p.o_sh + c * 8) = make_uint4(0u, 0u, 0u, 0u);
-    if (c == 0) p.lse[((int64_t)b * p.heads + h) * p.seqlen + s] = -INFINITY;
+  const int shift = p.head_dim == 128 ? 4 : 3, per_row = p.heads << shift;    // 16-byte vectors of a head, of a row
+  for (int s = len + (int)blockIdx.y; s < p.seqlen; s += gridDim.y) {
+    for (int k = threadIdx.x; k < per_row; k += blockDim.x) {
+      const int h = k >> shift, c = k - (h << shift);
+      *reinterpret_cast<uint4*>(p.o + b * p.o_sb + s * p.o_ss + h * p.o_sh + c * 8) = make_uint4(0u, 0u, 0u, 0u);
+      if (c == 0) p.lse[((int64_t)b * p.heads + h) * p.seqlen + s] = -INFINITY;
+    }
   }
 }
 
@@ -3952,6 +3954,7 @@ MSAMP_API int msamp_attention_tc_bwd(const void* q, const void* k, const void* v
     d.do_sb = strides[12]; d.do_ss = strides[13]; d.do_sh = strides[14];
     d.batch = batch; d.heads = heads; d.seqlen = seqlen;
     const int64_t rows = (int64_t)batch * heads * seqlen;
+    MSAMP_REQUIRE(rows < (1ll << 31), "attention: more than 2^31 rows");
     const int per_cta = 2 * 256 / (head_dim / 8);
     const unsigned blocks = (unsigned)((rows + per_cta - 1) / per_cta);
     if (head_dim == 128) attn_delta_tc_kernel<128, false><<<blocks, 256, 0, stream>>>(d);
@@ -4168,6 +4171,7 @@ MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) 
     d.dk = p.dk; d.dk_sb = p.dk_sb; d.dk_ss = p.dk_ss; d.dk_sh = p.dk_sh;
     d.dv = p.dv; d.dv_sb = p.dv_sb; d.dv_ss = p.dv_ss; d.dv_sh = p.dv_sh;
     const int64_t rows = (int64_t)batch * heads * seqlen;
+    MSAMP_REQUIRE(rows < (1ll << 31), "attention: more than 2^31 rows");
     const int per_cta = 2 * 256 / (head_dim / 8);
     const unsigned blocks = (unsigned)((rows + per_cta - 1) / per_cta);
     if (head_dim == 128 && lengths) attn_delta_tc_kernel<128, true><<<blocks, 256, 0, stream>>>(d);
