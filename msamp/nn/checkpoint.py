@@ -18,11 +18,10 @@ class _CheckpointFp8Fn(torch.autograd.Function):
         ctx.rng = None
         if preserve_rng_state:
             ctx.rng = (torch.get_rng_state(), torch.cuda.get_rng_state(x.device) if x.is_cuda else None)
+        ctx.save_for_backward(*_c.cast_blocks_to_fp8(x))    # before the function, which may change x
         with torch.no_grad():
             out = function(x, *args)
-        ctx.single = isinstance(out, torch.Tensor)
-        ctx.save_for_backward(*_c.cast_blocks_to_fp8(x))
-        return out if ctx.single else tuple(out)
+        return out if isinstance(out, torch.Tensor) else tuple(out)
 
     @staticmethod
     def backward(ctx, *grads):
@@ -37,7 +36,7 @@ class _CheckpointFp8Fn(torch.autograd.Function):
                     torch.cuda.set_rng_state(ctx.rng[1], ctx.device)
             with torch.enable_grad(), torch.autocast(ctx.device.type, enabled=enabled, dtype=dtype, cache_enabled=cache):
                 out = _outputs(ctx.function(x, *ctx.args))
-        pairs = [(o, g) for o, g in zip(out, grads) if g is not None and o.requires_grad]
+        pairs = [(o, g) for o, g in zip(out, grads) if g is not None and isinstance(o, torch.Tensor) and o.requires_grad]
         if pairs:
             torch.autograd.backward([o for o, _ in pairs], [g for _, g in pairs])
         return None, None, None, None, x.grad

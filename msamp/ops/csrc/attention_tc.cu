@@ -3622,8 +3622,8 @@ __global__ void __launch_bounds__(128) attn_bwd_join_kernel(const JoinParams j) 
 // 2 x 1000 x 12 / 4 of 64 in 1 and 3: 73 and 54 (3); 2 x 2048 x 16 / 4 of 128 in 1, 2 and 4: 204, 156 and 169 (2); 4 x 2048 x 32 / 8 of 128
 // in 1, 2 and 4: 499, 542 and 579 (1); 2 x 2048 x 16 / 4 of 128, not causal: 247, 261 and 278 (1).
 constexpr int kPartSlots = 3;    // items in parts at most, for each SM (their workspace is 128 KB each at head size 128)
-__host__ __device__ __forceinline__ int choose_parts(int rep, int64_t items, int64_t units, int longest, int head_dim, int sms, bool one_size) {
-  const float mean = (float)units / (float)sms;
+__host__ __device__ __forceinline__ int choose_parts(int rep, int64_t items, float units, int longest, int head_dim, int sms, bool one_size) {
+  const float mean = units / (float)sms;
   int best = 1;
   float least = 0.0f;
   for (int n = 1; n <= rep; ++n) {
@@ -3640,57 +3640,86 @@ __host__ __device__ __forceinline__ int choose_parts(int rep, int64_t items, int
 }
 
 // Row lengths of a padded batch: the list of 128-row tiles that hold rows of a sequence, longest work first, and zeros (lse: -inf) for the
-// output rows of padding.  plan[0]: number of tiles; plan[1]: parts (choose_parts); plan[2 + rank]: b * n_tiles + i for tile i of batch b.  The work of tile i is i + 1 tiles
-// when causal, else those of its row; ties go by batch, then by tile.  A tile counts the tiles in front of it, O(batch) each, so that no
-// sort and no atomic is needed.  blockIdx.x: batch, blockIdx.y: share of its padding.
+// output rows of padding.  plan[0]: number of tiles; plan[1]: parts (choose_parts); plan[2 + rank]: b * n_tiles + i for tile i of batch b; then
+// n_tiles words of scratch.  The work of tile i is i + 1 tiles when causal, else those of its row; ties go by batch, then by tile.
+// CTA 0 makes the list by counting: a warp takes one amount of work at a time, counts the batches that have it (ballots, in order, so that
+// nothing depends on timing), and after a scan over the amounts goes over them once more to place their tiles.  The other CTAs clear
+// padding, `share` of them for a batch.
 struct PlanParams {
   const int* lengths;
   int* plan;
   __nv_bfloat16* o;
   float* lse;
   int64_t o_sb, o_ss, o_sh;
-  int batch, heads, kv_heads, seqlen, head_dim, n_tiles, causal, sms;
+  int batch, heads, kv_heads, seqlen, head_dim, n_tiles, causal, sms, share;
 };
-__global__ void __launch_bounds__(256) attn_plan_kernel(const PlanParams p) {
-  const int b = blockIdx.x;
-  const int len = row_length(p.lengths, b, p.seqlen), n = (len + 127) / 128;
-  if (blockIdx.y == 0) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      int rank = p.causal ? 0 : i;
-      for (int c = 0; c < p.batch; ++c) {
-        const int m = (row_length(p.lengths, c, p.seqlen) + 127) / 128;
-        if (p.causal) rank += max(0, m - i - 1) + (c < b && m > i ? 1 : 0);
-        else          rank += m > n || (m == n && c < b) ? m : 0;
+constexpr int kPlanThreads = 512;
+__global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PlanParams p) {
+  if (blockIdx.x > 0) {
+    const int b = (int)(blockIdx.x - 1) / p.share, first = (int)(blockIdx.x - 1) - b * p.share;
+    const int shift = p.head_dim == 128 ? 4 : 3, per_row = p.heads << shift;    // 16-byte vectors of a head, of a row
+    for (int s = row_length(p.lengths, b, p.seqlen) + first; s < p.seqlen; s += p.share) {
+      for (int k = threadIdx.x; k < per_row; k += blockDim.x) {
+        const int h = k >> shift, c = k - (h << shift);
+        *reinterpret_cast<uint4*>(p.o + b * p.o_sb + s * p.o_ss + h * p.o_sh + c * 8) = make_uint4(0u, 0u, 0u, 0u);
+        if (c == 0) p.lse[((int64_t)b * p.heads + h) * p.seqlen + s] = -INFINITY;
       }
-      p.plan[2 + rank] = b * p.n_tiles + i;
     }
-    if (b == 0) {
-      __shared__ int s_total, s_longest;
-      __shared__ unsigned long long s_units;
-      if (threadIdx.x == 0) {
-        s_total = s_longest = 0;
-        s_units = 0;
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* start = p.plan + 2 + (int64_t)p.batch * p.n_tiles;
+  // the batches b0 .. b0 + 31 that have tiles of lv + 1 tiles of work: one such tile each when causal, else all their lv + 1
+  auto have = [&](int lv, int b0) {
+    const int b = b0 + lane;
+    const int m = b < p.batch ? (row_length(p.lengths, b, p.seqlen) + 127) / 128 : 0;
+    return __ballot_sync(0xffffffffu, p.causal ? m > lv : m == lv + 1);
+  };
+  for (int lv = warp; lv < p.n_tiles; lv += kPlanThreads / 32) {
+    int n = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) n += __popc(have(lv, b0));
+    if (lane == 0) start[lv] = p.causal ? n : n * (lv + 1);
+  }
+  __syncthreads();
+  if (warp == 0) {    // from the most work down: how many tiles come before; units and the longest row on the way
+    int total = 0, longest = 0;
+    float units = 0.0f;
+    for (int top = p.n_tiles - 1; top >= 0; top -= 32) {
+      const int lv = top - lane;
+      const int n = lv >= 0 ? start[lv] : 0;
+      int sum = n;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
       }
-      __syncthreads();
-      for (int c = threadIdx.x; c < p.batch; c += blockDim.x) {
-        const int m = (row_length(p.lengths, c, p.seqlen) + 127) / 128;
-        atomicAdd(&s_total, m);
-        atomicMax(&s_longest, m);
-        atomicAdd(&s_units, (unsigned long long)(p.causal ? (int64_t)m * (m + 1) / 2 : (int64_t)m * m) * p.heads);
-      }
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        p.plan[0] = s_total;
-        p.plan[1] = choose_parts(p.heads / p.kv_heads, (int64_t)s_total * p.kv_heads, (int64_t)s_units, s_longest, p.head_dim, p.sms, false);
-      }
+      if (lv >= 0) start[lv] = total + sum - n;
+      total += __shfl_sync(0xffffffffu, sum, 31);
+      if (n > 0) longest = max(longest, lv + 1);
+      units += (float)n * (float)(lv + 1);
+    }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    units = warp_sum(units);
+    if (lane == 0) {
+      p.plan[0] = total;
+      p.plan[1] = choose_parts(p.heads / p.kv_heads, (int64_t)total * p.kv_heads, units * (float)p.heads, longest, p.head_dim, p.sms, false);
     }
   }
-  const int shift = p.head_dim == 128 ? 4 : 3, per_row = p.heads << shift;    // 16-byte vectors of a head, of a row
-  for (int s = len + (int)blockIdx.y; s < p.seqlen; s += gridDim.y) {
-    for (int k = threadIdx.x; k < per_row; k += blockDim.x) {
-      const int h = k >> shift, c = k - (h << shift);
-      *reinterpret_cast<uint4*>(p.o + b * p.o_sb + s * p.o_ss + h * p.o_sh + c * 8) = make_uint4(0u, 0u, 0u, 0u);
-      if (c == 0) p.lse[((int64_t)b * p.heads + h) * p.seqlen + s] = -INFINITY;
+  __syncthreads();
+  for (int lv = warp; lv < p.n_tiles; lv += kPlanThreads / 32) {
+    int* dst = p.plan + 2 + start[lv];
+    const int each = p.causal ? 1 : lv + 1;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      const uint32_t mask = have(lv, b0);
+      if (mask >> lane & 1u) {
+        int* d = dst + __popc(mask & ((1u << lane) - 1u)) * each;
+        const int code = (b0 + lane) * p.n_tiles;
+        if (p.causal) {
+          *d = code + lv;
+        } else {
+          for (int i = 0; i < each; ++i) d[i] = code + i;
+        }
+      }
+      dst += __popc(mask) * each;
     }
   }
 }
@@ -4000,7 +4029,7 @@ MSAMP_API int msamp_attention_tc_bwd(const void* q, const void* k, const void* v
 // ---- shared key / value heads and row lengths ----------------------------------------------------
 // Query heads h * rep .. h * rep + rep - 1 read key / value head h (heads == kv_heads * rep).  lengths [batch] (int32, or null): positions at or
 // behind a row's length are padding, as queries and as keys; their outputs and gradients are zero, their lse -inf, whatever they hold.  With
-// lengths the forward pass writes `plan` (2 + batch * ceil(seqlen / 128) ints), which the backward pass of the same lengths reads.
+// lengths the forward pass writes `plan` (2 + (batch + 1) * ceil(seqlen / 128) ints), which the backward pass of the same lengths reads.
 // Strides as for the entry points above, those of k, v, dk and dv over kv_heads.
 static int shared_checks(int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, const int* lengths, const int* plan,
                          const int64_t* strides, int n) {
@@ -4095,9 +4124,9 @@ MSAMP_API int msamp_attention_shared_fwd(const SharedFwdArgs* a, void* stream_) 
   const int ctas = n_items < sms ? n_items : sms;
   cudaStream_t stream = (cudaStream_t)stream_;
   if (lengths) {
-    PlanParams w = {lengths, plan, p.o, lse, p.o_sb, p.o_ss, p.o_sh, batch, heads, kv_heads, seqlen, head_dim, n_qt, causal, sms};
-    const int share = (4 * sms + batch - 1) / batch;
-    attn_plan_kernel<<<dim3((unsigned)batch, (unsigned)(share < 64 ? share : 64)), 256, 0, stream>>>(w);
+    const int share = 2 * sms / batch < 1 ? 1 : 2 * sms / batch < 64 ? 2 * sms / batch : 64;
+    const PlanParams w = {lengths, plan, p.o, lse, p.o_sb, p.o_ss, p.o_sh, batch, heads, kv_heads, seqlen, head_dim, n_qt, causal, sms, share};
+    attn_plan_kernel<<<(unsigned)batch * (unsigned)share + 1, kPlanThreads, 0, stream>>>(w);
     rc = head_dim == 128 ? launch_fwd<128, 2>(m, p, n_qt, ctas, stream) : launch_fwd<64, 2>(m, p, n_qt, ctas, stream);
   } else {
     rc = head_dim == 128 ? launch_fwd<128, 1>(m, p, n_qt, ctas, stream) : launch_fwd<64, 1>(m, p, n_qt, ctas, stream);
@@ -4108,7 +4137,7 @@ MSAMP_API int msamp_attention_shared_fwd(const SharedFwdArgs* a, void* stream_) 
 // Parts of dK / dV without lengths.
 static int uniform_parts(int batch, int heads, int kv_heads, int seqlen, int head_dim, int causal) {
   const int64_t n = (seqlen + 127) / 128, items = n * batch * kv_heads;
-  return choose_parts(heads / kv_heads, items, (causal ? n * (n + 1) / 2 : n * n) * batch * heads, (int)n, head_dim, msamp_sm_count(),
+  return choose_parts(heads / kv_heads, items, (float)((causal ? n * (n + 1) / 2 : n * n) * batch * heads), (int)n, head_dim, msamp_sm_count(),
                       !causal);
 }
 // Floats of the workspace `partial` (0: none).  With lengths the parts are chosen on the device, up to kPartSlots items for each SM.

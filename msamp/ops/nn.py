@@ -232,7 +232,8 @@ def gelu(x, keep_fp8=False):
     if keep_fp8:
         if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise TypeError(f'gelu: unsupported dtype {x.dtype}')
-        return _GeluKeepFn.apply(x)
+        if (torch.is_grad_enabled() and x.requires_grad) or (x.is_cuda and x.data_ptr() % 16):
+            return _GeluKeepFn.apply(x)
     if _use_native(x):
         return _GeluFn.apply(x)
     return F.gelu(x.float(), approximate='tanh').to(x.dtype)
@@ -429,7 +430,7 @@ def _shared_fwd(q, k, v, causal, scale, lengths):
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((B, nh, S), dtype=torch.float32)
     # with lengths: the tiles that are not padding, listed by the forward pass for both passes
-    plan = q.new_empty(2 + B * ((S + 127) // 128), dtype=torch.int32) if lengths is not None else None
+    plan = q.new_empty(2 + (B + 1) * ((S + 127) // 128), dtype=torch.int32) if lengths is not None else None
     fields = _pack_sizes(B, nh, nkv, S, d, causal, scale) + _pack_st[4](*_map_strides(q), *_map_strides(k), *_map_strides(v),
                                                                         *_dense_strides(S, nh, d))
     with native.on_device(q):
@@ -506,13 +507,11 @@ def _places(*ts):
 def _attention_plain(q, k, v, causal, scale, lengths):
     """The same in torch operations on any device (the CPU form)."""
     B, S, nh, d = q.shape
-    nkv = k.shape[2]
     if lengths is not None:
         valid = torch.arange(S, device=q.device) < lengths.to(q.device)[:, None]
         q, k, v = (torch.where(valid[:, :, None, None], t, torch.zeros((), dtype=t.dtype, device=t.device)) for t in (q, k, v))
     qf, kf, vf = (t.float().permute(0, 2, 1, 3) for t in (q, k, v))
-    if nkv != nh:
-        kf, vf = (t.repeat_interleave(nh // nkv, dim=1) for t in (kf, vf))
+    kf, vf = (t if t.shape[1] == nh else t.repeat_interleave(nh // t.shape[1], dim=1) for t in (kf, vf))
     s = (qf @ kf.transpose(-1, -2)) * scale
     if causal:
         s = s.masked_fill(torch.ones(S, S, dtype=torch.bool, device=q.device).triu(1), float('-inf'))
@@ -615,7 +614,7 @@ def attention(q, k, v, causal=True, scale=None, grad_layout='separate', lengths=
     """
     d = q.shape[-1]
     scale = 1.0 / math.sqrt(d) if scale is None else scale
-    if lengths is not None or k.shape != q.shape:
+    if lengths is not None or (q.dim() == k.dim() == 4 and k.shape[2] != q.shape[2] and (q.is_cuda or k.shape[:2] == q.shape[:2])):
         return _attention_shared(q, k, v, causal, scale, grad_layout, lengths)
     if _use_native(q):
         if q.dtype != torch.bfloat16 or d not in (64, 128):

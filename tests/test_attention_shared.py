@@ -111,7 +111,7 @@ def test_shared_heads(device, d, causal, S, nh, nkv):
 @pytest.mark.parametrize('d', [64, 128])
 @pytest.mark.parametrize('junk', [0.0, float('nan'), float('inf'), torch.finfo(torch.bfloat16).min])
 @pytest.mark.parametrize('S, nh, nkv, lengths', [(130, 4, 2, (130, 0, 1, 129, 128, 127)), (300, 2, 2, (5, 300, 256, 255, 257, -3)),
-                                                 (7, 6, 1, (0, 0, 3)), (520, 2, 1, (1000, 385, 130))])
+                                                 (7, 6, 1, (0, 0, 3)), (7, 2, 1, (0, 0)), (520, 2, 1, (1000, 385, 130))])
 def test_lengths(device, d, causal, junk, S, nh, nkv, lengths):
     q, k, v, do = _inputs(len(lengths), S, nh, nkv, d, device)
     n = torch.tensor(lengths, device=device, dtype=torch.int32 if S % 2 else torch.int64)
@@ -125,7 +125,7 @@ def test_lengths(device, d, causal, junk, S, nh, nkv, lengths):
 @pytest.mark.gpu
 @pytest.mark.parametrize('d', [64, 128])
 @pytest.mark.parametrize('B, S, nh, nkv, ragged', [(1, 2048, 8, 1, False), (4, 1000, 24, 8, True), (40, 200, 12, 4, True), (3, 700, 36, 12, False),
-                                                   (2, 1500, 96, 96, True), (300, 10, 4, 2, True)])
+                                                   (2, 1500, 96, 96, True), (300, 10, 4, 2, True), (3000, 20, 2, 1, True)])
 def test_many_work_items(d, B, S, nh, nkv, ragged):
     """Several waves of items, items in parts, rows of every length in one batch."""
     q, k, v, do = _inputs(B, S, nh, nkv, d, 'cuda')
@@ -139,6 +139,25 @@ def test_many_work_items(d, B, S, nh, nkv, ragged):
             _compare([got[0][one, :, qs], got[1][one, :, qs], got[2][one, :, h:h + 1], got[3][one, :, h:h + 1]], want, valid)
     again = _run(q, k, v, do, True, n)
     assert all(torch.equal(a, b) for a, b in zip(got, again))    # no atomics: the same bits
+    _status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('B, S', [(1, 1), (1, 5000), (7, 700), (33, 300), (100, 129), (2000, 130), (70000, 3)])
+def test_list_of_tiles(B, S, causal):
+    """The tiles that hold rows of a sequence, each once, by falling work, then by batch and tile."""
+    n = torch.randint(-2, S + 3, (B, ), generator=torch.Generator().manual_seed(B))
+    q = torch.zeros(B, S, 2, 64, device='cuda', dtype=torch.bfloat16)
+    o, lse, plan = K.attention_shared_fwd_raw(q, q[:, :, :1], q[:, :, :1], causal, lengths=n.cuda())
+    tiles, want = (S + 127) // 128, []
+    for b, m in enumerate(((n.clamp(0, S) + 127) // 128).tolist()):
+        want += [(-(i + 1 if causal else m), b, i) for i in range(m)]
+    want = [b * tiles + i for _, b, i in sorted(want)]
+    plan = plan.tolist()
+    assert plan[0] == len(want) and plan[1] in (1, 2) and plan[2:2 + len(want)] == want
+    pad = (torch.arange(S) >= n[:, None]).cuda()
+    assert torch.equal(torch.isinf(lse).all(1), pad) and not o.any()
     _status_ok()
 
 
@@ -241,6 +260,37 @@ def test_empty(device):
         assert o.shape == q.shape and q.grad.shape == q.shape
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('lengths', [None, (200, 90)])
+def test_saved_tensors_in_other_layouts(d, lengths):
+    """What saved-tensor hooks bring back may lie anywhere: other strides, off the 16-byte grid, via the host."""
+    q, k, v, do = _inputs(2, 200, 4, 2, d, 'cuda')
+    n = None if lengths is None else torch.tensor(lengths, device='cuda')
+    want = _run(q, k, v, do, True, n)
+
+    def turned(t):
+        return t.transpose(0, t.dim() - 1).contiguous().transpose(0, t.dim() - 1) if t.dim() == 4 else t
+
+    def shifted(t):
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape).copy_(t) if t.dim() == 4 else t
+
+    for unpack in (turned, shifted, lambda t: t.cpu().cuda()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
+            got = _run(q, k, v, do, True, n)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    _status_ok()
+
+
+def test_other_numbers_of_keys_on_the_cpu():
+    """Equal heads, more keys than queries: what attention on the CPU has always taken."""
+    torch.manual_seed(0)
+    q, k, v = torch.randn(2, 3, 4, 8), torch.randn(2, 5, 4, 8), torch.randn(2, 5, 4, 8)
+    x = torch.einsum('bihd,bjhd->bhij', q, k) / 8**0.5
+    want = torch.einsum('bhij,bjhd->bihd', torch.softmax(x, -1), v)
+    assert torch.allclose(K.attention(q, k, v, causal=False), want, rtol=1e-5, atol=1e-6)
+
+
 def test_gradients_against_differences():
     """The CPU form in 32 bits, central differences of sum(o * do) in random directions."""
     torch.manual_seed(0)
@@ -262,11 +312,11 @@ def test_gradients_against_differences():
 def test_refusals():
     q, k = torch.randn(2, 3, 4, 8), torch.randn(2, 3, 2, 8)
     n = torch.tensor([3, 2])
-    for bad in (lambda: K.attention(q, k, k[:, :, :1]), lambda: K.attention(q, k[:, :2], k[:, :2]), lambda: K.attention(q, q[:, :, :3], q[:, :, :3]),
+    for bad in (lambda: K.attention(q, k, k[:, :, :1]), lambda: K.attention(q, k[:, :2], k[:, :2], lengths=n), lambda: K.attention(q, q[:, :, :3], q[:, :, :3]),
                 lambda: K.attention(q, k[..., :4], k[..., :4]), lambda: K.attention(q, k.half(), k), lambda: K.attention(q, k[:, :, :0], k[:, :, :0]),
                 lambda: K.attention(q, k, k, lengths=n[:1]), lambda: K.attention(q, k, k, lengths=n.float()),
                 lambda: K.attention(q, k, k, lengths=n.to('meta')), lambda: K.attention(q, k, k, scale=0.0),
-                lambda: K.attention(q, k, k, scale=float('nan')), lambda: K.attention(q, k, k, scale=float('inf')), lambda: K.attention(q[0], k, k)):
+                lambda: K.attention(q, k, k, scale=float('nan')), lambda: K.attention(q, k, k, scale=float('inf')), lambda: K.attention(q[0], k, k, lengths=n)):
         with pytest.raises(ValueError):
             bad()
 

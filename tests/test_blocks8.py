@@ -178,6 +178,19 @@ def test_gelu_views_and_gradient_layouts():
     assert torch.equal(gu, gv)
 
 
+@pytest.mark.parametrize('device', CPU_GPU)
+def test_gelu_without_gradients_keeps_nothing(device):
+    x = torch.randn(65, 31, device=device).to(torch.bfloat16 if device == 'cuda' else torch.float32).requires_grad_(True)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t) or t, lambda t: t):
+        K.gelu(x.detach(), keep_fp8=True)
+        with torch.no_grad():
+            y = K.gelu(x, keep_fp8=True)
+    assert not seen and torch.equal(y, K.gelu(x.detach()))
+    z = K.gelu(x.detach().flatten()[1:], keep_fp8=True)    # off the 16-byte grid
+    assert torch.equal(z, K.gelu(x.detach().flatten()[1:].clone()))
+
+
 def test_refusals():
     c, e = cast.cast_blocks_to_fp8(torch.randn(70))
     for bad in (lambda: cast.cast_blocks_to_fp8(torch.zeros(3, dtype=torch.float64)), lambda: cast.cast_blocks_to_fp8(torch.zeros(3, dtype=torch.int32)),
@@ -233,6 +246,15 @@ def test_checkpoint_dropout_tuple_and_frozen_input():
     assert torch.allclose(lin.weight.grad, 2 * (kept * 2.0).t() @ x) and x.grad is None
     with torch.no_grad():
         assert not checkpoint_fp8(f, x)[0].requires_grad
+
+
+def test_checkpoint_of_a_function_that_changes_its_input_and_returns_none():
+    x = torch.ones(4, 32, requires_grad=True)
+    lin = torch.nn.Linear(32, 32, bias=False)
+    y, nothing = checkpoint_fp8(lambda t: (lin(t.mul_(2.0) if not t.requires_grad else t * 2.0), None), x * 1.0)
+    y.sum().backward()
+    assert nothing is None
+    assert torch.equal(lin.weight.grad, torch.full((32, 32), 8.0)) and torch.allclose(x.grad, 2 * lin.weight.sum(0).expand(4, 32))
 
 
 def test_checkpoint_keeps_one_byte_per_element():
