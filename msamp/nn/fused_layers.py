@@ -142,20 +142,28 @@ class _MlpSublayerFn(torch.autograd.Function):
         w1_8, w1_sinv = weight_fp8(w1)
         w2_8, w2_sinv = weight_fp8(w2)
         g_meta = m2['input']
+        # the widest activation: the GeLU input h, two bytes an element for the backward pass, or 1.03 as e4m3 blocks, which the epilogue of
+        # the fc1 GEMM writes (where its rows are whole blocks) and the epilogue of the fc2 dgrad GEMM reads
+        kept, in_epilogue = None, w1_8.shape[0] % 32 == 0
+        if keep_fp8 and in_epilogue:
+            n = x.shape[0] * w1_8.shape[0]
+            kept = (torch.empty((x.shape[0], w1_8.shape[0]), dtype=torch.uint8, device=x.device),
+                    torch.empty(n // 32, dtype=torch.uint8, device=x.device))
         if g_meta.is_in_time_scaling():
             # fc1 epilogue reduces max|gelu(h)|; the quantising pass applies GeLU and the scale that amax implies
-            h = _g.gemm_fp8(y8, E4M3, y_sinv, w1_8, E4M3, w1_sinv, dt, bias=b1, amax_out=g_meta.amax[0], act='gelu')
+            h = _g.gemm_fp8(y8, E4M3, y_sinv, w1_8, E4M3, w1_sinv, dt, bias=b1, amax_out=g_meta.amax[0], act='gelu', keep_blocks=kept)
             g8, g_sinv = _quantize(h, g_meta, E4M3, act='gelu', amax_hint=g_meta.amax[0])
         else:
             # the scale is known: the fc1 epilogue writes gelu(h) as e4m3 next to h and records its amax
             g8 = torch.empty((x.shape[0], w1_8.shape[0]), dtype=torch.uint8, device=x.device)
             h = _g.gemm_fp8(y8, E4M3, y_sinv, w1_8, E4M3, w1_sinv, dt, bias=b1, amax_out=g_meta.amax[0], act='gelu', out8=g8,
-                            out8_qtype=E4M3, out8_scale=g_meta.scale, out8_scale_inv_out=g_meta.scale_inv)
+                            out8_qtype=E4M3, out8_scale=g_meta.scale, out8_scale_inv_out=g_meta.scale_inv, keep_blocks=kept,
+                            store_out=kept is None)
             g_sinv = g_meta.scale_inv.clone()
         out = _g.gemm_fp8(g8, E4M3, g_sinv, w2_8, E4M3, w2_sinv, dt, bias=b2, residual=x if add_residual else None)
         ctx.add_residual = add_residual
-        # the widest activation: the GeLU input, two bytes an element, or 1.03 as e4m3 blocks
-        kept = _k.cast_blocks_to_fp8(h) if keep_fp8 else (h, None)
+        if kept is None:
+            kept = _k.cast_blocks_to_fp8(h) if keep_fp8 else (h, None)
         ctx.save_for_backward(x, ln_weight, mean, rstd, y8, y_sinv, *kept, g8, g_sinv, w1_8, w1_sinv, w2_8, w2_sinv)
         ctx.w1, ctx.m1, ctx.w2, ctx.m2 = w1, m1, w2, m2
         ctx.has_ln_bias = ln_bias is not None
@@ -168,8 +176,9 @@ class _MlpSublayerFn(torch.autograd.Function):
         x, ln_weight, mean, rstd, y8, y_sinv, h, h_exp, g8, g_sinv, w1_8, w1_sinv, w2_8, w2_sinv = ctx.saved_tensors
         m1, m2 = ctx.m1, ctx.m2
         dt = x.dtype
+        gelu_in = dict(gelu_src=h)
         if h_exp is not None:
-            h = _k.cast_blocks_from_fp8(h, h_exp, dt)
+            gelu_in = dict(gelu_blocks=(h, h_exp)) if h.shape[1] % 32 == 0 else dict(gelu_src=_k.cast_blocks_from_fp8(h, h_exp, dt))
         g = g.contiguous()
         # fc2
         dy8, dy_sinv, db2 = _quantize_ograd(g, m2['ograd'], ctx.b2_dtype is not None, ctx.b2_dtype)
@@ -180,7 +189,7 @@ class _MlpSublayerFn(torch.autograd.Function):
             # in-time scaling: the scale of dh follows from its amax, which the epilogue reduces on the way; the
             # quantisation (and the bias gradient) is a second pass over dh
             dh_amax = torch.empty((), dtype=torch.float32, device=x.device)
-            dh = gemm_dgrad(dy8, dy_sinv, w2_8, w2_sinv, dt, gelu_src=h, amax_out=dh_amax)
+            dh = gemm_dgrad(dy8, dy_sinv, w2_8, w2_sinv, dt, amax_out=dh_amax, **gelu_in)
             setattr(dh, _AMAX_HINT, dh_amax)
             dh8, dh_sinv, db1 = _quantize_ograd(dh, og, ctx.b1_dtype is not None, ctx.b1_dtype)
             del dh
@@ -189,8 +198,8 @@ class _MlpSublayerFn(torch.autograd.Function):
             # the amax for the history and the column sums (= the bias gradient of fc1) itself; dh in bf16 is never stored
             dh8 = torch.empty((dy8.shape[0], h.shape[1]), dtype=torch.uint8, device=x.device)
             colsum = torch.empty(h.shape[1], dtype=torch.float32, device=x.device) if ctx.b1_dtype is not None else None
-            gemm_dgrad(dy8, dy_sinv, w2_8, w2_sinv, dt, gelu_src=h, amax_out=og.amax[0], out8=dh8, out8_qtype=E5M2, out8_scale=og.scale,
-                       out8_scale_inv_out=og.scale_inv, colsum_out=colsum, store_out=False)
+            gemm_dgrad(dy8, dy_sinv, w2_8, w2_sinv, dt, amax_out=og.amax[0], out8=dh8, out8_qtype=E5M2, out8_scale=og.scale,
+                       out8_scale_inv_out=og.scale_inv, colsum_out=colsum, store_out=False, **gelu_in)
             dh_sinv = og.scale_inv.clone()
             db1 = colsum.to(ctx.b1_dtype) if colsum is not None else None
         # fc1

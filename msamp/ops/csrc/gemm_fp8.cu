@@ -22,6 +22,7 @@
 //
 // Replaces the cuBLASLt call behind the reference's Gemm.fp8_gemm (msamp/operators/gemm/gemm.py:121-144)
 // and the fp8 transposes around it (msamp/nn/functional.py:81-103).
+#include "blocks8.cuh"
 #include "gemm_common.cuh"
 
 namespace {
@@ -56,6 +57,11 @@ struct GemmArgs {
   int tma_store;              // 1: tma_d describes D and full 16-bit tiles are stored through it
   float* colsum;              // optional [N] fp32: += column sums of D as stored (a bias gradient); zeroed by the caller
   int no_d;                   // 1: D itself is not written (only amax_out / d8 / colsum are wanted)
+  // kernels with KEEP: [M, N] in e4m3 blocks of 32 columns (see blocks8.cuh), dense, N a multiple of 32
+  const uint8_t* g_codes;     // in the place of gelu_src
+  const uint8_t* g_exps;
+  uint8_t* k_codes;           // receive D as stored
+  uint8_t* k_exps;
 };
 
 template <int BN, bool PAIR, int NSTAGES = 0>
@@ -115,7 +121,63 @@ __device__ __forceinline__ void colsum_chunk(float* cs, const float (&v)[32], in
     if (j < valid) atomicAdd(cs + j, to_f32<OutT>(from_f32<OutT>(v[j])));
 }
 
-template <int BN, bool PAIR, typename OutT, int NSTAGES = 0>
+// A thread of the epilogue holds 32 columns of a row, which is one block: its values' largest magnitude needs no exchange.
+template <typename OutT>
+__device__ __forceinline__ void keep_block(uint8_t* codes, uint8_t* exp, const float (&v)[32]) {
+  using namespace blocks8;
+  float w[32];
+  uint32_t a = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    w[j] = to_f32<OutT>(from_f32<OutT>(v[j]));
+    a = max(a, __float_as_uint(w[j]) & 0x7fffffffu);
+  }
+  if (a >= 0x7f800000u) {
+    a = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      a = max(a, finite_bits(w[j]));
+      w[j] = inf_to_nan(w[j]);
+    }
+  }
+  const int k = block_shift(a);
+  const float s = __uint_as_float((uint32_t)(k + 127) << 23);
+#pragma unroll
+  for (int j = 0; j < 32; j += 16) {
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* x = &w[j + 4 * i];
+      c[i] = (uint32_t)f32x2_to_fp8x2<FMT_E4M3>(mul_keep(x[0], s), mul_keep(x[1], s)) |
+             (uint32_t)f32x2_to_fp8x2<FMT_E4M3>(mul_keep(x[2], s), mul_keep(x[3], s)) << 16;
+    }
+    *reinterpret_cast<uint4*>(codes + j) = make_uint4(c[0], c[1], c[2], c[3]);
+  }
+  *exp = (uint8_t)(127 - k);
+}
+template <typename OutT>
+__device__ __forceinline__ void kept_block(const uint8_t* codes, uint32_t exp, float (&h)[32]) {
+  using namespace blocks8;
+  const float unit = block_unit(exp);
+#pragma unroll
+  for (int j = 0; j < 32; j += 16) {
+    const uint4 c = *reinterpret_cast<const uint4*>(codes + j);
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 4] >> (8 * (i & 2))), __NV_E4M3);
+      const float2 f = __half22float2(__half2(x));
+      h[j + i] = mul_keep(f.x, unit);
+      h[j + i + 1] = mul_keep(f.y, unit);
+    }
+  }
+  if (may_overflow<OutT>(exp)) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) h[j] = in_range<OutT>(h[j]);
+  }
+}
+
+template <int BN, bool PAIR, typename OutT, int NSTAGES = 0, bool KEEP = false>
 __global__ void __launch_bounds__(kThreadsEpi8, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                 const __grid_constant__ CUtensorMap tma_d, const GemmArgs p) {
@@ -333,6 +395,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
         for (int b = 0; b < cols_here * (int)sizeof(OutT); b += 128)
           asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(src) + b));
       }
+      if (KEEP && p.g_codes != nullptr && row < p.M) {
+        const int cols_here = (p.N - n0) < BN ? (p.N - n0) : BN;
+        for (int b = 0; b < cols_here; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.g_codes + (int64_t)row * p.N + n0 + b));
+      }
       if (!tc5::mbar_wait(tfull_bar(buf), aph, abort_flag, p.status, 1u)) break;
       tc5::fence_after_sync();
       const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN);
@@ -382,6 +448,16 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
             load_chunk<OutT>(G + (int64_t)row * p.ldg + col, h, vec_g, valid);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= gelu_grad_f(h[j]);
+          }
+          if constexpr (KEEP) {
+            const int64_t at = (int64_t)row * p.N + col;
+            if (p.g_codes != nullptr) {
+              float h[32];
+              kept_block<OutT>(p.g_codes + at, p.g_exps[at / 32], h);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] *= gelu_grad_f(h[j]);
+            }
+            if (p.k_codes != nullptr) keep_block<OutT>(p.k_codes + at, p.k_exps + at / 32, v);
           }
           OutT* dst = D + (int64_t)row * p.ldd + col;
           if constexpr (sizeof(OutT) == 2) {
@@ -485,7 +561,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
 }
 
 // Co-resident CTA pairs the device can hold for the pair kernel (one CTA per SM, clusters of two).
-template <int BN, typename OutT, int NSTAGES>
+template <int BN, typename OutT, int NSTAGES, bool KEEP>
 int max_pairs(int smem_bytes) {
   static int cached[64] = {0};
   int dev = 0;
@@ -504,7 +580,7 @@ int max_pairs(int smem_bytes) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_fp8_kernel<BN, true, OutT, NSTAGES>, &cfg) != cudaSuccess || n <= 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_fp8_kernel<BN, true, OutT, NSTAGES, KEEP>, &cfg) != cudaSuccess || n <= 0) {
       cudaGetLastError();
       n = msamp_sm_count() / 2;
     }
@@ -513,14 +589,14 @@ int max_pairs(int smem_bytes) {
   return cached[dev];
 }
 
-template <int BN, bool PAIR, typename OutT, int NSTAGES = 0>
+template <int BN, bool PAIR, typename OutT, int NSTAGES = 0, bool KEEP = false>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& md, const GemmArgs& p, int max_ctas, cudaStream_t stream) {
   using C = Tile<BN, PAIR, NSTAGES>;
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!configured[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_fp8_kernel<BN, PAIR, OutT, NSTAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    cudaError_t e = cudaFuncSetAttribute(gemm_fp8_kernel<BN, PAIR, OutT, NSTAGES, KEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     if (e != cudaSuccess) {
       msamp_set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       return MSAMP_ELAUNCH;
@@ -529,7 +605,7 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& md, 
   }
   const int num_tiles = ((p.M + C::TILE_M - 1) / C::TILE_M) * ((p.N + BN - 1) / BN);
   if (PAIR) {
-    int pairs = max_pairs<BN, OutT, NSTAGES>(C::SMEM_BYTES);
+    int pairs = max_pairs<BN, OutT, NSTAGES, KEEP>(C::SMEM_BYTES);
     if (max_ctas > 0 && max_ctas / 2 < pairs) pairs = max_ctas / 2 > 0 ? max_ctas / 2 : 1;
     if (num_tiles < pairs) pairs = num_tiles;
     cudaLaunchConfig_t cfg = {};
@@ -544,7 +620,7 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& md, 
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<BN, PAIR, OutT, NSTAGES>, ma, mb, md, p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_fp8_kernel<BN, PAIR, OutT, NSTAGES, KEEP>, ma, mb, md, p);
     if (e != cudaSuccess) {
       msamp_set_error("gemm_fp8 pair kernel launch: %s", cudaGetErrorString(e));
       cudaGetLastError();
@@ -555,7 +631,7 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& md, 
   int grid = msamp_sm_count();
   if (max_ctas > 0 && max_ctas < grid) grid = max_ctas;
   if (num_tiles < grid) grid = num_tiles;
-  gemm_fp8_kernel<BN, PAIR, OutT, NSTAGES><<<grid, kThreadsEpi8, C::SMEM_BYTES, stream>>>(ma, mb, md, p);
+  gemm_fp8_kernel<BN, PAIR, OutT, NSTAGES, KEEP><<<grid, kThreadsEpi8, C::SMEM_BYTES, stream>>>(ma, mb, md, p);
   return msamp_check_launch("gemm_fp8_kernel");
 }
 
@@ -589,6 +665,10 @@ struct MsampGemmDesc {
   int tile;
   unsigned long long* stats;    // optional tuning counters, 4 per CTA (see GemmArgs)
   float* colsum;                // optional [N] fp32, += column sums of D as stored; zeroed by the caller
+  const void* gelu_codes;       // optional: gelu_src as e4m3 blocks (codes [M, N] and exponents [M * N / 32]), N a multiple of 32
+  const void* gelu_exps;
+  void* keep_codes;             // optional: D as stored, as e4m3 blocks
+  void* keep_exps;
 };
 
 MSAMP_API int msamp_gemm_fp8_ex(const MsampGemmDesc* g, void* stream_) {
@@ -601,10 +681,17 @@ MSAMP_API int msamp_gemm_fp8_ex(const MsampGemmDesc* g, void* stream_) {
   MSAMP_REQUIRE((reinterpret_cast<uintptr_t>(g->a) & 15) == 0 && (reinterpret_cast<uintptr_t>(g->b) & 15) == 0,
                 "msamp_gemm_fp8: operands must be 16-byte aligned");
   MSAMP_REQUIRE(g->scale_inv_a && g->scale_inv_b, "msamp_gemm_fp8: null pointer");
-  MSAMP_REQUIRE(g->d != nullptr || g->d8 != nullptr || g->amax_out != nullptr || g->colsum != nullptr,
+  MSAMP_REQUIRE(g->d != nullptr || g->d8 != nullptr || g->amax_out != nullptr || g->colsum != nullptr || g->keep_codes != nullptr,
                 "msamp_gemm_fp8: no output requested");
   MSAMP_REQUIRE(g->d != nullptr || (g->residual == nullptr), "msamp_gemm_fp8: a residual needs the output it is added to");
   MSAMP_REQUIRE(g->d8 == nullptr || g->d8_scale != nullptr, "msamp_gemm_fp8: a quantised copy needs its scale");
+  const bool keep = g->gelu_codes != nullptr || g->keep_codes != nullptr;
+  if (keep) {
+    MSAMP_REQUIRE(N % 32 == 0, "msamp_gemm_fp8: e4m3 blocks need N to be a multiple of 32 (got %d)", N);
+    MSAMP_REQUIRE(!g->gelu_codes || (g->gelu_exps && !g->gelu_src), "msamp_gemm_fp8: GeLU source given twice or without exponents");
+    MSAMP_REQUIRE(!g->keep_codes || g->keep_exps, "msamp_gemm_fp8: e4m3 blocks without exponents");
+    MSAMP_REQUIRE(aligned16(g->gelu_codes) && aligned16(g->keep_codes), "msamp_gemm_fp8: e4m3 codes must be 16-byte aligned");
+  }
   const int sms = msamp_sm_count();
   // Tile choice.  Problems that fill the device with 256-wide tiles run on the CTA-pair kernel (256x256 tiles over two
   // SMs): it moves a third less data per FLOP through L2 and shared memory, and since the MMA issue loop stopped
@@ -648,6 +735,8 @@ MSAMP_API int msamp_gemm_fp8_ex(const MsampGemmDesc* g, void* stream_) {
   p.stats = g->stats;
   p.ldd = g->ldd; p.ldr = g->ldr; p.ldg = g->ldg; p.ld8 = g->ld8;
   p.M = M; p.N = N; p.K = K; p.bias_dtype = g->bias_dtype;
+  p.g_codes = (const uint8_t*)g->gelu_codes; p.g_exps = (const uint8_t*)g->gelu_exps;
+  p.k_codes = (uint8_t*)g->keep_codes; p.k_exps = (uint8_t*)g->keep_exps;
   p.a_fmt = g->a_fmt; p.b_fmt = g->b_fmt; p.d8_fmt = g->d8_fmt; p.a_mn = g->a_mn ? 1 : 0; p.b_mn = g->b_mn ? 1 : 0; p.act = g->act;
   {
     const int tile_m = pair ? 256 : BM;
@@ -655,6 +744,13 @@ MSAMP_API int msamp_gemm_fp8_ex(const MsampGemmDesc* g, void* stream_) {
     int64_t grp = (48ll << 20) / ((int64_t)tile_m * K);    // row tiles whose A slab is about 48 MB
     if (grp < 4) grp = 4;
     p.group_m = grp >= num_m ? num_m : (int)grp;
+  }
+  if (keep) {
+    MSAMP_DISPATCH_HP(g->out_dtype, T, {
+      if (pair) return launch<256, true, T, 0, true>(ma, mb, md, p, g->max_ctas, stream);
+      if (bn == 256) return launch<256, false, T, 0, true>(ma, mb, md, p, g->max_ctas, stream);
+      return launch<128, false, T, 0, true>(ma, mb, md, p, g->max_ctas, stream);
+    });
   }
   MSAMP_DISPATCH_HP(g->out_dtype, T, {
     if (pair) return launch<256, true, T>(ma, mb, md, p, g->max_ctas, stream);

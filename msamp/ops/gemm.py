@@ -30,7 +30,8 @@ class _GemmDesc(ctypes.Structure):
         ('M', ctypes.c_int), ('N', ctypes.c_int), ('K', ctypes.c_int), ('a_fmt', ctypes.c_int), ('b_fmt', ctypes.c_int),
         ('d8_fmt', ctypes.c_int), ('a_mn', ctypes.c_int), ('b_mn', ctypes.c_int), ('out_dtype', ctypes.c_int),
         ('bias_dtype', ctypes.c_int), ('act', ctypes.c_int), ('max_ctas', ctypes.c_int), ('tile', ctypes.c_int), ('stats', ctypes.c_void_p),
-        ('colsum', ctypes.c_void_p),
+        ('colsum', ctypes.c_void_p), ('gelu_codes', ctypes.c_void_p), ('gelu_exps', ctypes.c_void_p), ('keep_codes', ctypes.c_void_p),
+        ('keep_exps', ctypes.c_void_p),
     ]
 
 
@@ -54,7 +55,7 @@ def _fix_operand(t):
 
 def gemm_fp8(a, a_qtype, a_scale_inv, b, b_qtype, b_scale_inv, out_dtype, bias=None, accumulate=False, out=None, amax_out=None,
              max_ctas=0, a_mn=False, b_mn=False, residual=None, gelu_src=None, act=None, out8=None, out8_qtype=None, out8_scale=None,
-             out8_scale_inv_out=None, tile=0, stats=None, colsum_out=None, store_out=True):
+             out8_scale_inv_out=None, tile=0, stats=None, colsum_out=None, store_out=True, gelu_blocks=None, keep_blocks=None):
     """Multiply FP8 byte matrices.
 
     Args:
@@ -76,7 +77,11 @@ def gemm_fp8(a, a_qtype, a_scale_inv, b, b_qtype, b_scale_inv, out_dtype, bias=N
             ``out8_scale_inv_out`` (optional) then receives ``1 / out8_scale``.
         colsum_out: optional fp32 ``[N]`` receiving the column sums of ``D`` as stored (the bias gradient when ``D`` is the
             output gradient of a biased layer); it is overwritten.
-        store_out: ``False`` skips ``D`` itself (returns ``None``) when only ``amax_out`` / ``out8`` / ``colsum_out`` are wanted.
+        store_out: ``False`` skips ``D`` itself (returns ``None``) when only ``amax_out`` / ``out8`` / ``colsum_out`` /
+            ``keep_blocks`` are wanted.
+        gelu_blocks: ``gelu_src`` as ``(codes [M,N], exponents)`` of ``cast.cast_blocks_to_fp8``; ``N`` a multiple of 32.
+        keep_blocks: two uint8 tensors (``[M,N]`` and ``[M*N/32]``, contiguous) that receive the e4m3 blocks of ``D`` as stored, what
+            ``cast.cast_blocks_to_fp8(D)`` gives; ``N`` a multiple of 32.
         tile: 0 = choose, 1 = CTA-pair 256x256 tiles, 2 = single-CTA tiles (CUDA only; for tests and benchmarks).
         stats: optional int64 ``[4 * CTAs]`` CUDA tensor receiving per-CTA cycle counters (producer wait, MMA wait for
             data, MMA wait for TMEM, MMA warp total) for tuning.
@@ -92,7 +97,7 @@ def gemm_fp8(a, a_qtype, a_scale_inv, b, b_qtype, b_scale_inv, out_dtype, bias=N
     if not store_out:
         if out is not None or accumulate or residual is not None:
             raise ValueError('store_out=False excludes out, accumulate and residual')
-        if amax_out is None and out8 is None and colsum_out is None:
+        if amax_out is None and out8 is None and colsum_out is None and keep_blocks is None:
             raise ValueError('store_out=False needs another output')
     elif out is None:
         out = torch.empty((M, N), dtype=out_dtype, device=a.device)
@@ -107,6 +112,14 @@ def gemm_fp8(a, a_qtype, a_scale_inv, b, b_qtype, b_scale_inv, out_dtype, bias=N
             assert t.shape == (M, N) and t.dtype == out_dtype and t.stride(1) == 1
     if out8 is not None:
         assert out8.shape == (M, N) and out8.dtype == torch.uint8 and out8.stride(1) == 1 and out8_scale is not None
+    for blocks in (gelu_blocks, keep_blocks):
+        if blocks is not None:
+            if N % 32:
+                raise ValueError(f'gemm_fp8: e4m3 blocks need N to be a multiple of 32 (got {N})')
+            for t, n in zip(blocks, (M * N, M * N // 32)):
+                assert t.numel() == n and t.dtype == torch.uint8 and t.is_contiguous() and t.device == a.device
+    if gelu_blocks is not None and gelu_src is not None:
+        raise ValueError('gelu_src and gelu_blocks exclude each other')
     if a.is_cuda:
         a, b = _fix_operand(a), _fix_operand(b)
         if K % 16 and not (a_mn and b_mn):
@@ -127,7 +140,9 @@ def gemm_fp8(a, a_qtype, a_scale_inv, b, b_qtype, b_scale_inv, out_dtype, bias=N
             0 if gelu_src is None else gelu_src.stride(0), out8.stride(0) if has8 else 0,
             M, N, K, native.fmt(a_qtype), native.fmt(b_qtype), native.fmt(out8_qtype) if has8 else 0, int(bool(a_mn)), int(bool(b_mn)),
             native.dt(out_dtype), 0 if bias is None else native.dt(bias.dtype), 1 if act == 'gelu' else 0, int(max_ctas),
-            int(tile) or _DEFAULT_TILE, addr(stats), addr(colsum_out)
+            int(tile) or _DEFAULT_TILE, addr(stats), addr(colsum_out),
+            *((None, None) if gelu_blocks is None else (gelu_blocks[0].data_ptr(), gelu_blocks[1].data_ptr())),
+            *((None, None) if keep_blocks is None else (keep_blocks[0].data_ptr(), keep_blocks[1].data_ptr()))
         )
         native.check(native.lib().msamp_gemm_fp8_ex(ctypes.byref(g), native.stream()), 'gemm_fp8')
         return out
@@ -142,9 +157,16 @@ def gemm_fp8(a, a_qtype, a_scale_inv, b, b_qtype, b_scale_inv, out_dtype, bias=N
         res = res + bias.float()
     if residual is not None:
         res = res + residual.float()
+    if gelu_blocks is not None:
+        from msamp.ops.cast import cast_blocks_from_fp8
+        gelu_src = cast_blocks_from_fp8(gelu_blocks[0].view(M, N), gelu_blocks[1], out_dtype)
     if gelu_src is not None:
         res = res * _gelu_tanh_grad(gelu_src.float())
     stored = res.to(out_dtype)
+    if keep_blocks is not None:
+        from msamp.ops.cast import cast_blocks_to_fp8
+        for dst, src in zip(keep_blocks, cast_blocks_to_fp8(stored)):
+            dst.copy_(src.view(dst.shape))
     if out is not None:
         out.copy_(stored)
     if colsum_out is not None:

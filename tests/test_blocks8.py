@@ -213,6 +213,80 @@ def test_entry_points_refuse():
     assert lib.msamp_blocks_cast(None, None, None, None, 0, 0, None) == 0 and lib.msamp_blocks_uncast(None, None, None, None, 0, 0, None) == 0
 
 
+# ------------------------------------------------------------------------------------------------------------- GEMM epilogues
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize('mnk, tile', [((1, 32, 16), 0), ((300, 160, 96), 2), ((300, 160, 96), 1), ((513, 544, 256), 1), ((257, 256, 128), 2),
+                                       ((2048, 1024, 512), 0)])
+def test_gemm_epilogues(device, dtype, mnk, tile):
+    """The blocks that a GEMM writes are those of its output, and the GeLU slope it takes from blocks is that of their values: equal bits."""
+    from msamp.common.dtype import Dtypes
+    from msamp.ops import gemm
+    m, n, k = mnk
+    if device == 'cpu' and m * n > 400000:
+        pytest.skip('the same code as at the other sizes')
+    gen = torch.Generator().manual_seed(m)
+    e4 = Dtypes.kfloat8_e4m3
+    a, b = ((torch.randn(r, k, generator=gen) * 2).to(torch.float8_e4m3fn).view(torch.uint8).to(device) for r in (m, n))
+    one = torch.tensor(0.5, device=device)
+    bias = torch.randn(n, generator=gen).to(device)
+    kept = (torch.empty(m, n, dtype=torch.uint8, device=device), torch.empty(m * n // 32, dtype=torch.uint8, device=device))
+    want = gemm.gemm_fp8(a, e4, one, b, e4, one, dtype, bias=bias, tile=tile)
+    amax = torch.zeros((), device=device)
+    got = gemm.gemm_fp8(a, e4, one, b, e4, one, dtype, bias=bias, tile=tile, keep_blocks=kept, amax_out=amax, act='gelu')
+    codes, exps = cast.cast_blocks_to_fp8(want)
+    assert torch.equal(got, want) and torch.equal(kept[0], codes) and torch.equal(kept[1], exps)
+    again = tuple(torch.zeros_like(t) for t in kept)
+    assert gemm.gemm_fp8(a, e4, one, b, e4, one, dtype, bias=bias, tile=tile, keep_blocks=again, store_out=False) is None
+    assert torch.equal(again[0], codes) and torch.equal(again[1], exps)
+    h = _values(m * n, dtype, n).clamp(-1e3, 1e3).view(m, n).to(device)
+    blocks = cast.cast_blocks_to_fp8(h)
+    h = cast.cast_blocks_from_fp8(*blocks, dtype)
+    x = gemm.gemm_fp8(a, e4, one, b, e4, one, dtype, tile=tile, gelu_src=h)
+    y = gemm.gemm_fp8(a, e4, one, b, e4, one, dtype, tile=tile, gelu_blocks=blocks)
+    assert torch.equal(x, y)
+    out8, sums, scale = torch.empty(m, n, dtype=torch.uint8, device=device), torch.empty(n, device=device), torch.tensor(2.0, device=device)
+    gemm.gemm_fp8(a, e4, one, b, e4, one, dtype, tile=tile, gelu_blocks=blocks, out8=out8, out8_qtype=e4, out8_scale=scale, colsum_out=sums, store_out=False)
+    assert torch.equal(out8, cast.cast_to_fp8(x, e4, scale))
+    assert (sums - x.float().sum(0)).abs().max() <= 1e-4 * (1 + x.float().abs().sum(0).max())    # another order of 32-bit sums
+    if device == 'cuda':
+        torch.cuda.synchronize()
+        assert native.device_status() == 0
+
+
+def test_gemm_epilogues_of_not_finite_values():
+    """What does not fit the output type becomes infinite there and NaN in the blocks."""
+    from msamp.common.dtype import Dtypes
+    from msamp.ops import gemm
+    for device in ['cpu'] + (['cuda'] if torch.cuda.is_available() else []):
+        a = torch.ones(3, 16, device=device).to(torch.float8_e4m3fn).view(torch.uint8)
+        b = torch.ones(64, 16, device=device).to(torch.float8_e4m3fn).view(torch.uint8)
+        bias = torch.zeros(64, device=device)
+        bias[5], bias[40], bias[41] = 1e6, float('nan'), -1e6
+        one = torch.tensor(1.0, device=device)
+        kept = (torch.empty(3, 64, dtype=torch.uint8, device=device), torch.empty(6, dtype=torch.uint8, device=device))
+        d = gemm.gemm_fp8(a, Dtypes.kfloat8_e4m3, one, b, Dtypes.kfloat8_e4m3, one, torch.float16, bias=bias, keep_blocks=kept)
+        codes, exps = cast.cast_blocks_to_fp8(d)
+        assert torch.equal(kept[0], codes) and torch.equal(kept[1], exps)
+        v = cast.cast_blocks_from_fp8(*kept, torch.float16)
+        assert torch.equal(torch.isnan(v), ~torch.isfinite(d)) and (v[:, :5] == 16).all()
+
+
+def test_gemm_blocks_refused():
+    from msamp.common.dtype import Dtypes
+    from msamp.ops import gemm
+    e4, one = Dtypes.kfloat8_e4m3, torch.tensor(1.0)
+    a, b = torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(48, 16, dtype=torch.uint8)
+    u8 = lambda n: torch.zeros(n, dtype=torch.uint8)    # noqa: E731
+    with pytest.raises(ValueError):
+        gemm.gemm_fp8(a, e4, one, b, e4, one, torch.float32, keep_blocks=(u8(192), u8(6)))
+    b = torch.zeros(64, 16, dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        gemm.gemm_fp8(a, e4, one, b, e4, one, torch.float32, gelu_blocks=(u8(256), u8(8)), gelu_src=torch.zeros(4, 64))
+    with pytest.raises(AssertionError):
+        gemm.gemm_fp8(a, e4, one, b, e4, one, torch.float32, keep_blocks=(u8(256), u8(7)))
+
+
 # ------------------------------------------------------------------------------------------------------------- recomputation
 @pytest.mark.parametrize('device', CPU_GPU)
 def test_checkpoint_gradients_are_those_at_the_kept_input(device):

@@ -173,6 +173,43 @@ def test_fused_sublayers_compute_what_the_separate_calls_compute():
 
 
 @pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('ffn', [512, 528])
+def test_mlp_sublayer_with_delayed_scales(device, ffn):
+    """Past the warm-up the fc1 GEMM writes the blocks and no h at all (rows of whole blocks), or a pass over h does: the same bytes, so
+    the same gradients."""
+    from msamp.nn import model_state
+    torch.manual_seed(0)
+    dt = torch.bfloat16 if device == 'cuda' else torch.float32
+
+    class Parts(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            from msamp.models.gpt import LayerNorm
+            self.ln, self.fc1, self.fc2 = LayerNorm(128), torch.nn.Linear(128, ffn), torch.nn.Linear(ffn, 128)
+
+    parts = LinearReplacer.replace(Parts().to(device))
+    x, dy = torch.randn(40, 128, device=device).to(dt), torch.randn(40, 128, device=device).to(dt)
+    for lin in (parts.fc1, parts.fc2):    # any scale that was found before
+        for name, meta in lin.scaling_metas.items():
+            meta.amax_counter.fill_(10**6) if isinstance(meta.amax_counter, torch.Tensor) else setattr(meta, 'amax_counter', 10**6)
+            meta.scale.fill_(8.0)
+    assert not parts.fc2.scaling_metas['input'].is_in_time_scaling()
+    kept = []
+    leaf = x.clone().requires_grad_(True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        y = FL.mlp_sublayer(leaf, parts.ln, parts.fc1, parts.fc2, keep_fp8=True)
+    assert not any(t.shape == (40, ffn) and t.dtype == dt for t in kept)
+    y.backward(dy)
+    plain = x.clone().requires_grad_(True)
+    z = FL.mlp_sublayer(plain, parts.ln, parts.fc1, parts.fc2)
+    z.backward(dy)
+    assert torch.equal(y, z)
+    a, c = plain.grad.float(), leaf.grad.float()
+    assert 0 < (a - c).norm() <= 0.16 * a.norm()
+    model_state.clear()
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
 def test_mlp_sublayer_keeps_the_gelu_input_in_8_bits(device):
     torch.manual_seed(0)
     dt = torch.bfloat16 if device == 'cuda' else torch.float32
