@@ -398,8 +398,8 @@ def attention_qkv(qkv, causal=True, scale=None):
 
 # Attention whose query heads share key / value heads, on rows that may end early.  ``q [B, S, heads, d]``, ``k`` and ``v [B, S, kv_heads, d]``
 # as strided views, ``lengths`` int32 ``[B]`` or None.  The argument blocks of the native entry points: addresses, sizes and scale, strides.
-_pack_fwd, _pack_bwd = struct.Struct('7q').pack, struct.Struct('12q').pack
-_pack_one, _pack_sizes, _pack_st = struct.Struct('q').pack, struct.Struct('6qd').pack, [struct.Struct(f'{3 * n}q').pack for n in range(9)]
+_pack_fwd, _pack_bwd = struct.Struct('7q').pack, struct.Struct('13q').pack
+_pack_sizes, _pack_st = struct.Struct('6qd').pack, [struct.Struct(f'{3 * n}q').pack for n in range(9)]
 
 
 def _map_strides(t):
@@ -424,11 +424,15 @@ def _mappable(t):
 
 
 def _shared_fwd(q, k, v, causal, scale, lengths):
-    """``(o, lse, plan, fields)``; the last are sizes and strides of q, k, v and o, which the backward pass has too."""
+    """``(o, lse, plan, fields)``; the last are sizes and strides of q, k, v and o, which the backward pass has too.
+
+    ``lse`` is ``[2, B, heads, S]``: the log-sum-exps, and room for rowsum(dO * O) in the backward pass (1 / 64 of the size of ``o`` at
+    head size 128; an allocation there costs more than the kernel that fills it takes for short rows).
+    """
     B, S, nh, d = q.shape
     nkv = k.shape[2]
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = q.new_empty((B, nh, S), dtype=torch.float32)
+    lse = q.new_empty((2, B, nh, S), dtype=torch.float32)
     # with lengths: the tiles that are not padding, listed by the forward pass for both passes
     plan = q.new_empty(2 + (B + 1) * ((S + 127) // 128), dtype=torch.int32) if lengths is not None else None
     fields = _pack_sizes(B, nh, nkv, S, d, causal, scale) + _pack_st[4](*_map_strides(q), *_map_strides(k), *_map_strides(v),
@@ -444,24 +448,25 @@ def _shared_fwd(q, k, v, causal, scale, lengths):
 
 
 def _shared_workspace(B, nh, nkv, S, d, causal, lengths):
-    """Floats of the backward pass's workspace, and of its first part: delta, then the partial sums of dK and dV where there are several."""
-    first = (B * nh * S + 3) // 4 * 4
-    return first + native.lib().msamp_attention_shared_partial(B, nh, nkv, S, d, causal, lengths is not None), first
+    """Floats of the backward pass's workspace: partial sums of dK and dV where there may be several."""
+    return native.lib().msamp_attention_shared_partial(B, nh, nkv, S, d, causal, lengths is not None)
 
 
 def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, work, grad_strides):
     """Gradients into ``dq``, ``dk`` and ``dv``, whose packed strides are ``grad_strides``."""
     if not d_o.is_contiguous() or d_o.data_ptr() % 16:
         d_o = _rows16(_mappable(d_o))
-    total, first = work
-    space = q.new_empty(total, dtype=torch.float32)
-    at = space.data_ptr()
+    lse = lse.contiguous()
+    if lengths is not None:
+        lengths, plan = lengths.contiguous(), plan.contiguous()
+    space = q.new_empty(work, dtype=torch.float32) if work else None
     with native.on_device(q):
         native.check(
             native.lib().msamp_attention_shared_bwd(
                 _pack_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-                          0 if plan is None else plan.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), at) +
-                _pack_one(at + 4 * first) + fields + _pack_st[1](*_map_strides(d_o)) + grad_strides, native.raw_stream()
+                          0 if plan is None else plan.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                          lse.data_ptr() + 2 * lse.numel(), 0 if space is None else space.data_ptr()) + fields +
+                _pack_st[1](*_map_strides(d_o)) + grad_strides, native.raw_stream()
             ), 'attention_bwd'
         )
 
