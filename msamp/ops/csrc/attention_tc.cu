@@ -9,6 +9,8 @@
 //   attn_bwd_dkdv_ps_kernel   128 key rows: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
 //   attn_bwd_dq_ps_kernel     128 query rows: S = Q K^T, dP = dO V^T, dQ += dS K
 //   attn_fwd_tm_kernel, attn_fwd_split_kernel   forward of short rows of head size 128, two maxima per row (see kSplitRows)
+// The first three are also compiled for query heads that share key / value heads (X >= 1) and for rows with lengths (X == 2), at the end
+// of the file; attn_plan_kernel lists the work of rows with lengths, attn_bwd_join_kernel adds up dK and dV of items in parts.
 // Head size 128 also has earlier kernels with one CTA per work item, and with 64-wide tiles and P / dS in shared memory; they
 // run when MSAMP_ATTN_{FWD,BWD}_PERSIST=0 or MSAMP_ATTN_{FWD,BWD}_SMEM=1 and serve as a cross-check.
 //
