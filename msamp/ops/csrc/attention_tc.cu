@@ -3568,7 +3568,8 @@ attn_bwd_dkdv_ps_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
   if (warp == 1) tc5::tmem_dealloc(tmem_base, TM_COLS);
 }
 
-// dK and dV of the parts of a key tile, added up in order; a CTA takes 16 columns of 128 rows of one of them.  Bound by memory.
+// dK and dV of the parts of a key tile, added up in order; a CTA takes 16 columns of 128 rows of one of them, so that a warp reads 512
+// consecutive bytes at a time.  Bound by memory: 1 x 4096 x 16 / 1 heads of 128 in 8 parts (34 MB, most of it in L2) 6 us.
 struct JoinParams {
   TcParams p;
   int n_kt;
@@ -3646,7 +3647,8 @@ __host__ __device__ __forceinline__ int choose_parts(int rep, int64_t items, flo
 // n_tiles words of scratch.  The work of tile i is i + 1 tiles when causal, else those of its row; ties go by batch, then by tile.
 // CTA 0 makes the list by counting: a warp takes one amount of work at a time, counts the batches that have it (ballots, in order, so that
 // nothing depends on timing), and after a scan over the amounts goes over them once more to place their tiles.  The other CTAs clear
-// padding, `share` of them for a batch.
+// padding, `share` of them for a batch.  Bound by latency, 6.5 us for 8 rows of up to 1000.  With the list the kernels of 16 x 577 x 16 heads
+// of 64 (lengths 10 to 577) took 46 + 97 us in the place of 63 + 139 us with an item for every tile, padding or not.
 struct PlanParams {
   const int* lengths;
   int* plan;
@@ -4033,6 +4035,8 @@ MSAMP_API int msamp_attention_tc_bwd(const void* q, const void* k, const void* v
 // behind a row's length are padding, as queries and as keys; their outputs and gradients are zero, their lse -inf, whatever they hold.  With
 // lengths the forward pass writes `plan` (2 + (batch + 1) * ceil(seqlen / 128) ints), which the backward pass of the same lengths reads.
 // Strides as for the entry points above, those of k, v, dk and dv over kv_heads.
+// Measured: 4 x 2048 x 32 / 8 heads of 128, causal, 199 + 494 us (equal heads 195 + 540 us); 1 x 4096 x 16 / 1 88 + 247 us; 2 x 4096 x 16 / 4
+// heads of 64 166 + 382 us; 8 x 1000 x 12 / 4 heads of 64 with lengths 18 to 1000 40 + 71 us.
 static int shared_checks(int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, const int* lengths, const int* plan,
                          const int64_t* strides, int n) {
   MSAMP_REQUIRE(head_dim == 64 || head_dim == 128, "attention (shared heads): head_dim must be 64 or 128 (got %d)", head_dim);

@@ -98,7 +98,9 @@ __device__ __forceinline__ uint32_t vector_amax(const Bytes32& raw) {
 }
 
 // Bound by memory.  VEC: every pointer aligned for whole vectors of 32 bytes, so that a thread stores 16 codes at once and a warp 16 exponents;
-// two vectors a thread and step are in flight, L lanes find the maximum of a block with log2(L) shuffles.  A warp that sees an infinity or a NaN (its maxima are on top of all numbers) goes over its elements again.
+// two vectors a thread and step are in flight, L lanes find the maximum of a block with log2(L) shuffles.  8192 x 16384 bf16, L2 flushed:
+// 72 us (5.7 TB/s), with GeLU 120 us (5.6 TB/s); 16-byte vectors 84 and 128 us, one in flight 78 and 122 us, maxima of unpacked elements
+// 110 and 154 us.  A copy of 537 MB runs at 6.1 TB/s.  A warp that sees an infinity or a NaN (its maxima are on top of all numbers) goes over its elements again.
 template <typename T, bool GELU, bool VEC>
 __global__ void __launch_bounds__(kThreads) blocks_cast_kernel(const T* __restrict__ x, T* __restrict__ y, uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ exps, int64_t n) {
@@ -161,7 +163,8 @@ __device__ __forceinline__ T uncast_one(float v, T dy) {
   return from_f32<T>(in_range<T>(v));
 }
 
-// Bound by memory: two vectors a thread and step in flight.
+// Bound by memory: two vectors a thread and step in flight.  8192 x 16384 bf16, L2 flushed: 75 us (5.4 TB/s), with the GeLU slope 123 us
+// (5.5 TB/s); one vector in flight 74 and 143 us.
 template <typename T, bool GELU, bool VEC>
 __global__ void __launch_bounds__(kThreads) blocks_uncast_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps,
                                                                  const T* __restrict__ dy, T* __restrict__ out, int64_t n) {

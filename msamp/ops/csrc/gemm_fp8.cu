@@ -121,7 +121,9 @@ __device__ __forceinline__ void colsum_chunk(float* cs, const float (&v)[32], in
     if (j < valid) atomicAdd(cs + j, to_f32<OutT>(from_f32<OutT>(v[j])));
 }
 
-// A thread of the epilogue holds 32 columns of a row, which is one block: its values' largest magnitude needs no exchange.
+// A thread of the epilogue holds 32 columns of a row, which is one block: its values' largest magnitude needs no exchange.  A GPT step of four
+// layers of hidden size 4096 (8192 tokens) takes 29.4 to 29.8 ms with the blocks written and read here, 29.5 to 30.0 with passes of
+// their own and 29.2 with h in 16 bits.
 template <typename OutT>
 __device__ __forceinline__ void keep_block(uint8_t* codes, uint8_t* exp, const float (&v)[32]) {
   using namespace blocks8;

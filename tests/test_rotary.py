@@ -194,6 +194,17 @@ def test_entry_point_refuses():
 
 
 @pytest.mark.gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason='needs two GPUs')
+def test_tensors_of_another_device_than_the_current_one():
+    torch.manual_seed(6)
+    freqs, q = K.rotary_frequencies(64, device='cuda:1'), torch.randn(2, 5, 4, 64, device='cuda:1')
+    assert torch.cuda.current_device() == 0
+    _check(K.rotary(q, None, freqs), q, freqs, None, False)
+    with pytest.raises(ValueError):
+        K.rotary(q, None, freqs.to('cuda:0'))
+
+
+@pytest.mark.gpu
 def test_captured_and_on_a_side_stream():
     torch.manual_seed(4)
     freqs = K.rotary_frequencies(64, device='cuda')
