@@ -22,6 +22,7 @@
 // Head size 64 took the mma.sync kernels of attention.cu before: 8 x 1024 x 12 heads, causal, 71 + 253 us forward + backward on
 // the device, now 44 + 107 us; 64 x 197 x 12 heads, 61 + 218 us, now 45 + 119 us.  Those kernels remain for views that a tensor map
 // cannot describe, for short rows (see short_rows) and as a cross-check (MSAMP_ATTN_IMPL=mma).
+#include <atomic>
 #include <cstdlib>
 #include <initializer_list>
 #include <mutex>
@@ -4050,16 +4051,29 @@ static int shared_checks(int batch, int heads, int kv_heads, int seqlen, int hea
   return MSAMP_OK;
 }
 
+// The attribute stays with the kernel on its device; two threads that find it unset both set it.
+template <typename K>
+static int set_smem_once(std::atomic<bool> (&done)[64], K kernel, int bytes) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && done[dev]) return MSAMP_OK;
+  const int rc = set_smem(kernel, bytes);
+  if (rc == MSAMP_OK && dev >= 0 && dev < 64) done[dev] = true;
+  return rc;
+}
+
 template <int D, int X>
 static int launch_fwd(const CUtensorMap (&m)[3], const TcParams& p, int n_qt, int ctas, cudaStream_t stream) {
-  if (int rc = set_smem(attn_fwd_ps_kernel<D, X>, fwd3::Cfg<D>::SMEM)) return rc;
+  static std::atomic<bool> done[64];
+  if (int rc = set_smem_once(done, attn_fwd_ps_kernel<D, X>, fwd3::Cfg<D>::SMEM)) return rc;
   attn_fwd_ps_kernel<D, X><<<ctas, kPsThreads, fwd3::Cfg<D>::SMEM, stream>>>(m[0], m[1], m[2], p, n_qt, n_qt * p.batch * p.heads);
   return MSAMP_OK;
 }
 template <int D, int X>
 static int launch_bwd(const CUtensorMap (&m)[4], const TcParams& p, int n_t, int sms, cudaStream_t stream) {
-  if (int rc = set_smem(attn_bwd_dkdv_ps_kernel<D, X>, dkv3::Cfg<D>::SMEM)) return rc;
-  if (int rc = set_smem(attn_bwd_dq_ps_kernel<D, X>, dqk3::Cfg<D>::SMEM)) return rc;
+  static std::atomic<bool> done_k[64], done_q[64];
+  if (int rc = set_smem_once(done_k, attn_bwd_dkdv_ps_kernel<D, X>, dkv3::Cfg<D>::SMEM)) return rc;
+  if (int rc = set_smem_once(done_q, attn_bwd_dq_ps_kernel<D, X>, dqk3::Cfg<D>::SMEM)) return rc;
   // with lengths the number of parts is known on the device only: as many CTAs as any number of them needs
   const int n_q = n_t * p.batch * p.heads, n_k = n_t * p.batch * p.kv_heads * (X == 2 ? p.rep : p.parts);
   attn_bwd_dq_ps_kernel<D, X><<<n_q < sms ? n_q : sms, kPsThreads, dqk3::Cfg<D>::SMEM, stream>>>(m[0], m[1], m[2], m[3], p, n_t, n_q);

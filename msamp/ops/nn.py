@@ -423,39 +423,80 @@ def _mappable(t):
     return t.contiguous() if any(s == 0 and n > 1 for s, n in zip((a, b, c), t.shape)) else t
 
 
-def _shared_fwd(q, k, v, causal, scale, lengths):
-    """``(o, lse, plan, fields)``; the last are sizes and strides of q, k, v and o, which the backward pass has too.
+class _SharedCall:
+    """What calls of the same sizes and strides share: their checks, and the fields of both argument blocks that are no addresses."""
+    __slots__ = ('fields', 'tail', 'strides', 'work', 'lse_shape', 'plan_size', 'split', 'args')
+
+    def __init__(self, q, k, v, causal, scale, packed, ragged):
+        B, S, nh, d = q.shape
+        nkv = k.shape[2]
+        if q.dtype != torch.bfloat16 or d not in (64, 128):
+            raise RuntimeError(f'attention: CUDA kernel supports bf16 with head_dim 64/128 (got {q.dtype}, {d})')
+        for t in (q, k, v):
+            if t.stride(3) != 1 or any(s & 7 for s in _map_strides(t)):
+                raise RuntimeError('attention: operands must have unit inner stride and 16-byte aligned rows')
+        self.args = (causal, scale)
+        dense = _dense_strides(S, nh, d)
+        self.fields = _pack_sizes(B, nh, nkv, S, d, causal, scale) + _pack_st[4](*_map_strides(q), *_map_strides(k), *_map_strides(v), *dense)
+        # dO as a rule in the layout of o, then dq, dk and dv
+        grads = _dense_strides(S, nh + 2 * nkv, d) * 3 if packed else dense + _dense_strides(S, nkv, d) * 2
+        self.tail = _pack_st[4](*dense, *grads)
+        self.strides = (q.stride(), k.stride(), v.stride(), torch.empty((B, S, nh, d), device='meta').stride())
+        with native.on_device(q):
+            self.work = _shared_workspace(B, nh, nkv, S, d, causal, ragged)
+        self.lse_shape = (2, B, nh, S)
+        # with lengths: the tiles that are not padding, listed by the forward pass for both passes
+        self.plan_size = 2 + (B + 1) * ((S + 127) // 128) if ragged else 0
+        self.split = ((B, S, nh + 2 * nkv, d), [nh, nkv, nkv]) if packed else None
+
+
+_shared_calls = {}
+
+
+def _shared_call(q, k, v, causal, scale, packed, lengths):
+    """Checks and shared fields of a call, remembered by its sizes and strides."""
+    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), causal, scale, packed, lengths is None, q.device)
+    call = _shared_calls.get(key)
+    if call is None or q.dtype != torch.bfloat16:
+        _check_shared(q, k, v, scale, lengths)
+        if len(_shared_calls) > 1024:
+            _shared_calls.clear()
+        call = _shared_calls[key] = _SharedCall(q, k, v, causal, scale, packed, lengths is not None)
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.device != q.device or v.device != q.device:
+        _check_shared(q, k, v, scale, lengths)
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        raise RuntimeError('attention: operands must have unit inner stride and 16-byte aligned rows')
+    if lengths is not None:
+        _check_lengths(q, lengths)
+    return call
+
+
+def _shared_workspace(B, nh, nkv, S, d, causal, ragged):
+    """Floats of the backward pass's workspace: partial sums of dK and dV where there may be several."""
+    return native.lib().msamp_attention_shared_partial(B, nh, nkv, S, d, causal, ragged)
+
+
+def _shared_fwd(q, k, v, call, lengths):
+    """``(o, lse, plan)``.
 
     ``lse`` is ``[2, B, heads, S]``: the log-sum-exps, and room for rowsum(dO * O) in the backward pass (1 / 64 of the size of ``o`` at
     head size 128; an allocation there costs more than the kernel that fills it takes for short rows).
     """
-    B, S, nh, d = q.shape
-    nkv = k.shape[2]
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = q.new_empty((2, B, nh, S), dtype=torch.float32)
-    # with lengths: the tiles that are not padding, listed by the forward pass for both passes
-    plan = q.new_empty(2 + (B + 1) * ((S + 127) // 128), dtype=torch.int32) if lengths is not None else None
-    fields = _pack_sizes(B, nh, nkv, S, d, causal, scale) + _pack_st[4](*_map_strides(q), *_map_strides(k), *_map_strides(v),
-                                                                        *_dense_strides(S, nh, d))
+    lse = q.new_empty(call.lse_shape, dtype=torch.float32)
+    plan = q.new_empty(call.plan_size, dtype=torch.int32) if call.plan_size else None
     with native.on_device(q):
         native.check(
             native.lib().msamp_attention_shared_fwd(
                 _pack_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-                          0 if plan is None else plan.data_ptr()) + fields, native.raw_stream()
+                          0 if plan is None else plan.data_ptr()) + call.fields, native.raw_stream()
             ), 'attention_fwd'
         )
-    return o, lse, plan, fields
+    return o, lse, plan
 
 
-def _shared_workspace(B, nh, nkv, S, d, causal, lengths):
-    """Floats of the backward pass's workspace: partial sums of dK and dV where there may be several."""
-    return native.lib().msamp_attention_shared_partial(B, nh, nkv, S, d, causal, lengths is not None)
-
-
-def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, work, grad_strides):
-    """Gradients into ``dq``, ``dk`` and ``dv``, whose packed strides are ``grad_strides``."""
-    if not d_o.is_contiguous() or d_o.data_ptr() % 16:
-        d_o = _rows16(_mappable(d_o))
+def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, work, tail):
+    """Gradients into ``dq``, ``dk`` and ``dv``; ``tail``: packed strides of ``d_o`` and of theirs."""
     lse = lse.contiguous()
     if lengths is not None:
         lengths, plan = lengths.contiguous(), plan.contiguous()
@@ -465,48 +506,38 @@ def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, work, g
             native.lib().msamp_attention_shared_bwd(
                 _pack_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
                           0 if plan is None else plan.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                          lse.data_ptr() + 2 * lse.numel(), 0 if space is None else space.data_ptr()) + fields +
-                _pack_st[1](*_map_strides(d_o)) + grad_strides, native.raw_stream()
+                          lse.data_ptr() + 2 * lse.numel(), 0 if space is None else space.data_ptr()) + fields + tail, native.raw_stream()
             ), 'attention_bwd'
         )
 
 
 class _AttentionSharedFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, causal, scale, grad_layout, lengths):
-        o, lse, plan, ctx.fields = _shared_fwd(q, k, v, causal, scale, lengths)
+    def forward(ctx, q, k, v, lengths, call):
+        o, lse, plan = _shared_fwd(q, k, v, call, lengths)
         ctx.save_for_backward(q, k, v, o, lse, lengths, plan)
-        B, S, nh, d = q.shape
-        nkv = k.shape[2]
-        ctx.packed = grad_layout == 'packed'
-        if ctx.packed:
-            ctx.grad_strides = _pack_st[3](*_dense_strides(S, nh + 2 * nkv, d) * 3)
-        else:
-            ctx.grad_strides = _pack_st[3](*_dense_strides(S, nh, d), *_dense_strides(S, nkv, d) * 2)
-        ctx.work = _shared_workspace(B, nh, nkv, S, d, causal, lengths)
-        ctx.args, ctx.places = (causal, scale), _places(q, k, v, o)
+        ctx.call = call
         return o
 
     @staticmethod
     def backward(ctx, d_o):
         q, k, v, o, lse, lengths, plan = ctx.saved_tensors
-        fields = ctx.fields
-        if _places(q, k, v, o) != ctx.places:    # saved tensors may come back with other strides (saved-tensor hooks)
+        call = ctx.call
+        fields, tail = call.fields, call.tail
+        if (q.stride(), k.stride(), v.stride(), o.stride()) != call.strides or (q.data_ptr() | k.data_ptr() | v.data_ptr() | o.data_ptr()) & 15:
+            # saved tensors may come back with other strides (saved-tensor hooks)
             q, k, v, o = (_rows16(_mappable(t)) for t in (q, k, v, o))
             B, S, nh, d = q.shape
-            fields = _pack_sizes(B, nh, k.shape[2], S, d, *ctx.args) + _pack_st[4](*(s for t in (q, k, v, o) for s in _map_strides(t)))
-        if ctx.packed:
-            B, S, nh, d = q.shape
-            nkv = k.shape[2]
-            dq, dk, dv = q.new_empty((B, S, nh + 2 * nkv, d)).split([nh, nkv, nkv], dim=2)
-        else:
+            fields = _pack_sizes(B, nh, k.shape[2], S, d, *call.args) + _pack_st[4](*(s for t in (q, k, v, o) for s in _map_strides(t)))
+        if not d_o.is_contiguous() or d_o.data_ptr() & 15:
+            d_o = _rows16(_mappable(d_o))
+            tail = _pack_st[1](*_map_strides(d_o)) + tail[24:]
+        if call.split is None:
             dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, ctx.work, ctx.grad_strides)
-        return dq, dk, dv, None, None, None, None
-
-
-def _places(*ts):
-    return tuple((t.stride(), t.data_ptr() & 15) for t in ts)
+        else:
+            dq, dk, dv = q.new_empty(call.split[0]).split(call.split[1], dim=2)
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call.work, tail)
+        return dq, dk, dv, None, None
 
 
 def _attention_plain(q, k, v, causal, scale, lengths):
@@ -533,12 +564,43 @@ def _attention_plain(q, k, v, causal, scale, lengths):
     return out.contiguous()
 
 
+def _check_lengths(q, lengths):
+    if lengths.shape != q.shape[:1] or lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f'attention: lengths must be an int32 or int64 tensor [{q.shape[0]}] (got {lengths.dtype} {tuple(lengths.shape)})')
+    if lengths.device != q.device:
+        raise ValueError('attention: lengths must be on the device of q')
+
+
+def _check_shared(q, k, v, scale, lengths):
+    shape, kv = q.shape, k.shape
+    if len(shape) != 4 or len(kv) != 4 or v.shape != kv or kv[:2] != shape[:2] or kv[3] != shape[3]:
+        raise ValueError(f'attention: q {tuple(shape)}, k {tuple(kv)} and v {tuple(v.shape)} do not fit together')
+    if kv[2] == 0 or shape[2] % kv[2]:
+        raise ValueError(f'attention: {shape[2]} query heads do not share {kv[2]} key/value heads evenly')
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise ValueError('attention: q, k and v must have one dtype and one device')
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f'attention: scale must be positive (got {scale})')
+    if lengths is not None:
+        _check_lengths(q, lengths)
+
+
+def _shared_operands(q, k, v, causal, scale, packed, lengths):
+    """Mappable views, lengths in int32, and the shared fields of the call."""
+    if len(q.shape) == len(k.shape) == len(v.shape) == 4:
+        q, k, v = _mappable(q), _mappable(k), _mappable(v)
+    call = _shared_call(q, k, v, bool(causal), float(scale), packed, lengths)
+    if lengths is not None:
+        lengths = lengths.to(torch.int32).contiguous()
+    return q, k, v, lengths, call
+
+
 def attention_shared_fwd_raw(q, k, v, causal=True, scale=None, lengths=None):
     """Forward pass of :func:`attention` with shared key/value heads or row lengths, without autograd: ``(o, lse, plan)`` for its gradients."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if _use_native(q) and q.numel():
-        q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
-        return _shared_fwd(q, k, v, bool(causal), float(scale), lengths)[:3]
+        q, k, v, lengths, call = _shared_operands(q, k, v, causal, scale, False, lengths)
+        return _shared_fwd(q, k, v, call, lengths)
     _check_shared(q, k, v, scale, lengths)
     with torch.no_grad():
         return _attention_plain(q, k, v, causal, scale, lengths), None, None
@@ -548,12 +610,12 @@ def attention_shared_bwd_raw(q, k, v, o, lse, plan, d_o, dq, dk, dv, causal=True
     """Its gradients, written into ``dq``, ``dk`` and ``dv`` (views with unit inner stride and 16-byte aligned rows)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if _use_native(q) and q.numel():
-        q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
-        o = _rows16(_mappable(o))
+        q, k, v, lengths, call = _shared_operands(q, k, v, causal, scale, False, lengths)
+        o, d_o = _rows16(_mappable(o)), _rows16(_mappable(d_o))
         B, S, nh, d = q.shape
-        fields = _pack_sizes(B, nh, k.shape[2], S, d, bool(causal), float(scale)) + _pack_st[4](*(x for t in (q, k, v, o) for x in _map_strides(t)))
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, _shared_workspace(B, nh, k.shape[2], S, d, bool(causal), lengths),
-                    _pack_st[3](*(x for t in (dq, dk, dv) for x in _map_strides(t))))
+        fields = _pack_sizes(B, nh, k.shape[2], S, d, *call.args) + _pack_st[4](*(x for t in (q, k, v, o) for x in _map_strides(t)))
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call.work,
+                    _pack_st[4](*(x for t in (d_o, dq, dk, dv) for x in _map_strides(t))))
         return
     with torch.enable_grad():
         leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
@@ -562,48 +624,14 @@ def attention_shared_bwd_raw(q, k, v, o, lse, plan, d_o, dq, dk, dv, causal=True
         dst.copy_(g)
 
 
-def _check_shared(q, k, v, scale, lengths):
-    shape, kv = q.shape, k.shape
-    if len(shape) != 4 or len(kv) != 4 or v.shape != kv or kv[:2] != shape[:2] or kv[3] != shape[3]:
-        raise ValueError(f'attention: q {tuple(shape)}, k {tuple(kv)} and v {tuple(v.shape)} do not fit together')
-    if kv[2] == 0 or shape[2] % kv[2]:
-        raise ValueError(f'attention: {shape[2]} query heads do not share {kv[2]} key/value heads evenly')
-    dtype, device = q.dtype, q.device
-    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
-        raise ValueError('attention: q, k and v must have one dtype and one device')
-    if not 0.0 < scale < 3e38:
-        raise ValueError(f'attention: scale must be positive (got {scale})')
-    if lengths is not None:
-        if lengths.shape != shape[:1] or lengths.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f'attention: lengths must be an int32 or int64 tensor [{shape[0]}] (got {lengths.dtype} {tuple(lengths.shape)})')
-        if lengths.device != device:
-            raise ValueError('attention: lengths must be on the device of q')
-
-
-def _shared_operands(q, k, v, scale, lengths):
-    """Checked operands of the CUDA kernels: mappable views, lengths in int32."""
-    _check_shared(q, k, v, scale, lengths)
-    d = q.shape[3]
-    if q.dtype != torch.bfloat16 or d not in (64, 128):
-        raise RuntimeError(f'attention: CUDA kernel supports bf16 with head_dim 64/128 (got {q.dtype}, {d})')
-    q, k, v = _mappable(q), _mappable(k), _mappable(v)
-    for t in (q, k, v):
-        a, b, c = _map_strides(t)
-        if t.stride(3) != 1 or (a | b | c) & 7 or t.data_ptr() & 15:
-            raise RuntimeError('attention: operands must have unit inner stride and 16-byte aligned rows')
-    if lengths is not None:
-        lengths = lengths.to(torch.int32).contiguous()
-    return q, k, v, lengths
-
-
 def _attention_shared(q, k, v, causal, scale, grad_layout, lengths):
     if not q.is_cuda or q.numel() == 0:
         _check_shared(q, k, v, scale, lengths)
         return _attention_plain(q, k, v, causal, scale, lengths)
-    q, k, v, lengths = _shared_operands(q, k, v, scale, lengths)
+    q, k, v, lengths, call = _shared_operands(q, k, v, causal, scale, grad_layout == 'packed', lengths)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _AttentionSharedFn.apply(q, k, v, bool(causal), float(scale), grad_layout, lengths)
-    return _shared_fwd(q, k, v, bool(causal), float(scale), lengths)[0]
+        return _AttentionSharedFn.apply(q, k, v, lengths, call)
+    return _shared_fwd(q, k, v, call, lengths)[0]
 
 
 def attention(q, k, v, causal=True, scale=None, grad_layout='separate', lengths=None):
