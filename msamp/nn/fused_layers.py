@@ -245,8 +245,9 @@ class _AttnSublayerFn(torch.autograd.Function):
         o2 = o.view(batch * seq, n_head * head_dim)
         o8, o_sinv = _quantize(o2, m_proj['input'], E4M3)
         out = _g.gemm_fp8(o8, E4M3, o_sinv, wp8, E4M3, wp_sinv, dt, bias=b_proj, residual=x)
-        ctx.save_for_backward(x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths, plan)
-        ctx.n_kv, ctx.rope = n_kv, rope
+        ctx.save_for_backward(x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths, plan,
+                              *(rope or (None, None))[:2])
+        ctx.n_kv, ctx.interleaved = n_kv, rope is not None and rope[2]
         ctx.w_qkv, ctx.m_qkv, ctx.w_proj, ctx.m_proj = w_qkv, m_qkv, w_proj, m_proj
         ctx.shape = (batch, seq, n_head, head_dim)
         ctx.causal = causal
@@ -257,10 +258,11 @@ class _AttnSublayerFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
-        x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths, plan = ctx.saved_tensors
+        (x, ln_weight, mean, rstd, y8, y_sinv, qkv, o, lse, o8, o_sinv, wq8, wq_sinv, wp8, wp_sinv, lengths, plan, freqs,
+         positions) = ctx.saved_tensors
         m_qkv, m_proj = ctx.m_qkv, ctx.m_proj
         batch, seq, n_head, head_dim = ctx.shape
-        n_kv, rope = ctx.n_kv, ctx.rope
+        n_kv = ctx.n_kv
         dt = x.dtype
         g = g.contiguous()
         # proj
@@ -277,9 +279,9 @@ class _AttnSublayerFn(torch.autograd.Function):
                                          ctx.causal, lengths=lengths)
         del d_o
         dqkv2 = dqkv.view(batch * seq, (n_head + 2 * n_kv) * head_dim)
-        if rope is not None:
+        if freqs is not None:
             turned = _heads(dqkv2, batch, seq, n_head, n_kv)[3]
-            _nn.rotary_raw([turned], [turned], *rope, True)
+            _nn.rotary_raw([turned], [turned], freqs, positions, ctx.interleaved, True)
         # qkv
         dq8, dq_sinv, dbq = _quantize_ograd(dqkv2, m_qkv['ograd'], ctx.bq_dtype is not None, ctx.bq_dtype)
         del dqkv, dqkv2

@@ -105,6 +105,14 @@ def rotary_raw(xs, ys, freqs, positions, interleaved, inverse):
     Inner strides are one; the others are free.  ``inverse`` turns back, which is also the gradient.
     """
     x = xs[0]
+    _check_all(x, xs[1] if len(xs) > 1 else None, freqs, positions)
+    if len(ys) != len(xs) or len(xs) > 2:
+        raise ValueError(f'rotary: one or two tensors and as many results (got {len(xs)} and {len(ys)})')
+    for src, dst in zip(xs, ys):
+        if dst is not src and (dst.shape != src.shape or dst.dtype != src.dtype or dst.device != src.device):
+            raise ValueError(f'rotary: {tuple(src.shape)} {src.dtype} does not go into {tuple(dst.shape)} {dst.dtype}')
+        if (src.stride(3) != 1 or dst.stride(3) != 1) and src.shape[3] != 1 and src.numel():
+            raise ValueError('rotary: the elements of a head must be adjacent')
     if not x.is_cuda:
         for src, dst in zip(xs, ys):
             dst.copy_(_emulated(src, freqs, positions, interleaved, inverse))

@@ -249,6 +249,32 @@ def test_options_refused():
         _model('cpu')(torch.zeros(1, 4, dtype=torch.int64), positions=torch.arange(4))
 
 
+@pytest.mark.parametrize('fp8', [False, True])
+def test_positions_refused(fp8):
+    model = _model('cpu', **LONG)
+    model = LinearReplacer.replace(model) if fp8 else model
+    for positions in (torch.arange(5), torch.arange(4, device='meta'), torch.zeros(2, 4, dtype=torch.int64)):
+        with pytest.raises(ValueError):
+            model(torch.zeros(1, 4, dtype=torch.int64), positions=positions)
+    with pytest.raises(TypeError):
+        model(torch.zeros(1, 4, dtype=torch.int64), positions=torch.arange(4.0))
+
+
+# (on the CPU an unfused block has made its mask of the lengths in the forward pass: its gradients stay right)
+@pytest.mark.parametrize('device,fp8,which', [('cpu', False, 'positions'), ('cpu', True, 'positions'), ('cpu', True, 'lengths')] +
+                         [pytest.param('cuda', fp8, which, marks=pytest.mark.gpu) for fp8 in (False, True) for which in ('positions', 'lengths')])
+def test_changed_before_the_backward_pass(device, fp8, which):
+    """Gradients need the positions and lengths of the forward pass: overwritten ones are an error, not other gradients."""
+    model = _model(device, **LONG)
+    model = LinearReplacer.replace(model) if fp8 else model
+    tokens, labels, lengths = _batch(device)
+    given = dict(lengths=lengths.int(), positions=torch.arange(24, device=device))
+    loss = model(tokens, labels, **given)
+    given[which] += 1
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+
+
 def test_parameters_and_defaults():
     for kw in ({}, LONG, dict(n_kv_head=1), dict(rotary_dim=64)):
         model = GPT(_config(**kw))

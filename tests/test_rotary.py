@@ -177,6 +177,16 @@ def test_refusals():
         K.rotary(q, None, f.to('meta'))
 
 
+def test_raw_refusals():
+    f, q, k = K.rotary_frequencies(8), torch.randn(2, 3, 4, 8), torch.randn(2, 3, 1, 8)
+    for xs, ys, freqs, positions in (([q], [q], f, torch.arange(4)), ([q], [q], f, torch.arange(3, device='meta')), ([q], [q], f.to('meta'), None),
+                                     ([q], [q], K.rotary_frequencies(10), None), ([q, k[:, :2]], [q, k[:, :2]], f, None), ([q], [q, k], f, None),
+                                     ([q], [q[:, :, :2]], f, None), ([q], [q.bfloat16()], f, None), ([q], [torch.empty(2, 3, 8, 4).mT], f, None),
+                                     ([q, k, k], [q, k, k], f, None)):
+        with pytest.raises(ValueError):
+            K.rotary_raw(xs, ys, freqs, positions, False, False)
+
+
 @pytest.mark.skipif(not native.available(), reason='kernel library not built')
 def test_entry_point_refuses():
     """No launch: every call is refused by its arguments."""
