@@ -8,6 +8,21 @@ def _outputs(out):
     return (out, ) if isinstance(out, torch.Tensor) else tuple(out)
 
 
+def _tensors(args):
+    """Every tensor in nested arguments."""
+    if isinstance(args, torch.Tensor):
+        return [args]
+    if isinstance(args, dict):
+        args = args.values()
+    elif not isinstance(args, (tuple, list)):
+        return []
+    return [t for a in args for t in _tensors(a)]
+
+
+def _versions(args):
+    return [(t, t._version) for t in _tensors(args) if not t.is_inference()]
+
+
 class _CheckpointFp8Fn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, anchor, function, preserve_rng_state, args, x):
@@ -21,11 +36,14 @@ class _CheckpointFp8Fn(torch.autograd.Function):
         ctx.save_for_backward(*_c.cast_blocks_to_fp8(x))    # before the function, which may change x
         with torch.no_grad():
             out = function(x, *args)
+        ctx.versions = _versions(args)    # after the function, which may change them (a cache, a counter)
         return out if isinstance(out, torch.Tensor) else tuple(out)
 
     @staticmethod
     def backward(ctx, *grads):
         codes, exponents = ctx.saved_tensors
+        if any(t._version != v for t, v in ctx.versions):
+            raise RuntimeError('checkpoint_fp8: an argument was modified by an inplace operation before the backward pass ran the function again')
         x = _c.cast_blocks_from_fp8(codes, exponents, ctx.dtype).requires_grad_(ctx.needs_x)
         cuda = [ctx.device] if ctx.rng is not None and ctx.rng[1] is not None else []
         enabled, dtype, cache = ctx.autocast
@@ -36,6 +54,7 @@ class _CheckpointFp8Fn(torch.autograd.Function):
                     torch.cuda.set_rng_state(ctx.rng[1], ctx.device)
             with torch.enable_grad(), torch.autocast(ctx.device.type, enabled=enabled, dtype=dtype, cache_enabled=cache):
                 out = _outputs(ctx.function(x, *ctx.args))
+        ctx.versions = _versions(ctx.args)
         pairs = [(o, g) for o, g in zip(out, grads) if g is not None and isinstance(o, torch.Tensor) and o.requires_grad]
         if pairs:
             torch.autograd.backward([o for o, _ in pairs], [g for _, g in pairs])
@@ -47,15 +66,18 @@ def checkpoint_fp8(function, x, *args, preserve_rng_state=True):
 
     ``x`` (fp32, fp16 or bf16) is stored as e4m3 with a power-of-two scale per 32 elements (1.03 bytes each,
     :func:`msamp.ops.cast.cast_blocks_to_fp8`), so the outputs are those of ``function(x)`` and the gradients those at the stored
-    value, which is within 2^-4 of every element (of the small ones of a block: within 2^-17 of its largest).  Scaling metas of FP8 layers record the amaxes of the second run.  ``function``
-    returns a tensor or a tuple of tensors; ``args`` are handed on as they are and get no gradients.  Parameters receive theirs in
-    ``.grad``: use ``backward()``, not ``torch.autograd.grad``.  The random state of the first run is used again unless
-    ``preserve_rng_state`` is false.
+    value, which is within 2^-4 of every element (of the small ones of a block: within 2^-17 of its largest).  Scaling metas of FP8
+    layers record the amaxes of the second run.  ``function`` returns a tensor or a tuple of tensors.  ``args`` are handed on as they
+    are; a tensor among them that is computed from others with gradients is refused, as its gradient would not wait for its other uses.
+    Parameters, also among ``args``, receive their gradients in ``.grad``: use ``backward()``, not ``torch.autograd.grad``.  The random
+    state of the first run is used again unless ``preserve_rng_state`` is false.
     """
     if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f'checkpoint_fp8: unsupported dtype {x.dtype}')
     if not torch.is_grad_enabled():
         return function(x, *args)
+    if any(t.requires_grad and not t.is_leaf for t in _tensors(args)):
+        raise ValueError('checkpoint_fp8: only x may be computed from other tensors with gradients; give it to the function first, or detach the argument')
     # the anchor makes the outputs part of the graph where only parameters need gradients
     anchor = torch.empty(0, requires_grad=True)
     return _CheckpointFp8Fn.apply(anchor, function, preserve_rng_state, args, x)

@@ -331,6 +331,34 @@ def test_checkpoint_of_a_function_that_changes_its_input_and_returns_none():
     assert torch.equal(lin.weight.grad, torch.full((32, 32), 8.0)) and torch.allclose(x.grad, 2 * lin.weight.sum(0).expand(4, 32))
 
 
+def test_checkpoint_arguments():
+    torch.manual_seed(12)
+    x, w, side = torch.randn(4, 32, requires_grad=True), torch.randn(32, requires_grad=True), torch.randn(4, 32)
+
+    def f(x, parts):
+        w, (side, ) = parts['w'], parts['side']
+        return (x * w + side).sin()
+
+    def run(**kw):
+        return checkpoint_fp8(f, x, {**dict(w=w, side=(side, )), **kw})
+
+    with pytest.raises(ValueError):
+        run(w=w * 2)
+    out = run()
+    side.add_(1)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        out.sum().backward()
+    out = run()
+    out.sum().backward(retain_graph=True)
+    once = w.grad.clone(), x.grad.clone()
+    out.sum().backward()
+    assert torch.equal(w.grad, 2 * once[0]) and torch.equal(x.grad, 2 * once[1])
+    kept = cast.cast_blocks_from_fp8(*cast.cast_blocks_to_fp8(x.detach()), torch.float32).requires_grad_(True)
+    w.grad = None
+    f(kept, dict(w=w, side=(side, ))).sum().backward()
+    assert torch.equal(w.grad, once[0]) and torch.equal(kept.grad, once[1])
+
+
 def test_checkpoint_keeps_one_byte_per_element():
     seen = []
     lin = torch.nn.Linear(64, 64)
