@@ -57,6 +57,8 @@ def _check_all(q, k, freqs, positions):
         raise ValueError(f'rotary: frequencies are a float64 vector of 1 to 512 pairs (got {freqs.dtype}, {tuple(freqs.shape)})')
     if 2 * freqs.numel() > dim:
         raise ValueError(f'rotary: {freqs.numel()} pairs do not fit a head of {dim}')
+    if freqs.requires_grad:
+        raise ValueError('rotary: the frequencies get no gradient')
     if freqs.device != q.device:
         raise ValueError('rotary: q and the frequencies must be on one device')
     if k is not None:

@@ -175,6 +175,8 @@ def test_refusals():
         K.rotary(q.double(), None, f)
     with pytest.raises(ValueError):
         K.rotary(q, None, f.to('meta'))
+    with pytest.raises(ValueError):
+        K.rotary(q, None, f.clone().requires_grad_(True))
 
 
 def test_raw_refusals():
