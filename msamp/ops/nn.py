@@ -425,7 +425,7 @@ def _mappable(t):
 
 class _SharedCall:
     """What calls of the same sizes and strides share: their checks, and the fields of both argument blocks that are no addresses."""
-    __slots__ = ('fields', 'tail', 'strides', 'work', 'lse_shape', 'plan_size', 'split', 'args')
+    __slots__ = ('fields', 'tail', 'strides', 'partial', 'work', 'lse_shape', 'plan_size', 'split', 'args')
 
     def __init__(self, q, k, v, causal, scale, packed, ragged):
         B, S, nh, d = q.shape
@@ -443,8 +443,10 @@ class _SharedCall:
         self.tail = _pack_st[4](*dense, *grads)
         self.strides = (q.stride(), k.stride(), v.stride(), torch.empty((B, S, nh, d), device='meta').stride())
         with native.on_device(q):
-            self.work = _shared_workspace(B, nh, nkv, S, d, causal, ragged)
-        self.lse_shape = (2, B, nh, S)
+            # floats of the backward pass's workspace: partial sums of dK and dV where there may be several, rowsum(dO * O) behind them
+            self.partial = native.lib().msamp_attention_shared_partial(B, nh, nkv, S, d, causal, ragged)
+        self.work = self.partial + B * nh * S
+        self.lse_shape = (B, nh, S)
         # with lengths: the tiles that are not padding, listed by the forward pass for both passes
         self.plan_size = 2 + (B + 1) * ((S + 127) // 128) if ragged else 0
         self.split = ((B, S, nh + 2 * nkv, d), [nh, nkv, nkv]) if packed else None
@@ -471,17 +473,8 @@ def _shared_call(q, k, v, causal, scale, packed, lengths):
     return call
 
 
-def _shared_workspace(B, nh, nkv, S, d, causal, ragged):
-    """Floats of the backward pass's workspace: partial sums of dK and dV where there may be several."""
-    return native.lib().msamp_attention_shared_partial(B, nh, nkv, S, d, causal, ragged)
-
-
 def _shared_fwd(q, k, v, call, lengths):
-    """``(o, lse, plan)``.
-
-    ``lse`` is ``[2, B, heads, S]``: the log-sum-exps, and room for rowsum(dO * O) in the backward pass (1 / 64 of the size of ``o`` at
-    head size 128; an allocation there costs more than the kernel that fills it takes for short rows).
-    """
+    """``(o, lse, plan)``; ``lse`` is ``[B, heads, S]``."""
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty(call.lse_shape, dtype=torch.float32)
     plan = q.new_empty(call.plan_size, dtype=torch.int32) if call.plan_size else None
@@ -495,18 +488,20 @@ def _shared_fwd(q, k, v, call, lengths):
     return o, lse, plan
 
 
-def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, work, tail):
+def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call, tail):
     """Gradients into ``dq``, ``dk`` and ``dv``; ``tail``: packed strides of ``d_o`` and of theirs."""
     lse = lse.contiguous()
     if lengths is not None:
         lengths, plan = lengths.contiguous(), plan.contiguous()
-    space = q.new_empty(work, dtype=torch.float32) if work else None
+    # of this call alone: saved tensors may serve several backward passes, captured ones too
+    space = q.new_empty(call.work, dtype=torch.float32)
+    at = space.data_ptr()
     with native.on_device(q):
         native.check(
             native.lib().msamp_attention_shared_bwd(
                 _pack_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
                           0 if plan is None else plan.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                          lse.data_ptr() + 2 * lse.numel(), 0 if space is None else space.data_ptr()) + fields + tail, native.raw_stream()
+                          at + 4 * call.partial, at if call.partial else 0) + fields + tail, native.raw_stream()
             ), 'attention_bwd'
         )
 
@@ -536,7 +531,7 @@ class _AttentionSharedFn(torch.autograd.Function):
             dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         else:
             dq, dk, dv = q.new_empty(call.split[0]).split(call.split[1], dim=2)
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call.work, tail)
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call, tail)
         return dq, dk, dv, None, None
 
 
@@ -611,10 +606,17 @@ def attention_shared_bwd_raw(q, k, v, o, lse, plan, d_o, dq, dk, dv, causal=True
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     if _use_native(q) and q.numel():
         q, k, v, lengths, call = _shared_operands(q, k, v, causal, scale, False, lengths)
-        o, d_o = _rows16(_mappable(o)), _rows16(_mappable(d_o))
+        for t, like in ((o, q), (d_o, q), (dq, q), (dk, k), (dv, v)):
+            if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+                raise ValueError(f'attention: {tuple(t.shape)} {t.dtype} in the place of {tuple(like.shape)} {like.dtype}')
+            if t.stride(3) != 1 and t is not o and t is not d_o:
+                raise ValueError('attention: gradients must have unit inner stride')
         B, S, nh, d = q.shape
+        if lse.shape != (B, nh, S) or lse.dtype != torch.float32 or (0 if plan is None else plan.numel()) != call.plan_size:
+            raise ValueError(f'attention: log-sum-exps {tuple(lse.shape)} or plan of another forward pass')
+        o, d_o = _rows16(_mappable(o)), _rows16(_mappable(d_o))
         fields = _pack_sizes(B, nh, k.shape[2], S, d, *call.args) + _pack_st[4](*(x for t in (q, k, v, o) for x in _map_strides(t)))
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call.work,
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call,
                     _pack_st[4](*(x for t in (d_o, dq, dk, dv) for x in _map_strides(t))))
         return
     with torch.enable_grad():

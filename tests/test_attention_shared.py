@@ -157,7 +157,7 @@ def test_list_of_tiles(B, S, causal):
     plan = plan.tolist()
     assert plan[0] == len(want) and plan[1] in (1, 2) and plan[2:2 + len(want)] == want
     pad = (torch.arange(S) >= n[:, None]).cuda()
-    assert torch.equal(torch.isinf(lse[0]).all(1), pad) and not o.any()
+    assert torch.equal(torch.isinf(lse).all(1), pad) and not o.any()
     _status_ok()
 
 
@@ -282,6 +282,40 @@ def test_saved_tensors_in_other_layouts(d, lengths):
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
             got = _run(q, k, v, do, True, n)
         assert all(torch.equal(a, b) for a, b in zip(want, got))
+    _status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('S, lengths', [(100, None), (300, None), (300, [300, 7, 0])])
+def test_backward_leaves_saved_tensors_alone(S, lengths):
+    """Two backward passes of one forward pass, captured ones too, share nothing that either writes."""
+    q, k, v, do = _inputs(3, S, 4, 2, 64, 'cuda')
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device='cuda')
+    kept = []
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        out = K.attention(*leaves, causal=True, lengths=n)
+    before = [t.clone() for t in kept]
+    one = torch.autograd.grad(out, leaves, do, retain_graph=True)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(kept, before))
+    torch.autograd.grad(out, leaves, 2 * do, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(one, torch.autograd.grad(out, leaves, do)))
+    _status_ok()
+
+
+@pytest.mark.gpu
+def test_raw_backward_refusals():
+    q, k, v, do = _inputs(2, 40, 4, 2, 64, 'cuda')
+    n = torch.tensor([40, 7], dtype=torch.int32, device='cuda')
+    o, lse, plan = K.attention_shared_fwd_raw(q, k, v, lengths=n)
+    dq, dk, dv = (torch.empty_like(t) for t in (q, k, v))
+    good = [q, k, v, o, lse, plan, do, dq, dk, dv]
+    for at, bad in ((3, o[:, :39]), (4, lse[0]), (4, lse.half()), (5, None), (5, plan[:2]), (6, do.float()), (7, dk), (8, dk[:1]), (9, dv.cpu()),
+                    (7, torch.empty(2, 40, 64, 4, dtype=torch.bfloat16, device='cuda').mT)):
+        with pytest.raises(ValueError):
+            K.attention_shared_bwd_raw(*good[:at], bad, *good[at + 1:], lengths=n)
+    K.attention_shared_bwd_raw(*good, lengths=n)
+    assert all(t.isfinite().all() for t in (dq, dk, dv))
     _status_ok()
 
 

@@ -266,7 +266,7 @@ def test_positions_refused(fp8):
 def test_changed_before_the_backward_pass(device, fp8, which):
     """Gradients need the positions and lengths of the forward pass: overwritten ones are an error, not other gradients."""
     model = _model(device, **LONG)
-    model = LinearReplacer.replace(model) if fp8 else model
+    model = LinearReplacer.replace(model) if fp8 else model.to(model.act_dtype)
     tokens, labels, lengths = _batch(device)
     given = dict(lengths=lengths.int(), positions=torch.arange(24, device=device))
     loss = model(tokens, labels, **given)
