@@ -580,13 +580,20 @@ def _check_shared(q, k, v, scale, lengths):
         _check_lengths(q, lengths)
 
 
+def _lengths32(lengths, S):
+    """Lengths as the kernels read them; they clamp int32 ones themselves, int64 ones would wrap on the way."""
+    if lengths.dtype != torch.int32:
+        lengths = lengths.clamp(0, S).to(torch.int32)
+    return lengths.contiguous()
+
+
 def _shared_operands(q, k, v, causal, scale, packed, lengths):
     """Mappable views, lengths in int32, and the shared fields of the call."""
     if len(q.shape) == len(k.shape) == len(v.shape) == 4:
         q, k, v = _mappable(q), _mappable(k), _mappable(v)
     call = _shared_call(q, k, v, bool(causal), float(scale), packed, lengths)
     if lengths is not None:
-        lengths = lengths.to(torch.int32).contiguous()
+        lengths = _lengths32(lengths, q.shape[1])
     return q, k, v, lengths, call
 
 

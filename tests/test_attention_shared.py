@@ -439,3 +439,28 @@ def test_on_a_side_stream():
     torch.cuda.current_stream().wait_stream(s)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
     _status_ok()
+
+
+FAR = (2**63 - 1, 2**31 + 3, 2**32 + 2, 2**31, -2**63, -2**31 - 5, -2**32 + 2, 5)
+NEAR = (9, 9, 9, 9, 0, 0, 0, 5)    # the same in rows of 9
+
+
+def test_far_lengths_as_int32():
+    got = K._lengths32(torch.tensor(FAR), 9)
+    assert got.dtype == torch.int32 and got.tolist() == list(NEAR)
+    same = torch.tensor([3, -2**31, 2**31 - 1], dtype=torch.int32)
+    assert torch.equal(K._lengths32(same, 9), same)    # the kernels clamp those
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('d', [64, 128])
+def test_far_lengths(device, d):
+    """Lengths outside of 0 .. S count as 0 or S, int64 ones that no int32 holds as well."""
+    q, k, v, do = _inputs(len(FAR), 9, 4, 2, d, device)
+    near = torch.tensor(NEAR, device=device)
+    want, valid = _reference(q, k, v, do, True, near, d**-0.5)
+    got = _run(q, k, v, do, True, torch.tensor(FAR, device=device))
+    _compare(got, want, valid)
+    assert all(torch.equal(a, b) for a, b in zip(got, _run(q, k, v, do, True, near)))
+    if device == 'cuda':
+        _status_ok()
