@@ -34,10 +34,21 @@ class _CheckpointFp8Fn(torch.autograd.Function):
         if preserve_rng_state:
             ctx.rng = (torch.get_rng_state(), torch.cuda.get_rng_state(x.device) if x.is_cuda else None)
         ctx.save_for_backward(*_c.cast_blocks_to_fp8(x))    # before the function, which may change x
+        before = _versions(args)
         with torch.no_grad():
             out = function(x, *args)
         ctx.versions = _versions(args)    # after the function, which may change them (a cache, a counter)
-        return out if isinstance(out, torch.Tensor) else tuple(out)
+        # Aliases of the outputs: the function may hand back a tensor that is the caller's (an argument, a buffer, a parameter), which
+        # would otherwise become an output of this node itself.  x is an input of the node, autograd makes an alias of it.
+        outs, plain = list(_outputs(out)), {id(a) for a, version in before if not a.requires_grad and a._version == version}
+        constant = []
+        for i, o in enumerate(outs):
+            if isinstance(o, torch.Tensor) and o is not x:
+                outs[i] = o.detach()
+                if id(o) in plain:
+                    constant.append(outs[i])
+        ctx.mark_non_differentiable(*constant)
+        return outs[0] if isinstance(out, torch.Tensor) else tuple(outs)
 
     @staticmethod
     def backward(ctx, *grads):
@@ -67,7 +78,9 @@ def checkpoint_fp8(function, x, *args, preserve_rng_state=True):
     ``x`` (fp32, fp16 or bf16) is stored as e4m3 with a power-of-two scale per 32 elements (1.03 bytes each,
     :func:`msamp.ops.cast.cast_blocks_to_fp8`), so the outputs are those of ``function(x)`` and the gradients those at the stored
     value, which is within 2^-4 of every element (of the small ones of a block: within 2^-17 of its largest).  Scaling metas of FP8
-    layers record the amaxes of the second run.  ``function`` returns a tensor or a tuple of tensors.  ``args`` are handed on as they
+    layers record the amaxes of the second run.  ``function`` returns a tensor or a tuple of tensors; what it returns of its ``args``, or of
+    tensors that it holds, comes back as an alias.  Its outputs count as computed with gradients, except those of ``args`` that need none
+    and are as they were: one that it detaches says that it requires a gradient and passes none on.  ``args`` are handed on as they
     are; a tensor among them that is computed from others with gradients is refused, as its gradient would not wait for its other uses.
     Parameters, also among ``args``, receive their gradients in ``.grad``: use ``backward()``, not ``torch.autograd.grad``.  The random
     state of the first run is used again unless ``preserve_rng_state`` is false.

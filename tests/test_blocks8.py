@@ -370,3 +370,44 @@ def test_checkpoint_keeps_one_byte_per_element():
 
 def test_public_names():
     assert msamp.nn.checkpoint_fp8 is checkpoint_fp8 and 'checkpoint_fp8' in msamp.nn.__all__
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+def test_checkpoint_leaves_what_the_function_hands_back_alone(device):
+    """A function may return an argument, a buffer or a parameter: the caller's tensors keep their place in autograd."""
+    x = torch.ones(2, 32, device=device, requires_grad=True)
+    argument, buffer, nested = (torch.zeros(3, device=device) for _ in range(3))
+    count = torch.zeros(2, dtype=torch.int64, device=device)
+    weight = torch.nn.Parameter(torch.full((32, ), 3.0, device=device))
+    handed = torch.nn.Parameter(torch.full((4, ), 2.0, device=device))
+
+    def f(t, a, parts, w):
+        count.add_(1)
+        y = t * weight
+        return y, a, buffer, weight, w, parts['n'], count, y, t
+
+    out = checkpoint_fp8(f, x, argument, dict(n=nested), handed)
+    for t in (argument, buffer, nested, count):
+        assert not t.requires_grad and t.grad_fn is None and t.is_leaf
+    for t in (weight, handed):
+        assert t.requires_grad and t.grad_fn is None and t.is_leaf
+    assert all(a.data_ptr() == b.data_ptr() for a, b in zip(out[1:7], (argument, buffer, weight, handed, nested, count)))
+    # arguments that need no gradient come back as such, as does what is no floating-point number
+    assert not out[1].requires_grad and not out[5].requires_grad and not out[6].requires_grad
+    (out[0].sum() + 2 * out[7].sum() + 5 * out[8].sum() + 7 * out[3].sum() + 11 * out[4].sum()).backward()
+    assert torch.equal(x.grad, torch.full((2, 32), 3.0 * 3 + 5, device=device))
+    assert torch.equal(weight.grad, torch.full((32, ), 3.0 * 2 + 7, device=device)) and torch.equal(handed.grad, torch.full((4, ), 11.0, device=device))
+
+
+def test_checkpoint_of_one_returned_argument():
+    x, cache = torch.ones(2, 32, requires_grad=True), torch.zeros(4)
+    out = checkpoint_fp8(lambda t, c: c, x, cache)
+    assert out.data_ptr() == cache.data_ptr() and not out.requires_grad and not cache.requires_grad and cache.grad_fn is None
+
+
+def test_checkpoint_of_a_returned_argument_that_the_function_fills():
+    x, cache = torch.ones(2, 32, requires_grad=True), torch.zeros(2, 32)
+    out = checkpoint_fp8(lambda t, c: c.copy_(t * 3), x, cache)
+    assert out.requires_grad and not cache.requires_grad and torch.equal(cache, torch.full((2, 32), 3.0))
+    out.sum().backward()
+    assert torch.equal(x.grad, torch.full((2, 32), 3.0))
