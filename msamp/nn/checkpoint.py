@@ -1,7 +1,7 @@
 """Activation recomputation from an input that is kept in 8 bits."""
 import torch
 
-from msamp.ops import cast as _c
+from msamp.ops import cast as _c, native
 
 
 def _outputs(out):
@@ -91,6 +91,8 @@ def checkpoint_fp8(function, x, *args, preserve_rng_state=True):
         return function(x, *args)
     if any(t.requires_grad and not t.is_leaf for t in _tensors(args)):
         raise ValueError('checkpoint_fp8: only x may be computed from other tensors with gradients; give it to the function first, or detach the argument')
+    if any(native.carries_tangent(t) for t in _tensors(args)):
+        raise ValueError('checkpoint_fp8: an argument has a forward-mode tangent, which the function would not pass on')
     # the anchor makes the outputs part of the graph where only parameters need gradients
     anchor = torch.empty(0, requires_grad=True)
     return _CheckpointFp8Fn.apply(anchor, function, preserve_rng_state, args, x)

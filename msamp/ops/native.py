@@ -5,6 +5,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libmsamp_b200.so')
@@ -129,6 +130,17 @@ def on_device(t):
     if _raw_device is not None and t.device.index == _raw_device():
         return _here
     return torch.cuda.device(t.device)
+
+
+def carries_tangent(t):
+    """Whether ``t`` has a forward-mode tangent, which a kernel would drop (the autograd functions refuse one)."""
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
+def needs_function(*tensors):
+    """Whether a kernel on ``tensors`` (None among them) has to run in its autograd function: one asks for a gradient or carries a tangent."""
+    grad = torch.is_grad_enabled()
+    return any(t is not None and ((grad and t.requires_grad) or carries_tangent(t)) for t in tensors)
 
 
 def addr(t):

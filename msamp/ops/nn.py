@@ -638,7 +638,7 @@ def _attention_shared(q, k, v, causal, scale, grad_layout, lengths):
         _check_shared(q, k, v, scale, lengths)
         return _attention_plain(q, k, v, causal, scale, lengths)
     q, k, v, lengths, call = _shared_operands(q, k, v, causal, scale, grad_layout == 'packed', lengths)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if native.needs_function(q, k, v):
         return _AttentionSharedFn.apply(q, k, v, lengths, call)
     return _shared_fwd(q, k, v, call, lengths)[0]
 

@@ -202,7 +202,7 @@ def rotary(q, k, freqs, positions=None, interleaved=False):
     """
     _check_all(q, k, freqs, positions)
     freqs = freqs.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if native.needs_function(q, k) if q.is_cuda else torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _RotaryFn.apply(q, k, freqs, positions, bool(interleaved))
     yq, yk, _ = _forward(q, k, freqs, positions, bool(interleaved))
     return yq if k is None else (yq, yk)

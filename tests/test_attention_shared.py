@@ -464,3 +464,21 @@ def test_far_lengths(device, d):
     assert all(torch.equal(a, b) for a, b in zip(got, _run(q, k, v, do, True, near)))
     if device == 'cuda':
         _status_ok()
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('grad', [False, True])
+@pytest.mark.parametrize('which', [0, 1, 2])
+def test_forward_mode_tangents_are_not_dropped(monkeypatch, device, which, grad):
+    """Plain operations carry a tangent (the CPU form); the autograd function refuses one."""
+    monkeypatch.setenv('PYTORCH_JIT', '0')    # make_dual compiles torch's own rules otherwise, which fails on functions that msamp wraps
+    from torch.autograd import forward_ad as fwd
+    args = list(_inputs(2, 9, 4, 2, 64, device)[:3])
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+        for n in (None, torch.tensor([9, 4], device=device)):
+            if device == 'cuda':
+                with pytest.raises((NotImplementedError, RuntimeError), match='forward'):
+                    K.attention(*args, lengths=n)
+            else:
+                assert fwd.unpack_dual(K.attention(*args, lengths=n)).tangent is not None

@@ -411,3 +411,33 @@ def test_checkpoint_of_a_returned_argument_that_the_function_fills():
     assert out.requires_grad and not cache.requires_grad and torch.equal(cache, torch.full((2, 32), 3.0))
     out.sum().backward()
     assert torch.equal(x.grad, torch.full((2, 32), 3.0))
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('offset', [0, 1])
+def test_gelu_does_not_drop_a_forward_mode_tangent(monkeypatch, device, offset):
+    monkeypatch.setenv('PYTORCH_JIT', '0')    # make_dual compiles torch's own rules otherwise, which fails on functions that msamp wraps
+    from torch.autograd import forward_ad as fwd
+    x = torch.randn(1025, device=device)[offset:offset + 1024]
+    with fwd.dual_level():
+        x = fwd.make_dual(x, torch.ones_like(x))
+        if device == 'cuda':
+            with pytest.raises((NotImplementedError, RuntimeError), match='forward'):
+                K.gelu(x, keep_fp8=True)
+        else:
+            assert fwd.unpack_dual(K.gelu(x, keep_fp8=True)).tangent is not None
+
+
+def test_checkpoint_refuses_forward_mode_tangents(monkeypatch):
+    """The function runs without gradients inside of the node, where a tangent would be lost."""
+    monkeypatch.setenv('PYTORCH_JIT', '0')    # make_dual compiles torch's own rules otherwise, which fails on functions that msamp wraps
+    from torch.autograd import forward_ad as fwd
+    x, side = torch.ones(2, 32), torch.ones(2, 32)
+    with fwd.dual_level():
+        dual = fwd.make_dual(torch.ones(2, 32), torch.ones(2, 32))
+        with pytest.raises((NotImplementedError, RuntimeError), match='forward'):
+            checkpoint_fp8(lambda t, s: t * s, dual, side)
+        with pytest.raises(ValueError, match='forward'):
+            checkpoint_fp8(lambda t, s: t * s['side'], x, dict(side=dual))
+        with torch.no_grad():
+            assert fwd.unpack_dual(checkpoint_fp8(lambda t, s: t * s, x, dual)).tangent is not None

@@ -238,3 +238,24 @@ def test_captured_and_on_a_side_stream():
     s.synchronize()
     assert torch.equal(y, z)
     assert native.device_status() == 0
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('which', ['q', 'k'])
+@pytest.mark.parametrize('grad', [False, True])
+def test_forward_mode_tangents_are_not_dropped(monkeypatch, device, which, grad):
+    """Plain operations carry a tangent (the CPU form where nothing asks for a gradient); the autograd function refuses one."""
+    monkeypatch.setenv('PYTORCH_JIT', '0')    # make_dual compiles torch's own rules otherwise, which fails on functions that msamp wraps
+    from torch.autograd import forward_ad as fwd
+    freqs = K.rotary_frequencies(64, device=device)
+    q, k, t = (torch.randn(2, 5, 4, 64, device=device).bfloat16() for _ in range(3))
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        given = dict(q=q, k=k)
+        given[which] = fwd.make_dual(given[which], t)
+        if device == 'cuda':
+            with pytest.raises((NotImplementedError, RuntimeError), match='forward'):
+                K.rotary(**given, freqs=freqs)
+        else:
+            y = K.rotary(**given, freqs=freqs)['qk'.index(which)]
+            tangent = fwd.unpack_dual(y).tangent
+            _check(tangent, t, freqs, None, False)
