@@ -52,6 +52,8 @@ class _CheckpointFp8Fn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
+        if torch.is_grad_enabled():
+            raise RuntimeError('checkpoint_fp8: no create_graph, as the gradients of the parameters get no graph')
         codes, exponents = ctx.saved_tensors
         if any(t._version != v for t, v in ctx.versions):
             raise RuntimeError('checkpoint_fp8: an argument was modified by an inplace operation before the backward pass ran the function again')
@@ -82,7 +84,8 @@ def checkpoint_fp8(function, x, *args, preserve_rng_state=True):
     tensors that it holds, comes back as an alias.  Its outputs count as computed with gradients, except those of ``args`` that need none
     and are as they were: one that it detaches says that it requires a gradient and passes none on.  ``args`` are handed on as they
     are; a tensor among them that is computed from others with gradients is refused, as its gradient would not wait for its other uses.
-    Parameters, also among ``args``, receive their gradients in ``.grad``: use ``backward()``, not ``torch.autograd.grad``.  The random
+    Parameters, also among ``args``, receive their gradients in ``.grad``: use ``backward()``, not ``torch.autograd.grad``, and not with
+    ``create_graph``.  The random
     state of the first run is used again unless ``preserve_rng_state`` is false.
     """
     if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):

@@ -12,6 +12,7 @@ import torch
 import torch.nn.functional as F
 
 from msamp.ops import cast as _c, native
+from msamp.ops.autograd import once
 from msamp.ops.rotary import rotary, rotary_frequencies, rotary_raw    # noqa: F401
 
 _i64x24 = ctypes.c_int64 * 24
@@ -194,6 +195,7 @@ class _GeluKeepFn(torch.autograd.Function):
         return F.gelu(x.float(), approximate='tanh').to(x.dtype)
 
     @staticmethod
+    @once
     def backward(ctx, dy):
         kept, *rest = ctx.saved_tensors
         if rest:
@@ -515,6 +517,7 @@ class _AttentionSharedFn(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once
     def backward(ctx, d_o):
         q, k, v, o, lse, lengths, plan = ctx.saved_tensors
         call = ctx.call

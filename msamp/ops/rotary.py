@@ -147,49 +147,54 @@ def _like(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def _forward(q, k, freqs, positions, interleaved):
+def _forward(q, k, freqs, positions, interleaved, inverse):
     """``(q', k' or None, fields)``; the last are what the gradient needs again on CUDA."""
     if not q.is_cuda:
-        return (_emulated(q, freqs, positions, interleaved, False).contiguous(),
-                None if k is None else _emulated(k, freqs, positions, interleaved, False).contiguous(), None)
+        return (_emulated(q, freqs, positions, interleaved, inverse).contiguous(),
+                None if k is None else _emulated(k, freqs, positions, interleaved, inverse).contiguous(), None)
     q = _unit_inner(q)
     batch, seq, heads, dim = q.shape
     if k is None:
         common = _common(freqs, positions, batch, seq, heads, 0, dim, interleaved)
         y = _like(q)
-        _turn(q, y, None, None, common, 0)
+        _turn(q, y, None, None, common, inverse)
         return y, None, common
     k = _unit_inner(k)
     common = _common(freqs, positions, batch, seq, heads, k.shape[2], dim, interleaved)
     yq, yk = _like(q), _like(k)
-    _turn(q, yq, k, yk, common, 0)
+    _turn(q, yq, k, yk, common, inverse)
     return yq, yk, common
 
 
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, freqs, positions, interleaved):
+    def forward(ctx, q, k, freqs, positions, interleaved, inverse):
         ctx.set_materialize_grads(False)
-        yq, yk, ctx.common = _forward(q, k, freqs, positions, interleaved)
+        yq, yk, ctx.common = _forward(q, k, freqs, positions, interleaved, inverse)
         ctx.save_for_backward(freqs, positions)
-        ctx.interleaved, ctx.freqs_at, ctx.positions_at = interleaved, freqs.data_ptr(), 0 if positions is None else positions.data_ptr()
+        ctx.interleaved, ctx.back, ctx.freqs_at, ctx.positions_at = interleaved, not inverse, freqs.data_ptr(), 0 if positions is None else positions.data_ptr()
         return yq if k is None else (yq, yk)
 
     @staticmethod
     def backward(ctx, gq, gk=None):
         freqs, positions = ctx.saved_tensors
+        if torch.is_grad_enabled() and (gq is not None or gk is not None):    # create_graph: the gradient is a rotation and has one too
+            given = [g for g in (gq, gk) if g is not None]
+            out = _RotaryFn.apply(given[0], given[1] if len(given) == 2 else None, freqs, positions, ctx.interleaved, ctx.back)
+            back = iter(out if len(given) == 2 else (out, ))
+            return (None if gq is None else next(back)), (None if gk is None else next(back)), None, None, None, None
         if gq is not None and gk is not None and gq.is_cuda and gq.is_contiguous() and gk.is_contiguous() and freqs.data_ptr() == ctx.freqs_at and (
                 positions is None or positions.data_ptr() == ctx.positions_at):
             # as a rule: both gradients, in the layout of the outputs, with the fields of the forward call
             dq, dk = torch.empty_like(gq), torch.empty_like(gk)
-            _turn(gq, dq, gk, dk, ctx.common, 1)
-            return dq, dk, None, None, None
+            _turn(gq, dq, gk, dk, ctx.common, ctx.back)
+            return dq, dk, None, None, None, None
         given = [_unit_inner(g) for g in (gq, gk) if g is not None]
         out = [_like(g) for g in given]
         if given:
-            rotary_raw(given, out, freqs, positions, ctx.interleaved, True)
+            rotary_raw(given, out, freqs, positions, ctx.interleaved, ctx.back)
         back = iter(out)
-        return (None if gq is None else next(back)), (None if gk is None else next(back)), None, None, None
+        return (None if gq is None else next(back)), (None if gk is None else next(back)), None, None, None, None
 
 
 def rotary(q, k, freqs, positions=None, interleaved=False):
@@ -203,6 +208,6 @@ def rotary(q, k, freqs, positions=None, interleaved=False):
     _check_all(q, k, freqs, positions)
     freqs = freqs.contiguous()
     if native.needs_function(q, k) if q.is_cuda else torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryFn.apply(q, k, freqs, positions, bool(interleaved))
-    yq, yk, _ = _forward(q, k, freqs, positions, bool(interleaved))
+        return _RotaryFn.apply(q, k, freqs, positions, bool(interleaved), False)
+    yq, yk, _ = _forward(q, k, freqs, positions, bool(interleaved), False)
     return yq if k is None else (yq, yk)

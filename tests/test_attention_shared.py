@@ -482,3 +482,24 @@ def test_forward_mode_tangents_are_not_dropped(monkeypatch, device, which, grad)
                     K.attention(*args, lengths=n)
             else:
                 assert fwd.unpack_dual(K.attention(*args, lengths=n)).tangent is not None
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('lengths', [None, (9, 4)])
+def test_second_derivatives(device, lengths):
+    """The CPU form differentiates twice; on CUDA the gradients have no gradient and say so, also where the incoming one is a constant."""
+    q, k, v, _ = _inputs(2, 9, 4, 2, 64, device)
+    n = None if lengths is None else torch.tensor(lengths, device=device)
+    for power in (1, 2):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+        o = K.attention(*leaves, lengths=n)
+        plain = torch.autograd.grad((o.float()**power).sum(), leaves, retain_graph=True)
+        first = torch.autograd.grad((o.float()**power).sum(), leaves, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, first)) and all(t.requires_grad for t in first[:2])
+        total = first[0].float().pow(2).sum() + leaves[0].float().sum()
+        if device == 'cuda':
+            with pytest.raises(RuntimeError, match='twice'):
+                total.backward()
+        else:
+            total.backward()
+            assert (leaves[0].grad.float() - 1.0).abs().sum() > 0

@@ -441,3 +441,27 @@ def test_checkpoint_refuses_forward_mode_tangents(monkeypatch):
             checkpoint_fp8(lambda t, s: t * s['side'], x, dict(side=dual))
         with torch.no_grad():
             assert fwd.unpack_dual(checkpoint_fp8(lambda t, s: t * s, x, dual)).tangent is not None
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('power', [1, 2])
+def test_gelu_refuses_second_derivatives(device, power):
+    """Its slope at the kept value has no gradient; a constant incoming gradient (power 1) does not hide that."""
+    x = torch.randn(64, device=device, requires_grad=True)
+    y = K.gelu(x, keep_fp8=True)
+    plain, = torch.autograd.grad((y**power).sum(), x, retain_graph=True)
+    first, = torch.autograd.grad((y**power).sum(), x, create_graph=True)
+    assert torch.equal(plain, first)
+    with pytest.raises(RuntimeError, match='twice'):
+        (first.pow(2).sum() + x.sum()).backward()
+
+
+def test_checkpoint_refuses_create_graph():
+    """The gradients of the parameters go to .grad without a graph, so there is nothing to differentiate again."""
+    x, w = torch.ones(2, 32, requires_grad=True), torch.ones(32, requires_grad=True)
+    out = checkpoint_fp8(lambda t: (t * w)**2, x)
+    with pytest.raises(RuntimeError, match='create_graph'):
+        out.sum().backward(create_graph=True)
+    assert w.grad is None and x.grad is None
+    out.sum().backward()
+    assert torch.equal(w.grad, torch.full((32, ), 4.0)) and torch.equal(x.grad, torch.full((2, 32), 2.0))

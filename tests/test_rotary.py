@@ -259,3 +259,34 @@ def test_forward_mode_tangents_are_not_dropped(monkeypatch, device, which, grad)
             y = K.rotary(**given, freqs=freqs)['qk'.index(which)]
             tangent = fwd.unpack_dual(y).tangent
             _check(tangent, t, freqs, None, False)
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('with_k', [False, True])
+def test_second_derivatives(device, with_k):
+    """y = R q, L = sum y^3: dL/dq = R^T 3 y^2, and the gradient of sum(w dL/dq) is R^T (6 y R w), which 64 bits give from the plain form."""
+    torch.manual_seed(3)
+    freqs, at = K.rotary_frequencies(16, device=device), torch.arange(5, device=device) + 100
+    q, w = (torch.randn(2, 5, 3, 20, device=device) for _ in range(2))
+    k, wk = (torch.randn(2, 5, 1, 20, device=device) for _ in range(2))
+
+    def second(turn, leaves, weights):
+        y = turn(*leaves)
+        first = torch.autograd.grad(sum((t**3).sum() for t in y), leaves, create_graph=True)
+        return first + torch.autograd.grad(sum((a * b).sum() for a, b in zip(first, weights)), leaves)
+
+    def mine(q, k=None):
+        y = K.rotary(q, k, freqs, positions=at, interleaved=True)
+        return y if k is not None else (y, )
+
+    def plain(*xs):
+        u = torch.polar(torch.ones(5, 8, dtype=torch.float64, device=device), at.double()[:, None] * freqs)[:, None]
+        turned = [torch.view_as_real(torch.view_as_complex(x[..., :16].unflatten(-1, (8, 2)).contiguous()) * u).flatten(-2) for x in xs]
+        return [torch.cat([t, x[..., 16:]], -1) for t, x in zip(turned, xs)]
+
+    xs, weights = ([q, k], [w, wk]) if with_k else ([q], [w])
+    got = second(mine, [x.clone().requires_grad_(True) for x in xs], weights)
+    want = second(plain, [x.double().requires_grad_(True) for x in xs], [t.double() for t in weights])
+    for a, b in zip(got, want):
+        # three rotations and two products in 32 bits of numbers up to 6 * 5^3
+        assert (a.double() - b).abs().max() <= 6 * 5.0**3 * 2.0**-20
