@@ -141,8 +141,8 @@ class GPT(nn.Module):
         self.cfg = cfg
         self.act_dtype = act_dtype
         self.wte = nn.Embedding(cfg.vocab_size, cfg.hidden, device=device, dtype=act_dtype)
-        if cfg.recompute not in (False, True, 'fp8'):
-            raise ValueError(f"recompute is False, True or 'fp8' (got {cfg.recompute!r})")
+        if isinstance(cfg.recompute, str) and cfg.recompute not in ('', 'fp8'):
+            raise ValueError(f"recompute goes by its truth, or is 'fp8' (got {cfg.recompute!r})")
         self.wpe = None if cfg.rotary_dim else nn.Embedding(cfg.max_seq, cfg.hidden, device=device, dtype=act_dtype)
         # a plain attribute: a float64 buffer would follow the module's casts to other dtypes
         self._freqs = K.rotary_frequencies(cfg.rotary_dim, cfg.rotary_base, cfg.rotary_scaling or None, cfg.rotary_factor,

@@ -286,3 +286,14 @@ def test_parameters_and_defaults():
 
 def test_block_casts_are_in_the_public_module():
     assert cast.cast_blocks_to_fp8(torch.zeros(3))[1].tolist() == [127]
+
+
+@pytest.mark.parametrize('recompute', [None, 0, 1, 2, [], [3], ''])
+def test_recompute_goes_by_its_truth(recompute):
+    """Any value but a string other than 'fp8', as before there was one."""
+    from unittest import mock
+    model = _model('cpu', recompute=recompute)
+    with mock.patch('torch.utils.checkpoint.checkpoint', side_effect=torch.utils.checkpoint.checkpoint) as again, \
+            mock.patch('msamp.models.gpt.checkpoint_fp8') as fp8:
+        model(*_batch('cpu')[:2]).backward()
+    assert again.called == bool(recompute) and not fp8.called
