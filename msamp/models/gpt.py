@@ -144,9 +144,9 @@ class GPT(nn.Module):
         if isinstance(cfg.recompute, str) and cfg.recompute not in ('', 'fp8'):
             raise ValueError(f"recompute goes by its truth, or is 'fp8' (got {cfg.recompute!r})")
         self.wpe = None if cfg.rotary_dim else nn.Embedding(cfg.max_seq, cfg.hidden, device=device, dtype=act_dtype)
-        # a plain attribute: a float64 buffer would follow the module's casts to other dtypes
+        # a plain attribute: a float64 buffer would follow the module's casts to other dtypes (and to_empty of a model built on 'meta')
         self._freqs = K.rotary_frequencies(cfg.rotary_dim, cfg.rotary_base, cfg.rotary_scaling or None, cfg.rotary_factor,
-                                           cfg.rotary_trained or None) if cfg.rotary_dim else None
+                                           cfg.rotary_trained or None, device='cpu') if cfg.rotary_dim else None
         self.blocks = nn.ModuleList(Block(cfg, device) for _ in range(cfg.n_layer))
         self.ln_f = LayerNorm(cfg.hidden, cfg.eps, device)
         self.lm_head = nn.Linear(cfg.hidden, cfg.vocab_size, bias=False, device=device)
@@ -171,7 +171,8 @@ class GPT(nn.Module):
                 raise ValueError('positions need a model with rotary positions (rotary_dim)')
             return None
         if self._freqs.device != device:
-            self._freqs = self._freqs.to(device)
+            with torch.inference_mode(False):    # kept for later calls, which may train
+                self._freqs = self._freqs.to(device)
         return self._freqs, positions, self.cfg.rotary_interleaved
 
     def forward(self, tokens, labels=None, lengths=None, positions=None):

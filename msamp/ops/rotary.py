@@ -32,7 +32,7 @@ def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, trained=None
         base = base * factor**(dim / (dim - 2))
     elif scaling not in (None, 'linear', 'parts'):
         raise ValueError(f"rotary_frequencies: scaling is None, 'linear', 'base' or 'parts' (got {scaling!r})")
-    f = torch.tensor([base**(-2.0 * i / dim) for i in range(dim // 2)], dtype=torch.float64)
+    f = torch.tensor([base**(-2.0 * i / dim) for i in range(dim // 2)], dtype=torch.float64, device=device)
     if scaling == 'linear':
         f = f / factor
     elif scaling == 'parts':
@@ -41,7 +41,7 @@ def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, trained=None
         turns = f * (trained / (2.0 * math.pi))
         keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
         f = f * keep + f / factor * (1.0 - keep)
-    return f.to(device) if device is not None else f
+    return f
 
 
 _TYPES = {torch.float32: native.DT_F32, torch.float16: native.DT_F16, torch.bfloat16: native.DT_BF16}

@@ -297,3 +297,21 @@ def test_recompute_goes_by_its_truth(recompute):
             mock.patch('msamp.models.gpt.checkpoint_fp8') as fp8:
         model(*_batch('cpu')[:2]).backward()
     assert again.called == bool(recompute) and not fp8.called
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('first', ['inference', 'meta'])
+def test_frequencies_of_the_model_serve_every_mode(device, first):
+    """A model whose first call, or whose construction, was under another mode or default device trains."""
+    if first == 'meta':
+        with torch.device('meta'):
+            model = GPT(_config(**LONG), act_dtype=torch.float32)
+        assert model._freqs.device.type == 'cpu'
+        return
+    model = GPT(_config(**LONG), device='cpu', act_dtype=torch.bfloat16 if device == 'cuda' else torch.float32).to(device)
+    model = model.to(model.act_dtype)
+    tokens, labels, _ = _batch(device)
+    with torch.inference_mode():
+        model(tokens)
+    assert not model._freqs.is_inference()
+    model(tokens, labels).backward()
