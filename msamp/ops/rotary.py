@@ -166,13 +166,20 @@ def _forward(q, k, freqs, positions, interleaved, inverse):
     return yq, yk, common
 
 
+def _layout(freqs, positions):
+    """What the fields of a call take from these two: saved tensors may come back with other strides, at the same address too."""
+    if positions is None:
+        return freqs.data_ptr(), freqs.stride()
+    return freqs.data_ptr(), freqs.stride(), positions.data_ptr(), positions.stride(), positions.dtype
+
+
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, freqs, positions, interleaved, inverse):
         ctx.set_materialize_grads(False)
         yq, yk, ctx.common = _forward(q, k, freqs, positions, interleaved, inverse)
         ctx.save_for_backward(freqs, positions)
-        ctx.interleaved, ctx.back, ctx.freqs_at, ctx.positions_at = interleaved, not inverse, freqs.data_ptr(), 0 if positions is None else positions.data_ptr()
+        ctx.interleaved, ctx.back, ctx.layout = interleaved, not inverse, _layout(freqs, positions)
         return yq if k is None else (yq, yk)
 
     @staticmethod
@@ -183,8 +190,8 @@ class _RotaryFn(torch.autograd.Function):
             out = _RotaryFn.apply(given[0], given[1] if len(given) == 2 else None, freqs, positions, ctx.interleaved, ctx.back)
             back = iter(out if len(given) == 2 else (out, ))
             return (None if gq is None else next(back)), (None if gk is None else next(back)), None, None, None, None
-        if gq is not None and gk is not None and gq.is_cuda and gq.is_contiguous() and gk.is_contiguous() and freqs.data_ptr() == ctx.freqs_at and (
-                positions is None or positions.data_ptr() == ctx.positions_at):
+        both = gq is not None and gk is not None and gq.is_cuda and gq.is_contiguous() and gk.is_contiguous()
+        if both and _layout(freqs, positions) == ctx.layout:
             # as a rule: both gradients, in the layout of the outputs, with the fields of the forward call
             dq, dk = torch.empty_like(gq), torch.empty_like(gk)
             _turn(gq, dq, gk, dk, ctx.common, ctx.back)

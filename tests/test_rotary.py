@@ -290,3 +290,36 @@ def test_second_derivatives(device, with_k):
     for a, b in zip(got, want):
         # three rotations and two products in 32 bits of numbers up to 6 * 5^3
         assert (a.double() - b).abs().max() <= 6 * 5.0**3 * 2.0**-20
+
+
+def test_fields_of_the_forward_call_hold_for_the_same_layout_only():
+    """Saved tensors may come back with other strides, in the place where the first ones were: their fields are worked out again."""
+    from msamp.ops.rotary import _layout
+    freqs, wide = K.rotary_frequencies(8), torch.arange(24).view(2, 12)
+    pos = wide[:, ::2]
+    here = _layout(freqs, pos)
+    assert here == _layout(freqs, wide[:, ::2]) and _layout(freqs, None) == _layout(freqs, None)
+    dense = torch.as_strided(wide, (2, 6), (6, 1))
+    assert dense.data_ptr() == pos.data_ptr()
+    for other in (dense, wide.int()[:, ::2], wide.clone()[:, ::2], None):
+        assert _layout(freqs, other) != here
+    assert _layout(freqs.clone(), pos) != here and _layout(torch.as_strided(freqs, (4, ), (0, )), pos) != here
+
+
+@pytest.mark.gpu
+def test_saved_positions_in_another_layout():
+    """Hooks that bring the positions back dense, and a hook that leaves them alone, against the call without hooks."""
+    torch.manual_seed(8)
+    freqs = K.rotary_frequencies(64, device='cuda')
+    q, k = torch.randn(2, 6, 4, 64, device='cuda'), torch.randn(2, 6, 2, 64, device='cuda')
+    g = torch.randn_like(q), torch.randn_like(k)
+    wide = torch.randint(0, 1000, (2, 12), device='cuda')
+    results = []
+    for pack in (None, lambda t: t, lambda t: t.clone(memory_format=torch.contiguous_format), lambda t: t.cpu()):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k)]
+        with torch.autograd.graph.saved_tensors_hooks(pack or (lambda t: t), lambda t: t.cuda()):
+            y = K.rotary(*leaves, freqs, positions=wide[:, ::2])
+        results.append(torch.autograd.grad(y, leaves, g))
+    for dq, dk in results:
+        assert torch.equal(dq, results[0][0]) and torch.equal(dk, results[0][1])
+        _check(dq, g[0], freqs, wide[:, ::2], False, inverse=True)
