@@ -622,8 +622,11 @@ def attention_shared_bwd_raw(q, k, v, o, lse, plan, d_o, dq, dk, dv, causal=True
             if t.stride(3) != 1 and t is not o and t is not d_o:
                 raise ValueError('attention: gradients must have unit inner stride')
         B, S, nh, d = q.shape
-        if lse.shape != (B, nh, S) or lse.dtype != torch.float32 or (0 if plan is None else plan.numel()) != call.plan_size:
-            raise ValueError(f'attention: log-sum-exps {tuple(lse.shape)} or plan of another forward pass')
+        if lse.shape != (B, nh, S) or lse.dtype != torch.float32 or lse.device != q.device:
+            raise ValueError(f'attention: log-sum-exps {tuple(lse.shape)} {lse.dtype} of another forward pass')
+        if (plan is not None) != bool(call.plan_size) or (plan is not None and (plan.numel() != call.plan_size or plan.dtype != torch.int32 or
+                                                                                plan.device != q.device)):
+            raise ValueError('attention: plan of another forward pass')
         o, d_o = _rows16(_mappable(o)), _rows16(_mappable(d_o))
         fields = _pack_sizes(B, nh, k.shape[2], S, d, *call.args) + _pack_st[4](*(x for t in (q, k, v, o) for x in _map_strides(t)))
         _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call,

@@ -503,3 +503,20 @@ def test_second_derivatives(device, lengths):
         else:
             total.backward()
             assert (leaves[0].grad.float() - 1.0).abs().sum() > 0
+
+
+@pytest.mark.gpu
+def test_raw_backward_refuses_saved_tensors_of_another_place_or_type():
+    """Addresses of the host's memory, or 64-bit words, never reach the kernels: the call is refused before its first launch."""
+    q, k, v, do = _inputs(2, 40, 4, 2, 64, 'cuda')
+    n = torch.tensor([40, 7], dtype=torch.int32, device='cuda')
+    o, lse, plan = K.attention_shared_fwd_raw(q, k, v, lengths=n)
+    dq, dk, dv = (torch.zeros_like(t) for t in (q, k, v))
+    good = [q, k, v, o, lse, plan, do, dq, dk, dv]
+    for at, bad in ((4, lse.cpu()), (4, lse.double()), (5, plan.cpu()), (5, plan.long()), (5, plan.float())):
+        with pytest.raises(ValueError):
+            K.attention_shared_bwd_raw(*good[:at], bad, *good[at + 1:], lengths=n)
+    with pytest.raises(ValueError):
+        K.attention_shared_bwd_raw(*good[:5], plan, *good[6:])    # a plan without lengths
+    _status_ok()
+    assert not dq.any() and not dk.any() and not dv.any()
