@@ -545,7 +545,8 @@ def _attention_plain(q, k, v, causal, scale, lengths):
         valid = torch.arange(S, device=q.device) < lengths.to(q.device)[:, None]
         q, k, v = (torch.where(valid[:, :, None, None], t, torch.zeros((), dtype=t.dtype, device=t.device)) for t in (q, k, v))
     qf, kf, vf = (t.float().permute(0, 2, 1, 3) for t in (q, k, v))
-    kf, vf = (t if t.shape[1] == nh else t.repeat_interleave(nh // t.shape[1], dim=1) for t in (kf, vf))
+    # a single head is broadcast, as is everything to a single query head
+    kf, vf = (t if t.shape[1] in (1, nh) or nh == 1 else t.repeat_interleave(nh // t.shape[1], dim=1) for t in (kf, vf))
     s = (qf @ kf.transpose(-1, -2)) * scale
     if causal:
         s = s.masked_fill(torch.ones(S, S, dtype=torch.bool, device=q.device).triu(1), float('-inf'))
@@ -662,7 +663,9 @@ def attention(q, k, v, causal=True, scale=None, grad_layout='separate', lengths=
     """
     d = q.shape[-1]
     scale = 1.0 / math.sqrt(d) if scale is None else scale
-    if lengths is not None or (q.dim() == k.dim() == 4 and k.shape[2] != q.shape[2] and (q.is_cuda or k.shape[:2] == q.shape[:2])):
+    shared = q.dim() == k.dim() == 4 and k.shape[2] != q.shape[2]
+    # CPU form: other batches or numbers of keys, and heads that broadcast, are whatever its products allow
+    if lengths is not None or (shared and (q.is_cuda or (k.shape[:2] == q.shape[:2] and 1 not in (q.shape[2], k.shape[2])))):
         return _attention_shared(q, k, v, causal, scale, grad_layout, lengths)
     if _use_native(q):
         if q.dtype != torch.bfloat16 or d not in (64, 128):

@@ -520,3 +520,18 @@ def test_raw_backward_refuses_saved_tensors_of_another_place_or_type():
         K.attention_shared_bwd_raw(*good[:5], plan, *good[6:])    # a plan without lengths
     _status_ok()
     assert not dq.any() and not dk.any() and not dv.any()
+
+
+@pytest.mark.parametrize('q_heads, k_heads, v_heads, keys, v_dim, scale', [(1, 4, 4, 5, 8, None), (1, 4, 4, 7, 8, None), (4, 1, 1, 5, 6, None),
+                                                                           (4, 1, 4, 5, 8, None), (4, 4, 1, 5, 8, None), (4, 1, 1, 7, 8, None),
+                                                                           (4, 1, 1, 5, 8, -0.3), (4, 1, 1, 5, 8, 0.0), (4, 2, 2, 7, 8, None)])
+def test_single_heads_on_the_cpu(q_heads, k_heads, v_heads, keys, v_dim, scale):
+    """On the CPU a single head has always served all heads of the other side, with any sizes that the products allow."""
+    torch.manual_seed(0)
+    q, k, v = torch.randn(2, 5, q_heads, 8), torch.randn(2, keys, k_heads, 8), torch.randn(2, keys, v_heads, v_dim)
+    n = max(q_heads, k_heads)
+    qn, kn, vn = (t.double().repeat_interleave(n // t.shape[2], 2) for t in (q, k, v))
+    x = torch.einsum('bihd,bjhd->bhij', qn, kn) * (8**-0.5 if scale is None else scale)
+    want = torch.einsum('bhij,bjhd->bihd', torch.softmax(x, -1), vn)
+    got = K.attention(q, k, v, causal=False, scale=scale)
+    assert got.shape == want.shape and torch.allclose(got.double(), want, rtol=1e-5, atol=1e-6)
