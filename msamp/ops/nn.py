@@ -670,6 +670,9 @@ def attention(q, k, v, causal=True, scale=None, grad_layout='separate', lengths=
     if _use_native(q):
         if q.dtype != torch.bfloat16 or d not in (64, 128):
             raise RuntimeError(f'attention: CUDA kernel supports bf16 with head_dim 64/128 (got {q.dtype}, {d})')
+        for t in (k, v):
+            if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
+                raise ValueError(f'attention: q {tuple(q.shape)} {q.dtype} and {tuple(t.shape)} {t.dtype} do not fit together')
         for t in (q, k, v):
             if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
                 raise RuntimeError('attention: operands must have unit inner stride and 16-byte aligned rows')

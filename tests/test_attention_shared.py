@@ -535,3 +535,14 @@ def test_single_heads_on_the_cpu(q_heads, k_heads, v_heads, keys, v_dim, scale):
     want = torch.einsum('bhij,bjhd->bihd', torch.softmax(x, -1), vn)
     got = K.attention(q, k, v, causal=False, scale=scale)
     assert got.shape == want.shape and torch.allclose(got.double(), want, rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.gpu
+def test_equal_heads_of_other_sizes_are_refused_on_cuda():
+    """The kernels take the sizes of q for k and v as well: others would be read past their end."""
+    q = torch.randn(2, 6, 4, 64, device='cuda').bfloat16()
+    for k, v in ((q[:, :5], q[:, :5]), (q, q[:, :5]), (q[:1], q[:1]), (q, q[:1]), (q, q[:, :, :2]), (q, q.float()), (q.half(), q), (q, q.cpu())):
+        with pytest.raises(ValueError):
+            K.attention(q, k, v, causal=False)
+    assert K.attention(q, q, q).isfinite().all()
+    _status_ok()
