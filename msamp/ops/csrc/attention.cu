@@ -26,7 +26,7 @@ struct AttnParams {
   float* lse;    // [b, h, s]
   // backward only
   const __nv_bfloat16* d_o;
-  const float* delta;    // [b, h, s] rowsum(dO * O)
+  float* delta;          // [b, h, s] rowsum(dO * O)
   __nv_bfloat16* dq;
   __nv_bfloat16* dk;
   __nv_bfloat16* dv;
@@ -290,7 +290,7 @@ __global__ void attn_delta_kernel(const AttnParams p) {
     acc += __bfloat162float(a.x) * __bfloat162float(e.x) + __bfloat162float(a.y) * __bfloat162float(e.y);
   }
   acc = warp_sum(acc);
-  if (lane == 0) const_cast<float*>(p.delta)[gw] = acc;
+  if (lane == 0) p.delta[gw] = acc;
 }
 
 // ===================================================================================== dK, dV
@@ -442,7 +442,10 @@ __global__ void __launch_bounds__(kAttnThreads) attn_bwd_dkdv_kernel(const AttnP
 }
 
 // ===================================================================================== dQ
-// CTA owns 64 query rows (16 per warp); loops over 64-row key tiles.
+// CTA owns 64 query rows (16 per warp); loops over 64-row key tiles.  Where the keys of its rows are one tile, delta is not rowsum(dO * O)
+// of the rounded output but sum P dP, in 32 bits from the tile, and is left for the dK / dV kernel, which comes after this one: with few
+// keys a row's dS is a small difference, and the rounding of O put the gradients of rows of 2 to 4 keys up to 1 % off in norm (one
+// rounding of dS: 0.3 %).  Rows of up to 64 keys need no delta kernel then.
 template <int D>
 __global__ void __launch_bounds__(kAttnThreads) attn_bwd_dq_kernel(const AttnParams p) {
   constexpr int BR = 64, BC = 64;
@@ -478,11 +481,12 @@ __global__ void __launch_bounds__(kAttnThreads) attn_bwd_dq_kernel(const AttnPar
 
   const int row_a = q0 + warp * 16 + g;
   const float* glse = p.lse + (int64_t)bh * p.seqlen;
-  const float* gdelta = p.delta + (int64_t)bh * p.seqlen;
+  float* gdelta = p.delta + (int64_t)bh * p.seqlen;
   const float lse0 = row_a < p.seqlen ? glse[row_a] : INFINITY;
   const float lse1 = row_a + 8 < p.seqlen ? glse[row_a + 8] : INFINITY;
-  const float dl0 = row_a < p.seqlen ? gdelta[row_a] : 0.0f;
-  const float dl1 = row_a + 8 < p.seqlen ? gdelta[row_a + 8] : 0.0f;
+  const bool one_tile = n_kv == 1;
+  float dl0 = !one_tile && row_a < p.seqlen ? gdelta[row_a] : 0.0f;
+  float dl1 = !one_tile && row_a + 8 < p.seqlen ? gdelta[row_a + 8] : 0.0f;
 
   float dq[D / 8][4];
 #pragma unroll
@@ -532,9 +536,29 @@ __global__ void __launch_bounds__(kAttnThreads) attn_bwd_dq_kernel(const AttnPar
         bool hi = (e >> 1) != 0;
         int row = row_a + (hi ? 8 : 0);
         bool masked = (col >= p.seqlen) || (row >= p.seqlen) || (p.causal && col > row);
-        float pv = masked ? 0.0f : exp2f((s[i][e] * p.scale - (hi ? lse1 : lse0)) * kLog2e);
-        s[i][e] = pv * (dp[i][e] - (hi ? dl1 : dl0)) * p.scale;    // dS
+        s[i][e] = masked ? 0.0f : exp2f((s[i][e] * p.scale - (hi ? lse1 : lse0)) * kLog2e);
       }
+    }
+    if (one_tile) {
+#pragma unroll
+      for (int i = 0; i < BC / 8; ++i) {
+        dl0 += s[i][0] * dp[i][0] + s[i][1] * dp[i][1];
+        dl1 += s[i][2] * dp[i][2] + s[i][3] * dp[i][3];
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {    // the four lanes of a row
+        dl0 += __shfl_xor_sync(0xffffffffu, dl0, o);
+        dl1 += __shfl_xor_sync(0xffffffffu, dl1, o);
+      }
+      if (t == 0) {
+        if (row_a < p.seqlen) gdelta[row_a] = dl0;
+        if (row_a + 8 < p.seqlen) gdelta[row_a + 8] = dl1;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < BC / 8; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] = s[i][e] * (dp[i][e] - ((e >> 1) ? dl1 : dl0)) * p.scale;    // dS
     }
     // dQ += dS K
 #pragma unroll
@@ -585,24 +609,23 @@ int run_fwd(const AttnParams& p, cudaStream_t stream) {
 
 template <int D>
 int run_bwd(const AttnParams& p, cudaStream_t stream) {
-  {
+  dim3 grid((p.seqlen + 63) / 64, p.batch * p.heads);
+  if (p.seqlen > 64) {    // else the dQ kernel finds delta itself
     int64_t warps = (int64_t)p.batch * p.heads * p.seqlen;
     int blocks = (int)((warps * 32 + 255) / 256);
     attn_delta_kernel<D><<<blocks, 256, 0, stream>>>(p);
   }
   {
-    constexpr int SMEM = 2 * 64 * D * 2 + 4 * 32 * D * 2 + 4 * 32 * 4;
-    int rc = set_smem(attn_bwd_dkdv_kernel<D>, SMEM);
-    if (rc) return rc;
-    dim3 grid((p.seqlen + 63) / 64, p.batch * p.heads);
-    attn_bwd_dkdv_kernel<D><<<grid, kAttnThreads, SMEM, stream>>>(p);
-  }
-  {
     constexpr int SMEM = 2 * 64 * D * 2 + 4 * 64 * D * 2;
     int rc = set_smem(attn_bwd_dq_kernel<D>, SMEM);
     if (rc) return rc;
-    dim3 grid((p.seqlen + 63) / 64, p.batch * p.heads);
     attn_bwd_dq_kernel<D><<<grid, kAttnThreads, SMEM, stream>>>(p);
+  }
+  {
+    constexpr int SMEM = 2 * 64 * D * 2 + 4 * 32 * D * 2 + 4 * 32 * 4;
+    int rc = set_smem(attn_bwd_dkdv_kernel<D>, SMEM);
+    if (rc) return rc;
+    attn_bwd_dkdv_kernel<D><<<grid, kAttnThreads, SMEM, stream>>>(p);
   }
   return msamp_check_launch("attn_bwd kernels");
 }
