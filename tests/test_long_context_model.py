@@ -315,3 +315,103 @@ def test_frequencies_of_the_model_serve_every_mode(device, first):
         model(tokens)
     assert not model._freqs.is_inference()
     model(tokens, labels).backward()
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('ffn', [512, 528])
+@pytest.mark.parametrize('delayed', [False, True])
+def test_mlp_sublayer_keeps_the_blocks_of_its_gelu_input(device, ffn, delayed):
+    """The kept bytes are those of a cast of the GeLU input that the sublayer without blocks keeps, and the input's gradient is bit for bit the one that this
+    sublayer gives when its kept GeLU input is replaced by what the bytes stand for."""
+    torch.manual_seed(0)
+    dt = torch.bfloat16 if device == 'cuda' else torch.float32
+
+    class Parts(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            from msamp.models.gpt import LayerNorm
+            self.ln, self.fc1, self.fc2 = LayerNorm(128), torch.nn.Linear(128, ffn), torch.nn.Linear(ffn, 128)
+
+    parts = LinearReplacer.replace(Parts().to(device))
+    x, dy = (3 * torch.randn(40, 128, device=device)).to(dt), torch.randn(40, 128, device=device).to(dt)
+    if delayed:
+        for lin in (parts.fc1, parts.fc2):
+            for meta in lin.scaling_metas.values():
+                meta.amax_counter.fill_(10**6) if isinstance(meta.amax_counter, torch.Tensor) else setattr(meta, 'amax_counter', 10**6)
+                meta.scale.fill_(8.0)
+    assert parts.fc2.scaling_metas['input'].is_in_time_scaling() != delayed
+
+    def run(keep, unpack):
+        leaf, kept = x.clone().requires_grad_(True), []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, unpack):
+            y = FL.mlp_sublayer(leaf, parts.ln, parts.fc1, parts.fc2, keep_fp8=keep)
+        y.backward(dy)
+        return leaf.grad, kept
+
+    got, kept = run(True, lambda t: t)
+    exps = [t for t in kept if t.dtype == torch.uint8 and t.shape == (40 * ffn // 32, )]
+    assert len(exps) == 1
+    replaced = []
+
+    def unpack(t):
+        if t.shape == (40, ffn) and t.dtype == dt:    # the GeLU input
+            codes, e = cast.cast_blocks_to_fp8(t)
+            assert torch.equal(e, exps[0]) and any(k.shape == (40, ffn) and k.dtype == torch.uint8 and torch.equal(k, codes) for k in kept)
+            replaced.append(t)
+            return cast.cast_blocks_from_fp8(codes, e, dt)
+        return t
+
+    want, _ = run(False, unpack)
+    assert len(replaced) == 1 and torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d, n, m, interleaved, lengths, seq', [(64, 4, 2, False, (150, 5, 0), 150), (64, 4, 4, True, (140, 129, 128), 150),
+                                                                (128, 4, 1, True, None, 200), (64, 6, 2, False, None, 40)])
+def test_fused_attention_sublayer_on_cuda_computes_what_the_separate_calls_compute(d, n, m, interleaved, lengths, seq):
+    """The rotation in place on the packed projection and on its packed gradient, and the attention on its strided views, against LayerNorm,
+    FP8 linear, rotary, attention, FP8 linear one by one.  All of them see the same bytes on both ways, so the weight gradients are equal bit for bit;
+    sums over the rows are in 32 bits in any order (fewer than 2^10 terms: 2^-14 of the sum of their sizes, far less in norm).  The fused
+    forms add the residual, or its gradient, before the rounding to bf16 and the separate ones after it as well: with u = 2^-8 and r the residual,
+    the sum s and the other term t = s - r the two differ by at most u |t| + 2 u |s| <= u (3 |s| + |r|)."""
+    torch.manual_seed(0)
+    h, b = n * d, 3
+
+    class Parts(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            from msamp.models.gpt import LayerNorm
+            self.ln, self.qkv, self.proj = LayerNorm(h), torch.nn.Linear(h, (n + 2 * m) * d), torch.nn.Linear(h, h)
+
+    parts = LinearReplacer.replace(Parts().cuda())
+    x, dy = (torch.randn(b * seq, h, device='cuda').bfloat16() for _ in range(2))
+    freqs = K.rotary_frequencies(d // 2, device='cuda')
+    at = torch.randint(0, 10000, (b, seq), device='cuda')
+    lens = None if lengths is None else torch.tensor(lengths, device='cuda')
+    results = []
+    for fused in (True, False):
+        for lin in (parts.qkv, parts.proj):
+            for meta in lin.scaling_metas.values():
+                meta.amax.zero_()
+                meta.scale.fill_(1.0)
+            lin.weight.grad = None
+        parts.zero_grad()
+        leaf = x.clone().requires_grad_(True)
+        if fused:
+            y = FL.attention_sublayer(leaf, parts.ln, parts.qkv, parts.proj, b, seq, n, n_kv_head=m, rope=(freqs, at, interleaved), lengths=lens)
+        else:
+            q, k, v = parts.qkv(parts.ln(leaf)).view(b, seq, -1, d).split([n, m, m], 2)
+            q, k = K.rotary(q, k, freqs, positions=at, interleaved=interleaved)
+            y = leaf + parts.proj(K.attention(q, k, v, lengths=lens).view(b * seq, -1))
+        y.backward(dy)
+        results.append((y.detach().float(), leaf.grad.float(), parts.qkv.weight.grad.float(), parts.proj.weight.grad.float(), parts.qkv.bias.grad.float(),
+                        parts.ln.weight.grad.float()))
+    (y, dx, *sums), (y2, dx2, *sums2) = results
+    u = 2.0**-8
+    assert (y - y2).norm() <= u * (3 * y2.norm() + x.float().norm()) and (dx - dx2).norm() <= u * (3 * dx2.norm() + dy.float().norm())
+    assert torch.equal(sums[0], sums2[0]) and torch.equal(sums[1], sums2[1])
+    for a, c in zip(sums[2:], sums2[2:]):
+        assert (a - c).norm() <= 2.0**-14 * c.norm()
+    for a in results[0]:
+        assert torch.isfinite(a).all() and a.abs().sum() > 0
+    assert native.device_status() == 0
