@@ -79,8 +79,8 @@ def checkpoint_fp8(function, x, *args, preserve_rng_state=True):
 
     ``x`` (fp32, fp16 or bf16) is stored as e4m3 with a power-of-two scale per 32 elements (1.03 bytes each,
     :func:`msamp.ops.cast.cast_blocks_to_fp8`), so the outputs are those of ``function(x)`` and the gradients those at the stored
-    value, which is within 2^-4 of every element (of the small ones of a block: within 2^-17 of its largest).  Scaling metas of FP8
-    layers record the amaxes of the second run.  ``function`` returns a tensor or a tuple of tensors; what it returns of its ``args``, or of
+    value, which is within 2^-4 of every element (of the small ones of a block: within 2^-17 of its largest, or 2^-137 if that is more).
+    Scaling metas of FP8 layers record the amaxes of the second run.  ``function`` returns a tensor or a tuple of tensors; what it returns of its ``args``, or of
     tensors that it holds, comes back as an alias.  Its outputs count as computed with gradients, except those of ``args`` that need none
     and are as they were: one that it detaches says that it requires a gradient and passes none on.  ``args`` are handed on as they
     are; a tensor among them that is computed from others with gradients is refused, as its gradient would not wait for its other uses.

@@ -325,7 +325,7 @@ def cast_blocks_to_fp8(x):
     Returns ``(codes, exponents)``: uint8 codes in the shape of ``x`` and one byte ``127 - k`` per block, where ``k <= 127`` is the largest
     shift that keeps the block's finite values times ``2**k`` within 448.  Nothing finite saturates; NaN and infinities become the NaN
     code and do not affect the rest of their block.  1.03 bytes per element, each value within 2^-4 of itself (below 2^-13 of the
-    largest of its block: within 2^-17 of that).
+    largest of its block: within 2^-17 of that; in a block below 2^-119, where ``k`` ends at 127: within 2^-137 or 2^-4 of itself).
     """
     if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f'cast_blocks_to_fp8: unsupported dtype {x.dtype}')

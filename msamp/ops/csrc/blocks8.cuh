@@ -4,7 +4,8 @@
 // so that every |x 2^k| is at most 448 and no finite value saturates; code = e4m3(x 2^k), nearest even; NaN and +-inf become the NaN
 // code and leave the rest of their block alone.  The exponent byte is 127 - k, i.e. the fp32 exponent field of 2^-k, and a code stands
 // for code * 2^-k.  k is read off the bits of a (448 = 1.75 * 2^8), and the products with 2^k are exact, so the rounding to e4m3 is the
-// only one: at most 2^-4 of a value that is above 2^-13 of its block's largest, and 2^-17 of the largest below that.
+// only one: at most 2^-4 of a value that is above 2^-13 of its block's largest, and 2^-17 of the largest below that.  Where k ends at 127, in
+// blocks below 2^-119, a value is off by 2^-4 of itself or by 2^-137, whichever is more.
 // The products with 2^k keep subnormal numbers (mul.rn.f32 written out: the library is compiled with flush-to-zero arithmetic).
 #pragma once
 #include "common.cuh"

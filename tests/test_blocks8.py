@@ -465,3 +465,22 @@ def test_checkpoint_refuses_create_graph():
     assert w.grad is None and x.grad is None
     out.sum().backward()
     assert torch.equal(w.grad, torch.full((32, ), 4.0)) and torch.equal(x.grad, torch.full((2, 32), 2.0))
+
+
+@pytest.mark.parametrize('device', CPU_GPU)
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_distance_of_the_smallest_blocks(device, dtype):
+    """The shift ends at 127: below 2^-119 the largest of a block no longer comes near 448.  The steps of e4m3's numbers below 2^-6 are 2^-9, here
+    2^-136, so a value is off by at most 2^-4 of itself or by 2^-137 (which may be all of it), whichever is more."""
+    gen = torch.Generator().manual_seed(2)
+    top = torch.exp2(-119.0 - 29.0 * torch.rand(256, 1, generator=gen, dtype=torch.float64))    # down to the last subnormal number
+    x = (top * torch.exp2(-14 * torch.rand(256, 32, generator=gen, dtype=torch.float64)) * torch.randn(256, 32, generator=gen).sign()).to(dtype).to(device)
+    codes, exps = cast.cast_blocks_to_fp8(x)
+    largest = x.double().abs().amax(1)
+    assert (exps[(largest < 2.0**-119) & (largest > 0)] == 0).all()    # k = 127 (blocks of zeros, which bf16 has here too: k = 0)
+    v = cast.cast_blocks_from_fp8(codes, exps, torch.float32).double()
+    err = (v - x.double()).abs()
+    assert (err <= torch.maximum(x.double().abs() * 2.0**-4, torch.tensor(2.0**-137, device=device, dtype=torch.float64))).all()
+    if dtype == torch.float32:    # the bounds for larger blocks do not hold here (bf16 has no numbers below 2^-133, which is 2^-6 2^-127)
+        lost = (x != 0) & (v == 0)
+        assert lost.any() and (err > x.double().abs() * 0.3)[~lost].any()
