@@ -134,13 +134,17 @@ def on_device(t):
 
 def carries_tangent(t):
     """Whether ``t`` has a forward-mode tangent, which a kernel would drop (the autograd functions refuse one)."""
-    return forward_ad.unpack_dual(t).tangent is not None
+    # the level that unpack_dual looks at first, an attribute of its module; the call takes 0.7 us
+    return getattr(forward_ad, '_current_level', 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
 def needs_function(*tensors):
     """Whether a kernel on ``tensors`` (None among them) has to run in its autograd function: one asks for a gradient or carries a tangent."""
     grad = torch.is_grad_enabled()
-    return any(t is not None and ((grad and t.requires_grad) or carries_tangent(t)) for t in tensors)
+    for t in tensors:
+        if t is not None and ((grad and t.requires_grad) or carries_tangent(t)):
+            return True
+    return False
 
 
 def addr(t):
