@@ -54,7 +54,7 @@ struct TcParams {
   unsigned int* status;
   // kernels with X only
   int kv_heads, rep;       // key / value heads; query heads of each
-  const int* lengths;      // X == 2: [batch] positions of a row that are not padding
+  const int* lengths;      // X == 2: [batch] positions of a row that are not padding, in the plan
   const int* plan;         // X == 2: the number of tiles that are not padding alone, parts, then those tiles (see attn_plan_kernel)
   int parts;               // X == 1, dK / dV: work items that share the query heads of a key / value head
   float* partial;          // [item][dK, dV][head_dim / 4][128 rows][4] when there are several
@@ -3645,25 +3645,33 @@ __host__ __device__ __forceinline__ int choose_parts(int rep, int64_t items, flo
 
 // Row lengths of a padded batch: the list of 128-row tiles that hold rows of a sequence, longest work first, and zeros (lse: -inf) for the
 // output rows of padding.  plan[0]: number of tiles; plan[1]: parts (choose_parts); plan[2 + rank]: b * n_tiles + i for tile i of batch b; then
-// n_tiles words of scratch.  The work of tile i is i + 1 tiles when causal, else those of its row; ties go by batch, then by tile.
+// n_tiles words of scratch; then the lengths, within 0 .. seqlen, which is where the other kernels of both passes read them.  The work of
+// tile i is i + 1 tiles when causal, else those of its row; ties go by batch, then by tile.
 // CTA 0 makes the list by counting: a warp takes one amount of work at a time, counts the batches that have it (ballots, in order, so that
 // nothing depends on timing), and after a scan over the amounts goes over them once more to place their tiles.  The other CTAs clear
 // padding, `share` of them for a batch.  Bound by latency, 6.5 us for 8 rows of up to 1000.  With the list the kernels of 16 x 577 x 16 heads
 // of 64 (lengths 10 to 577) took 46 + 97 us in the place of 63 + 139 us with an item for every tile, padding or not.
 struct PlanParams {
-  const int* lengths;
+  const void* lengths;    // int32, or int64 where len64
   int* plan;
+  int len64;
   __nv_bfloat16* o;
   float* lse;
   int64_t o_sb, o_ss, o_sh;
   int batch, heads, kv_heads, seqlen, head_dim, n_tiles, causal, sms, share;
 };
 constexpr int kPlanThreads = 512;
+// where the lengths begin in the plan
+__host__ __device__ __forceinline__ int64_t plan_lengths(int batch, int n_tiles) { return 2 + (int64_t)(batch + 1) * n_tiles; }
+__device__ __forceinline__ int given_length(const PlanParams& p, int b) {
+  if (p.len64) return (int)min(max(__ldg(reinterpret_cast<const long long*>(p.lengths) + b), 0ll), (long long)p.seqlen);
+  return row_length(reinterpret_cast<const int*>(p.lengths), b, p.seqlen);
+}
 __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PlanParams p) {
   if (blockIdx.x > 0) {
     const int b = (int)(blockIdx.x - 1) / p.share, first = (int)(blockIdx.x - 1) - b * p.share;
     const int shift = p.head_dim == 128 ? 4 : 3, per_row = p.heads << shift;    // 16-byte vectors of a head, of a row
-    for (int s = row_length(p.lengths, b, p.seqlen) + first; s < p.seqlen; s += p.share) {
+    for (int s = given_length(p, b) + first; s < p.seqlen; s += p.share) {
       for (int k = threadIdx.x; k < per_row; k += blockDim.x) {
         const int h = k >> shift, c = k - (h << shift);
         *reinterpret_cast<uint4*>(p.o + b * p.o_sb + s * p.o_ss + h * p.o_sh + c * 8) = make_uint4(0u, 0u, 0u, 0u);
@@ -3674,10 +3682,11 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PlanParam
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* start = p.plan + 2 + (int64_t)p.batch * p.n_tiles;
+  for (int b = threadIdx.x; b < p.batch; b += kPlanThreads) p.plan[plan_lengths(p.batch, p.n_tiles) + b] = given_length(p, b);
   // the batches b0 .. b0 + 31 that have tiles of lv + 1 tiles of work: one such tile each when causal, else all their lv + 1
   auto have = [&](int lv, int b0) {
     const int b = b0 + lane;
-    const int m = b < p.batch ? (row_length(p.lengths, b, p.seqlen) + 127) / 128 : 0;
+    const int m = b < p.batch ? (given_length(p, b) + 127) / 128 : 0;
     return __ballot_sync(0xffffffffu, p.causal ? m > lv : m == lv + 1);
   };
   for (int lv = warp; lv < p.n_tiles; lv += kPlanThreads / 32) {
@@ -4032,13 +4041,14 @@ MSAMP_API int msamp_attention_tc_bwd(const void* q, const void* k, const void* v
 }
 
 // ---- shared key / value heads and row lengths ----------------------------------------------------
-// Query heads h * rep .. h * rep + rep - 1 read key / value head h (heads == kv_heads * rep).  lengths [batch] (int32, or null): positions at or
-// behind a row's length are padding, as queries and as keys; their outputs and gradients are zero, their lse -inf, whatever they hold.  With
-// lengths the forward pass writes `plan` (2 + (batch + 1) * ceil(seqlen / 128) ints), which the backward pass of the same lengths reads.
+// Query heads h * rep .. h * rep + rep - 1 read key / value head h (heads == kv_heads * rep).  lengths [batch] (int32, int64, or null): positions
+// at or behind a row's length are padding, as queries and as keys; their outputs and gradients are zero, their lse -inf, whatever they hold.
+// With lengths the forward pass writes `plan` (2 + (batch + 1) * ceil(seqlen / 128) + batch ints).  The backward pass reads the lengths there:
+// its own argument says only that there are some.
 // Strides as for the entry points above, those of k, v, dk and dv over kv_heads.
 // Measured: 4 x 2048 x 32 / 8 heads of 128, causal, 199 + 494 us (equal heads 195 + 540 us); 1 x 4096 x 16 / 1 88 + 247 us; 2 x 4096 x 16 / 4
 // heads of 64 166 + 382 us; 8 x 1000 x 12 / 4 heads of 64 with lengths 18 to 1000 40 + 71 us.
-static int shared_checks(int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, const int* lengths, const int* plan,
+static int shared_checks(int batch, int heads, int kv_heads, int seqlen, int head_dim, float scale, const void* lengths, const int* plan,
                          const int64_t* strides, int n) {
   MSAMP_REQUIRE(head_dim == 64 || head_dim == 128, "attention (shared heads): head_dim must be 64 or 128 (got %d)", head_dim);
   MSAMP_REQUIRE(batch > 0 && heads > 0 && kv_heads > 0 && seqlen > 0, "attention (shared heads): empty problem");
@@ -4081,17 +4091,18 @@ static int launch_bwd(const CUtensorMap (&m)[4], const TcParams& p, int n_t, int
   return MSAMP_OK;
 }
 
+constexpr int64_t kCausal = 1, kLengths64 = 2;
 // The arguments of both passes come as one block of 64-bit fields, which a caller in Python packs several times faster than it passes
 // thirty arguments.
 struct SharedArgs {
-  int64_t batch, heads, kv_heads, seqlen, head_dim, causal;
+  int64_t batch, heads, kv_heads, seqlen, head_dim, flags;    // flags: kCausal, kLengths64
   double scale;
 };
 struct SharedFwdArgs {
   const void *q, *k, *v;
   void* o;
   float* lse;
-  const int* lengths;
+  const void* lengths;
   int* plan;
   SharedArgs n;
   int64_t strides[12];    // (batch, seq, head) element strides of q, k, v, o
@@ -4099,7 +4110,8 @@ struct SharedFwdArgs {
 struct SharedBwdArgs {
   const void *q, *k, *v, *o;
   const float* lse;
-  const int *lengths, *plan;
+  const void* lengths;
+  const int* plan;
   const void* d_o;
   void *dq, *dk, *dv;
   float *delta, *partial;    // [batch, heads, seqlen]; msamp_attention_shared_partial floats
@@ -4119,11 +4131,11 @@ MSAMP_API int msamp_attention_shared_fwd(const SharedFwdArgs* a, void* stream_) 
   const void *q = a->q, *k = a->k, *v = a->v;
   void* o = a->o;
   float* lse = a->lse;
-  const int* lengths = a->lengths;
+  const void* lengths = a->lengths;
   int* plan = a->plan;
   const int64_t* strides = a->strides;
   const int batch = (int)a->n.batch, heads = (int)a->n.heads, kv_heads = (int)a->n.kv_heads, seqlen = (int)a->n.seqlen, head_dim = (int)a->n.head_dim;
-  const int causal = a->n.causal != 0;
+  const int causal = (a->n.flags & kCausal) != 0;
   const float scale = (float)a->n.scale;
   int rc = shared_checks(batch, heads, kv_heads, seqlen, head_dim, scale, lengths, plan, strides, 12);
   if (rc) return rc;
@@ -4136,16 +4148,18 @@ MSAMP_API int msamp_attention_shared_fwd(const SharedFwdArgs* a, void* stream_) 
   p.o = (__nv_bfloat16*)o; p.lse = lse;
   p.o_sb = strides[9]; p.o_ss = strides[10]; p.o_sh = strides[11];
   p.batch = batch; p.heads = heads; p.seqlen = seqlen; p.causal = causal; p.scale = scale;
-  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.lengths = lengths; p.plan = plan;
+  const int n_qt = (seqlen + 127) / 128;
+  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.plan = plan;
+  if (lengths) p.lengths = plan + plan_lengths(batch, n_qt);
   p.status = msamp_device_status_ptr();
   p.group = item_group(seqlen, head_dim);
-  const int n_qt = (seqlen + 127) / 128;
   const int n_items = n_qt * batch * heads, sms = msamp_sm_count();
   const int ctas = n_items < sms ? n_items : sms;
   cudaStream_t stream = (cudaStream_t)stream_;
   if (lengths) {
     const int share = 2 * sms / batch < 1 ? 1 : 2 * sms / batch < 64 ? 2 * sms / batch : 64;
-    const PlanParams w = {lengths, plan, p.o, lse, p.o_sb, p.o_ss, p.o_sh, batch, heads, kv_heads, seqlen, head_dim, n_qt, causal, sms, share};
+    const PlanParams w = {lengths, plan, (a->n.flags & kLengths64) != 0, p.o, lse, p.o_sb, p.o_ss, p.o_sh, batch, heads, kv_heads, seqlen, head_dim,
+                          n_qt, causal, sms, share};
     attn_plan_kernel<<<(unsigned)batch * (unsigned)share + 1, kPlanThreads, 0, stream>>>(w);
     rc = head_dim == 128 ? launch_fwd<128, 2>(m, p, n_qt, ctas, stream) : launch_fwd<64, 2>(m, p, n_qt, ctas, stream);
   } else {
@@ -4181,10 +4195,11 @@ MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) 
   void *dq = a->dq, *dk = a->dk, *dv = a->dv;
   const float* lse = a->lse;
   float *delta = a->delta, *partial = a->partial;
-  const int *lengths = a->lengths, *plan = a->plan;
+  const void* lengths = a->lengths;
+  const int* plan = a->plan;
   const int64_t* strides = a->strides;
   const int batch = (int)a->n.batch, heads = (int)a->n.heads, kv_heads = (int)a->n.kv_heads, seqlen = (int)a->n.seqlen, head_dim = (int)a->n.head_dim;
-  const int causal = a->n.causal != 0;
+  const int causal = (a->n.flags & kCausal) != 0;
   const float scale = (float)a->n.scale;
   int rc = shared_checks(batch, heads, kv_heads, seqlen, head_dim, scale, lengths, plan, strides, 24);
   if (rc) return rc;
@@ -4206,7 +4221,9 @@ MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) 
   p.dk_sb = strides[18]; p.dk_ss = strides[19]; p.dk_sh = strides[20];
   p.dv_sb = strides[21]; p.dv_ss = strides[22]; p.dv_sh = strides[23];
   p.batch = batch; p.heads = heads; p.seqlen = seqlen; p.causal = causal; p.scale = scale;
-  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.lengths = lengths; p.plan = plan; p.parts = parts; p.partial = partial;
+  const int n_t = (seqlen + 127) / 128;    // key tiles of dK / dV, query tiles of dQ
+  p.kv_heads = kv_heads; p.rep = heads / kv_heads; p.plan = plan; p.parts = parts; p.partial = partial;
+  if (lengths) p.lengths = plan + plan_lengths(batch, n_t);
   p.status = msamp_device_status_ptr();
   p.group = item_group(seqlen, head_dim);
   if (lengths || seqlen > 128) {    // rows of one key tile: the dQ kernel finds delta itself
@@ -4215,7 +4232,7 @@ MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) 
     d.o_sb = strides[9]; d.o_ss = strides[10]; d.o_sh = strides[11];
     d.do_sb = strides[12]; d.do_ss = strides[13]; d.do_sh = strides[14];
     d.batch = batch; d.heads = heads; d.seqlen = seqlen;
-    d.lengths = lengths; d.kv_heads = kv_heads;
+    d.lengths = p.lengths; d.kv_heads = kv_heads;
     d.dq = p.dq; d.dq_sb = p.dq_sb; d.dq_ss = p.dq_ss; d.dq_sh = p.dq_sh;
     d.dk = p.dk; d.dk_sb = p.dk_sb; d.dk_ss = p.dk_ss; d.dk_sh = p.dk_sh;
     d.dv = p.dv; d.dv_sb = p.dv_sb; d.dv_ss = p.dv_ss; d.dv_sh = p.dv_sh;
@@ -4228,7 +4245,6 @@ MSAMP_API int msamp_attention_shared_bwd(const SharedBwdArgs* a, void* stream_) 
     else if (lengths)               attn_delta_tc_kernel<64, true><<<blocks, 256, 0, stream>>>(d);
     else                            attn_delta_tc_kernel<64, false><<<blocks, 256, 0, stream>>>(d);
   }
-  const int n_t = (seqlen + 127) / 128;    // key tiles of dK / dV, query tiles of dQ
   const int sms = msamp_sm_count();
   if (lengths) rc = head_dim == 128 ? launch_bwd<128, 2>(m, p, n_t, sms, stream) : launch_bwd<64, 2>(m, p, n_t, sms, stream);
   else         rc = head_dim == 128 ? launch_bwd<128, 1>(m, p, n_t, sms, stream) : launch_bwd<64, 1>(m, p, n_t, sms, stream);

@@ -399,7 +399,7 @@ def attention_qkv(qkv, causal=True, scale=None):
 
 
 # Attention whose query heads share key / value heads, on rows that may end early.  ``q [B, S, heads, d]``, ``k`` and ``v [B, S, kv_heads, d]``
-# as strided views, ``lengths`` int32 ``[B]`` or None.  The argument blocks of the native entry points: addresses, sizes and scale, strides.
+# as strided views, ``lengths`` ``[B]`` (int32 or int64) or None.  The argument blocks of the native entry points: addresses, sizes and scale, strides.
 _pack_fwd, _pack_bwd = struct.Struct('7q').pack, struct.Struct('13q').pack
 _pack_sizes, _pack_st = struct.Struct('6qd').pack, [struct.Struct(f'{3 * n}q').pack for n in range(9)]
 
@@ -429,7 +429,7 @@ class _SharedCall:
     """What calls of the same sizes and strides share: their checks, and the fields of both argument blocks that are no addresses."""
     __slots__ = ('fields', 'tail', 'strides', 'partial', 'work', 'lse_shape', 'plan_size', 'split', 'args')
 
-    def __init__(self, q, k, v, causal, scale, packed, ragged):
+    def __init__(self, q, k, v, causal, scale, packed, lengths):
         B, S, nh, d = q.shape
         nkv = k.shape[2]
         if q.dtype != torch.bfloat16 or d not in (64, 128):
@@ -437,9 +437,11 @@ class _SharedCall:
         for t in (q, k, v):
             if t.stride(3) != 1 or any(s & 7 for s in _map_strides(t)):
                 raise RuntimeError('attention: operands must have unit inner stride and 16-byte aligned rows')
-        self.args = (causal, scale)
+        ragged = lengths is not None
+        flags = int(causal) | (2 if lengths == torch.int64 else 0)
+        self.args = (flags, scale)
         dense = _dense_strides(S, nh, d)
-        self.fields = _pack_sizes(B, nh, nkv, S, d, causal, scale) + _pack_st[4](*_map_strides(q), *_map_strides(k), *_map_strides(v), *dense)
+        self.fields = _pack_sizes(B, nh, nkv, S, d, flags, scale) + _pack_st[4](*_map_strides(q), *_map_strides(k), *_map_strides(v), *dense)
         # dO as a rule in the layout of o, then dq, dk and dv
         grads = _dense_strides(S, nh + 2 * nkv, d) * 3 if packed else dense + _dense_strides(S, nkv, d) * 2
         self.tail = _pack_st[4](*dense, *grads)
@@ -449,8 +451,8 @@ class _SharedCall:
             self.partial = native.lib().msamp_attention_shared_partial(B, nh, nkv, S, d, causal, ragged)
         self.work = self.partial + B * nh * S
         self.lse_shape = (B, nh, S)
-        # with lengths: the tiles that are not padding, listed by the forward pass for both passes
-        self.plan_size = 2 + (B + 1) * ((S + 127) // 128) if ragged else 0
+        # with lengths: the tiles that are not padding, listed by the forward pass for both passes, and the lengths within 0 .. S
+        self.plan_size = 2 + (B + 1) * ((S + 127) // 128) + B if ragged else 0
         self.split = ((B, S, nh + 2 * nkv, d), [nh, nkv, nkv]) if packed else None
 
 
@@ -459,13 +461,14 @@ _shared_calls = {}
 
 def _shared_call(q, k, v, causal, scale, packed, lengths):
     """Checks and shared fields of a call, remembered by its sizes and strides."""
-    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), causal, scale, packed, lengths is None, q.device)
+    kind = None if lengths is None else lengths.dtype
+    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), causal, scale, packed, kind, q.device)
     call = _shared_calls.get(key)
     if call is None or q.dtype != torch.bfloat16:
         _check_shared(q, k, v, scale, lengths)
         if len(_shared_calls) > 1024:
             _shared_calls.clear()
-        call = _shared_calls[key] = _SharedCall(q, k, v, causal, scale, packed, lengths is not None)
+        call = _shared_calls[key] = _SharedCall(q, k, v, causal, scale, packed, kind)
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.device != q.device or v.device != q.device:
         _check_shared(q, k, v, scale, lengths)
     if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
@@ -490,20 +493,19 @@ def _shared_fwd(q, k, v, call, lengths):
     return o, lse, plan
 
 
-def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call, tail):
+def _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, plan, fields, call, tail):
     """Gradients into ``dq``, ``dk`` and ``dv``; ``tail``: packed strides of ``d_o`` and of theirs."""
     lse = lse.contiguous()
-    if lengths is not None:
-        lengths, plan = lengths.contiguous(), plan.contiguous()
+    plan = None if plan is None else plan.contiguous()
+    plan_at = 0 if plan is None else plan.data_ptr()    # holds the lengths too
     # of this call alone: saved tensors may serve several backward passes, captured ones too
     space = q.new_empty(call.work, dtype=torch.float32)
     at = space.data_ptr()
     with native.on_device(q):
         native.check(
             native.lib().msamp_attention_shared_bwd(
-                _pack_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-                          0 if plan is None else plan.data_ptr(), d_o.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                          at + 4 * call.partial, at if call.partial else 0) + fields + tail, native.raw_stream()
+                _pack_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), plan_at, plan_at, d_o.data_ptr(),
+                          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), at + 4 * call.partial, at if call.partial else 0) + fields + tail, native.raw_stream()
             ), 'attention_bwd'
         )
 
@@ -512,14 +514,15 @@ class _AttentionSharedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, call):
         o, lse, plan = _shared_fwd(q, k, v, call, lengths)
-        ctx.save_for_backward(q, k, v, o, lse, lengths, plan)
+        # int32 lengths are saved for the check that nothing has overwritten them; the backward pass has those of the plan
+        ctx.save_for_backward(q, k, v, o, lse, plan, lengths if lengths is not None and lengths.dtype == torch.int32 else None)
         ctx.call = call
         return o
 
     @staticmethod
     @once
     def backward(ctx, d_o):
-        q, k, v, o, lse, lengths, plan = ctx.saved_tensors
+        q, k, v, o, lse, plan, _ = ctx.saved_tensors
         call = ctx.call
         fields, tail = call.fields, call.tail
         if (q.stride(), k.stride(), v.stride(), o.stride()) != call.strides or (q.data_ptr() | k.data_ptr() | v.data_ptr() | o.data_ptr()) & 15:
@@ -534,7 +537,7 @@ class _AttentionSharedFn(torch.autograd.Function):
             dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         else:
             dq, dk, dv = q.new_empty(call.split[0]).split(call.split[1], dim=2)
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call, tail)
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, plan, fields, call, tail)
         return dq, dk, dv, None, None
 
 
@@ -584,20 +587,13 @@ def _check_shared(q, k, v, scale, lengths):
         _check_lengths(q, lengths)
 
 
-def _lengths32(lengths, S):
-    """Lengths as the kernels read them; they clamp int32 ones themselves, int64 ones would wrap on the way."""
-    if lengths.dtype != torch.int32:
-        lengths = lengths.clamp(0, S).to(torch.int32)
-    return lengths.contiguous()
-
-
 def _shared_operands(q, k, v, causal, scale, packed, lengths):
-    """Mappable views, lengths in int32, and the shared fields of the call."""
+    """Mappable views, dense lengths, and the shared fields of the call."""
     if len(q.shape) == len(k.shape) == len(v.shape) == 4:
         q, k, v = _mappable(q), _mappable(k), _mappable(v)
     call = _shared_call(q, k, v, bool(causal), float(scale), packed, lengths)
     if lengths is not None:
-        lengths = _lengths32(lengths, q.shape[1])
+        lengths = lengths.contiguous()
     return q, k, v, lengths, call
 
 
@@ -630,7 +626,7 @@ def attention_shared_bwd_raw(q, k, v, o, lse, plan, d_o, dq, dk, dv, causal=True
             raise ValueError('attention: plan of another forward pass')
         o, d_o = _rows16(_mappable(o)), _rows16(_mappable(d_o))
         fields = _pack_sizes(B, nh, k.shape[2], S, d, *call.args) + _pack_st[4](*(x for t in (q, k, v, o) for x in _map_strides(t)))
-        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, lengths, plan, fields, call,
+        _shared_bwd(q, k, v, o, lse, d_o, dq, dk, dv, plan, fields, call,
                     _pack_st[4](*(x for t in (d_o, dq, dk, dv) for x in _map_strides(t))))
         return
     with torch.enable_grad():

@@ -445,13 +445,6 @@ FAR = (2**63 - 1, 2**31 + 3, 2**32 + 2, 2**31, -2**63, -2**31 - 5, -2**32 + 2, 5
 NEAR = (9, 9, 9, 9, 0, 0, 0, 5)    # the same in rows of 9
 
 
-def test_far_lengths_as_int32():
-    got = K._lengths32(torch.tensor(FAR), 9)
-    assert got.dtype == torch.int32 and got.tolist() == list(NEAR)
-    same = torch.tensor([3, -2**31, 2**31 - 1], dtype=torch.int32)
-    assert torch.equal(K._lengths32(same, 9), same)    # the kernels clamp those
-
-
 @pytest.mark.parametrize('device', CPU_GPU)
 @pytest.mark.parametrize('d', [64, 128])
 def test_far_lengths(device, d):
@@ -573,4 +566,22 @@ def test_gradients_of_few_keys_in_norm_with_equal_heads(d, S, causal, packed):
         for name, a, (value, _) in zip(('o', 'dq', 'dk', 'dv'), got, want):
             err, size = (a.detach().double() - value).norm().item(), value.norm().item()
             assert err <= 0.005 * size + zero, (seed, name, err / size if size else err)
+    _status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', [torch.int32, torch.int64])
+def test_backward_takes_the_lengths_of_its_forward_pass(kind):
+    """Without autograd's version check (as in graphs that are replayed apart) other lengths in the same tensor change nothing between the passes."""
+    q, k, v, do = _inputs(3, 150, 4, 2, 64, 'cuda')
+    n = torch.tensor([150, 20, 0], dtype=kind, device='cuda')
+    o, lse, plan = K.attention_shared_fwd_raw(q, k, v, lengths=n)
+    grads = []
+    for other in ((150, 20, 0), (0, 150, 140)):
+        n.copy_(torch.tensor(other))
+        grads.append([torch.full_like(t, float('nan')) for t in (q, k, v)])
+        K.attention_shared_bwd_raw(q, k, v, o, lse, plan, do, *grads[-1], lengths=n)
+    want, valid = _reference(q, k, v, do, True, torch.tensor([150, 20, 0], device='cuda'), 64**-0.5)
+    _compare([o, *grads[0]], want, valid)
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
     _status_ok()
