@@ -307,14 +307,14 @@ def _gelu_keep(x):
     return kept, y
 
 
-def _gelu_keep_bwd(kept, dy):
-    """Its gradient for a contiguous ``dy``."""
-    n = dy.numel()
+def _gelu_keep_bwd(codes_at, exponents_at, dy):
+    """Its gradient for a contiguous ``dy`` and the blocks at these addresses."""
     dx = torch.empty_like(dy)
-    at = kept.data_ptr()
     with native.on_device(dy):
         native.check(
-            native.lib().msamp_blocks_uncast(at, at + n, dy.data_ptr(), dx.data_ptr(), n, native.dt(dy.dtype), native.raw_stream()), 'gelu_bwd'
+            native.lib().msamp_blocks_uncast(
+                codes_at, exponents_at, dy.data_ptr(), dx.data_ptr(), dy.numel(), native.dt(dy.dtype), native.raw_stream()
+            ), 'gelu_bwd'
         )
     return dx
 

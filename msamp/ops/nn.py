@@ -200,8 +200,8 @@ class _GeluKeepFn(torch.autograd.Function):
         kept, *rest = ctx.saved_tensors
         if rest:
             return gelu_bwd_blocks(kept, rest[0], dy)
-        dy = dy.contiguous()
-        return _c._gelu_keep_bwd(kept, dy)
+        at = kept.data_ptr()
+        return _c._gelu_keep_bwd(at, at + dy.numel(), dy.contiguous())
 
 
 def gelu_bwd_blocks(codes, exponents, dy):
@@ -210,15 +210,8 @@ def gelu_bwd_blocks(codes, exponents, dy):
     if codes.shape != dy.shape or codes.device != dy.device:
         raise ValueError(f'gelu: codes {tuple(codes.shape)} and gradient {tuple(dy.shape)} differ')
     if dy.is_cuda:
-        dy, codes, exponents = dy.contiguous(), codes.contiguous(), exponents.contiguous()
-        dx = torch.empty_like(dy)
-        with native.on_device(dy):
-            native.check(
-                native.lib().msamp_blocks_uncast(
-                    codes.data_ptr(), exponents.data_ptr(), dy.data_ptr(), dx.data_ptr(), dy.numel(), native.dt(dy.dtype), native.raw_stream()
-                ), 'gelu_bwd_blocks'
-            )
-        return dx
+        codes, exponents = codes.contiguous(), exponents.contiguous()
+        return _c._gelu_keep_bwd(codes.data_ptr(), exponents.data_ptr(), dy.contiguous())
     with torch.enable_grad():
         x = _c.cast_blocks_from_fp8(codes, exponents, torch.float32).requires_grad_(True)
         grad, = torch.autograd.grad(F.gelu(x, approximate='tanh'), x, dy.float())
