@@ -585,3 +585,32 @@ def test_backward_takes_the_lengths_of_its_forward_pass(kind):
     _compare([o, *grads[0]], want, valid)
     assert all(torch.equal(a, b) for a, b in zip(*grads))
     _status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('S, nh, nkv, lengths', [(5000, 2, 1, None), (4097, 2, 2, (4097, )), (6001, 1, 1, (5890, ))])
+def test_long_rows(d, S, nh, nkv, lengths):
+    q, k, v, do = _inputs(1, S, nh, nkv, d, 'cuda')
+    n = None if lengths is None else torch.tensor(lengths, device='cuda')
+    want, valid = _reference(q, k, v, do, True, n, d**-0.5)
+    _compare(_run(q, k, v, do, True, n), want, valid)
+    _status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('lengths', [None, (150, 70)])
+def test_offsets_beyond_32_bits(lengths):
+    """Two batches of a packed projection that lie more than 2^31 elements apart."""
+    S, nh, nkv, d = 150, 4, 2, 64
+    width = (nh + 2 * nkv) * d
+    buf = torch.zeros(2**31 + 8 * width + S * width, dtype=torch.bfloat16, device='cuda')
+    x = buf.as_strided((2, S, nh + 2 * nkv, d), (2**31 + 8 * width, width, d, 1))
+    q, k, v, do = _inputs(2, S, nh, nkv, d, 'cuda')
+    for part, at in ((q, 0), (k, nh), (v, nh + nkv)):
+        x[:, :, at:at + part.shape[2]] = part
+    n = None if lengths is None else torch.tensor(lengths, device='cuda')
+    want = _run(q, k, v, do, True, n)
+    got = _run(*x.split([nh, nkv, nkv], 2), do, True, n)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _status_ok()

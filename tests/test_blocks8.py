@@ -484,3 +484,27 @@ def test_distance_of_the_smallest_blocks(device, dtype):
     if dtype == torch.float32:    # the bounds for larger blocks do not hold here (bf16 has no numbers below 2^-133, which is 2^-6 2^-127)
         lost = (x != 0) & (v == 0)
         assert lost.any() and (err > x.double().abs() * 0.3)[~lost].any()
+
+
+@pytest.mark.gpu
+def test_more_elements_than_32_bits_count():
+    n, tail = 2**31 + 1000, 4096 + 1000
+    end = torch.randn(tail, device='cuda').half()
+    x = torch.zeros(n, dtype=torch.float16, device='cuda')
+    x[-tail:] = end
+    start = n - tail    # a multiple of 32, so that the tail is whole blocks
+    assert start % 32 == 0
+    codes, exps = cast.cast_blocks_to_fp8(x)
+    want, e = cast.cast_blocks_to_fp8(end)
+    assert torch.equal(codes[start:], want) and torch.equal(exps[start // 32:], e) and (exps[:start // 32] == 127).all()
+    back = cast.cast_blocks_from_fp8(codes, exps, torch.float16)
+    assert torch.equal(back[start:], cast.cast_blocks_from_fp8(want, e, torch.float16)) and back[:start].count_nonzero() == 0
+    del back, codes, exps
+    y = K.gelu(x.requires_grad_(True), keep_fp8=True)
+    small = end.clone().requires_grad_(True)
+    z = K.gelu(small, keep_fp8=True)
+    dz = torch.randn_like(z)
+    dy = torch.zeros_like(y)
+    dy[start:] = dz
+    dx, = torch.autograd.grad(y, x, dy)
+    assert torch.equal(y[start:], z) and torch.equal(dx[start:], torch.autograd.grad(z, small, dz)[0]) and dx[:start].count_nonzero() == 0

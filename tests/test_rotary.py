@@ -323,3 +323,19 @@ def test_saved_positions_in_another_layout():
     for dq, dk in results:
         assert torch.equal(dq, results[0][0]) and torch.equal(dk, results[0][1])
         _check(dq, g[0], freqs, wide[:, ::2], False, inverse=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('interleaved', [False, True])
+def test_offsets_beyond_32_bits(interleaved):
+    torch.manual_seed(2)
+    buf = torch.zeros(2**31 + 4096, dtype=torch.bfloat16, device='cuda')
+    x = buf.as_strided((2, 3, 2, 64), (2**31 + 256, 128, 64, 1))
+    q = torch.randn(2, 3, 2, 64, device='cuda').bfloat16()
+    x.copy_(q)
+    freqs = K.rotary_frequencies(64, device='cuda')
+    want = K.rotary(q, None, freqs, interleaved=interleaved)
+    assert torch.equal(K.rotary(x, None, freqs, interleaved=interleaved), want)
+    K.rotary_raw([x], [x], freqs, None, interleaved, False)    # in place
+    assert torch.equal(x, want)
+    assert native.device_status() == 0
