@@ -11,6 +11,12 @@
 //   attn_fwd_tm_kernel, attn_fwd_split_kernel   forward of short rows of head size 128, two maxima per row (see kSplitRows)
 // The first three are also compiled for query heads that share key / value heads (X >= 1) and for rows with lengths (X == 2), at the end
 // of the file; attn_plan_kernel lists the work of rows with lengths, attn_bwd_join_kernel adds up dK and dV of items in parts.
+// All of them run at the 168 registers that setmaxnreg's split gives.  Spills (bytes stored / loaded a thread): dQ of head size 64 none,
+// X = 1 40 / 68, X = 2 36 / 60; dK/dV of head size 128 4 / 20, 8 / 36 and 20 / 88; forward of head size 64 with X = 2 4 / 40; the others none.
+//
+// Rounded to bf16 on the way, because the operands of kind::f16 are 16 bits wide: P for P V and P^T dO, dS for dS K and dS^T Q, each
+// at most 2^-8 of a value.  Scores, maxima, sums, lse, delta and every accumulator are in 32 bits.  Gradients are 0.24 to 0.26 % from 64 bits
+// in norm (few keys: up to 0.35 %), of which the rounding of the results alone is 0.17 %.
 // Head size 128 also has earlier kernels with one CTA per work item, and with 64-wide tiles and P / dS in shared memory; they
 // run when MSAMP_ATTN_{FWD,BWD}_PERSIST=0 or MSAMP_ATTN_{FWD,BWD}_SMEM=1 and serve as a cross-check.
 //
@@ -3622,6 +3628,8 @@ __global__ void __launch_bounds__(128) attn_bwd_join_kernel(const JoinParams j) 
 // 128 x 128 (1.8 us): the longest item, or the mean over the SMs where that is more (items of one size: whole waves of them); parts add
 // the launch that joins them, two, and the writing and reading of their sums, one for 50 items of head size 128.  items: key tiles times
 // key / value heads; units: tiles of all of them; longest: tiles of the longest row.
+// A tile takes nearly the same time at both head sizes: dK / dV of 2 x 4096 x 16 / 4 heads of 64 217 us for 114 tiles an SM, of 4 x 2048 x 32 / 8
+// heads of 128 253 us for 118; what joining moves is half at 64.
 // Backward pass of 1 x 4096 x 16 / 1 heads of 128, causal, in 1, 2, 4, 8 and 16 parts: 1048, 591, 362, 249 and 259 us (8 chosen);
 // 2 x 1000 x 12 / 4 of 64 in 1 and 3: 73 and 54 (3); 2 x 2048 x 16 / 4 of 128 in 1, 2 and 4: 204, 156 and 169 (2); 4 x 2048 x 32 / 8 of 128
 // in 1, 2 and 4: 499, 542 and 579 (1); 2 x 2048 x 16 / 4 of 128, not causal: 247, 261 and 278 (1).
@@ -3866,6 +3874,7 @@ static bool has_repeats(const int64_t* strides, int tensors, int batch, int head
 //   64    384       1.1/1.1  0.9/0.8  0.9/0.6        0.8/0.7  0.5/0.4  0.6/0.5
 //   128   16        1.1/1.1  1.1/1.2  1.1/1.1        1.3/1.3  1.3/1.3  1.5/1.5
 //   128   64        1.1/1.2  1.2/1.2  1.1/1.2        1.1/1.1  1.1/1.0  1.1/1.0
+// (backward of up to 64 rows with the delta kernel that mma.sync has lost there since: its time is 12 to 25 % less, the ratios are higher)
 // Above 64 rows the line depends on how many of the persistent kernels' items (128-row tiles) there are for each SM.  Head size 128
 // stays on tcgen05 there: its rows are split into two running maxima, which mma.sync does not do (see kSplitRows).
 static bool short_rows(int seqlen, int head_dim, int64_t heads, bool backward) {

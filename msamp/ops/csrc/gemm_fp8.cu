@@ -121,9 +121,11 @@ __device__ __forceinline__ void colsum_chunk(float* cs, const float (&v)[32], in
     if (j < valid) atomicAdd(cs + j, to_f32<OutT>(from_f32<OutT>(v[j])));
 }
 
-// A thread of the epilogue holds 32 columns of a row, which is one block: its values' largest magnitude needs no exchange.  A GPT step of four
-// layers of hidden size 4096 (8192 tokens) takes 29.4 to 29.8 ms with the blocks written and read here, 29.5 to 30.0 with passes of
-// their own and 29.2 with h in 16 bits.
+// A thread of the epilogue holds 32 columns of a row, which is one block: its values' largest magnitude needs no exchange.  8192 x 16384 x 4096,
+// bf16: fc1 with GeLU in FP8 529 us with h in 16 bits, 600 with the blocks written here in the place of h, 595 with h and a pass over it (what
+// is saved here is the memory of h, not time); the dgrad that takes the GeLU slope 553 us from h, 574 from the blocks, 615 with a pass
+// before it.  A GPT step of four layers of hidden size 4096 (8192 tokens) takes 29.4 to 29.8 ms with the blocks written and read here,
+// 29.5 to 30.0 with passes of their own and 29.2 with h in 16 bits.
 template <typename OutT>
 __device__ __forceinline__ void keep_block(uint8_t* codes, uint8_t* exp, const float (&v)[32]) {
   using namespace blocks8;

@@ -91,9 +91,12 @@ struct Slot {
 };
 
 // The CTA's work is a list of (token, head, slot); a thread takes every 256th and counts up in mixed radix instead of dividing.  Its first
-// loads are under way while the angles are worked out.  Six CTAs an SM (42 registers, no spills) and two loads in flight a thread measure the
-// same (L2 flushed before each call): 8192 tokens x 40 heads of 128, bf16, 39 us, interleaved 43 to 45, half of each head 41 to 43; a copy
-// of the same bytes takes 33 us.  With divisions for every item it took 37, 53 and 51 us.
+// loads are under way while the angles are worked out.  Six CTAs an SM (40 registers; the interleaved vector forms spill one of them, 4 bytes
+// in and out) and two loads in flight a thread measure the same (L2 flushed before each call): 8192 tokens x 40 heads of 128, bf16, 39 us,
+// interleaved 43, half of each head 41; a copy of the same bytes takes 33 us.  With divisions for every item it took 37, 53 and 51 us.
+// Far from memory's time: narrow parts.  Where half of the part is no whole number of vectors, everything goes one element at a time, what
+// is only copied as well (6000 tokens x 32 heads of 80, part 20, bf16: 62 us, a copy 16); with vectors but few of them a CTA is mostly its
+// chain of offsets, barrier, angles, barrier, store (3069 tokens x 24 heads of 64, part 16, fp16: 10 us for the 3 of its bytes).
 template <typename T, bool INTER, bool VEC>
 __global__ void __launch_bounds__(kThreads, 6) rotary_kernel(const RotParams p) {
   extern __shared__ float2 s_cs[];    // [per_cta][half] cosine, signed sine
