@@ -614,3 +614,16 @@ def test_offsets_beyond_32_bits(lengths):
     got = _run(*x.split([nh, nkv, nkv], 2), do, True, n)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     _status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason='needs two GPUs')
+@pytest.mark.parametrize('lengths', [None, (150, 70)])
+def test_tensors_of_another_device_than_the_current_one(lengths):
+    q, k, v, do = _inputs(2, 150, 4, 2, 64, 'cuda:1')
+    n = None if lengths is None else torch.tensor(lengths, device='cuda:1')
+    assert torch.cuda.current_device() == 0
+    want, valid = _reference(q, k, v, do, True, n, 64**-0.5)
+    _compare(_run(q, k, v, do, True, n), want, valid)
+    with pytest.raises(ValueError):
+        K.attention(q, k, v, lengths=torch.tensor([150, 70], device='cuda:0'))
